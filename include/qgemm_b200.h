@@ -273,6 +273,127 @@ qgemm_status_t qgemm_umma_status(int32_t* faulted);
  * capturable. */
 qgemm_status_t qgemm_clear_faults(void);
 
+/* ---- serving operators around the GEMMs -----------------------------------
+ * What a decoder layer needs between its W4A16 products: a paged KV cache in
+ * 8 bits (plan, append, attention) and the norms around a block.  No
+ * counterpart in the reference, which stops at the GEMMs.  The same
+ * conventions hold: device pointers, caller-owned buffers, stream-ordered,
+ * capturable, errors decided on the host before any launch.
+ *
+ * The cache is a pool of blocks.  A block holds `block` consecutive tokens of
+ * one request for every KV head; codes lie [blocks][heads][block][head_dim],
+ * one E8M0 scale byte (2^(byte - 127)) per (block, head) beside them, for K
+ * and for V.  A request's row of the block table names its blocks in order.  */
+typedef enum { QGEMM_KV_E4M3 = 0, QGEMM_KV_INT8 = 1 } qgemm_kv_type_t;
+typedef struct {
+  int32_t type;       /* qgemm_kv_type_t                                     */
+  int32_t block;      /* tokens in a block: 16, 32, 64 or 128                */
+  int32_t heads;      /* KV heads                                            */
+  int32_t head_dim;   /* 64 or 128                                           */
+  int64_t blocks;     /* blocks in the pool                                  */
+  uint8_t* k;         /* codes, 16-byte aligned                              */
+  uint8_t* v;
+  uint8_t* k_scales;  /* E8M0 bytes [blocks][heads]                          */
+  uint8_t* v_scales;
+} qgemm_kv_cache_t;
+
+/* Block tables and slot maps from the requests' lengths.  Request r holds
+ * lens[r] tokens and brings news[r] (negative: 0); its new tokens are rows
+ * starts[r] .. starts[r + 1] - 1 of the step's activations, starts being the
+ * exclusive prefix sum.  New blocks come off the end of the free list
+ * (free_list[*free_count - 1] first) in request order and go into
+ * table[r][ceil(lens[r] / block) ..].  A request is refused, and takes no
+ * block, if its length is negative, if its tokens exceed its row of the
+ * table or the `tokens` rows, or if the blocks its predecessors and itself
+ * need exceed the free ones (one that needs no new block is still served).
+ * Outputs: lens_out[r] (the length with the new tokens; a refused one's is
+ * unchanged), starts [requests + 1], for each of the `tokens` rows its slot
+ * (block id * block + place, -1 for rows of refused or no requests) and its
+ * position in its request (-1 likewise), runs [qgemm_kv_max_runs + 1]: the
+ * first row of each run of rows that share a block, in order, then the row
+ * count as end marks, and counts [4]: free blocks left, runs, rows, refused
+ * requests.  free_list and *free_count are not changed: the caller keeps
+ * counts[0] as the next call's free_count and pushes a finished request's
+ * blocks back behind it.  A null free_list is an empty one.  lens_out must not
+ * be lens.                                                                   */
+int32_t qgemm_kv_max_runs(int32_t requests, int32_t tokens, int32_t block);
+qgemm_status_t qgemm_kv_plan(int32_t block, int32_t requests, const int32_t* lens,
+                             const int32_t* news, int32_t* table, int32_t table_width,
+                             const int32_t* free_list, const int32_t* free_count,
+                             int32_t tokens, int32_t* lens_out, int32_t* starts,
+                             int64_t* slots, int32_t* positions, int32_t* runs,
+                             int32_t* counts, void* stream);
+
+/* Quantises the step's K and V rows (bf16 bits, [tokens][heads][head_dim],
+ * tokens *_stride and heads *_head_stride elements apart, head_dim values
+ * together; 16-byte aligned, strides multiples of 8) into their slots.  slots and runs
+ * as qgemm_kv_plan writes them (max_runs + 1 entries of runs).  A block's
+ * scale is the smallest power of two 2^e >= 2^-64 with max|x| <= 448 * 2^e
+ * (E4M3) or 127 * 2^e (INT8) over its tokens; when new tokens raise it, the
+ * codes already in the block are rescaled with it.  Codes round to nearest
+ * even; infinities saturate and do not count for the scale; NaN is stored as
+ * 0.  Rows with slots outside the pool are skipped.                          */
+qgemm_status_t qgemm_kv_append(const qgemm_kv_cache_t* cache, const uint16_t* k,
+                               const uint16_t* v, int64_t k_stride, int64_t k_head_stride,
+                               int64_t v_stride, int64_t v_head_stride, int32_t tokens, const int64_t* slots, const int32_t* runs,
+                               int32_t max_runs, void* stream);
+
+/* Attention over the cache.  Request r has q rows starts[r] .. starts[r + 1]
+ * - 1 (bf16 bits, [tokens][q_heads][head_dim], tokens q_stride and heads
+ * q_head_stride elements apart) and lens[r] tokens in the cache, its new ones among them: row i of n is at
+ * position lens[r] - n + i and sees the tokens up to its own position
+ * (causal != 0, else all lens[r]) and, for window > 0, none further back than
+ * window - 1 before its own position.  q head h reads KV head
+ * h / (q_heads / cache->heads).  out (bf16 bits, [tokens][q_heads][head_dim])
+ * is softmax(scale * q.K) . V; a row that sees no token gets zeros.  lse
+ * (null or [tokens][q_heads] float): log of the sum of exp(scale * q.k) over
+ * the tokens it sees, -infinity where there is none.  max_new: a bound on the
+ * requests' row counts (rows past it are not computed).  Lengths above
+ * table_width * block are cut to it; tokens of a block id outside the pool
+ * read as zeros.  Rows beyond starts[requests] are left as they are.  head_dim
+ * values of q lie together, q is 16-byte aligned, its strides multiples of 8.
+ * workspace: qgemm_kv_attention_workspace() bytes, zeroed once
+ * (qgemm_workspace_init); every call returns its tickets to zero.            */
+size_t qgemm_kv_attention_workspace(const qgemm_kv_cache_t* cache, int32_t q_heads,
+                                    int32_t requests, int32_t tokens, int32_t max_new);
+qgemm_status_t qgemm_kv_attention(const qgemm_kv_cache_t* cache, const uint16_t* q,
+                                  int64_t q_stride, int64_t q_head_stride,
+                                  int32_t q_heads, int32_t requests,
+                                  const int32_t* starts, const int32_t* lens,
+                                  const int32_t* table, int32_t table_width,
+                                  int32_t tokens, int32_t max_new, float scale,
+                                  int32_t window, int32_t causal, uint16_t* out,
+                                  float* lse, void* workspace, size_t ws_bytes,
+                                  void* stream);
+
+/* The norms around a block with its gate and residual scale, row by row:
+ *   residual_out = residual + alpha * gate * N(y; post, post_bias)
+ *   h            = N(residual_out; pre, pre_bias)        (before rounding it)
+ * N is x * rsqrt(mean(x^2) + eps) * weight (QGEMM_NORM_RMS) or the same of
+ * x - mean(x) plus a bias (QGEMM_NORM_LAYER).  y, weights, biases, gate and h
+ * are bf16 bits; residual and residual_out bf16 bits, or float with
+ * residual_f32.  A null post leaves y as it is, a null gate is 1, a null bias
+ * 0; gate is [tokens][width] with gate_stride elements between rows, or one
+ * row for all with gate_stride 0.  With y null, h is the norm of residual and
+ * residual_out is not written (post, gate must be null).  With pre null, h is
+ * not written.  residual_out may be residual, and h may be y.
+ * width: a multiple of 8, at most 16384; rows 16-byte aligned.               */
+typedef enum { QGEMM_NORM_RMS = 0, QGEMM_NORM_LAYER = 1 } qgemm_norm_kind_t;
+typedef struct {
+  int32_t kind;               /* qgemm_norm_kind_t                           */
+  int32_t tokens, width;
+  int32_t residual_f32;       /* residual and residual_out are float         */
+  const uint16_t* y;          /* the block's output, or null                 */
+  const void* residual;
+  const uint16_t *post, *post_bias, *gate;
+  int64_t gate_stride;
+  const uint16_t *pre, *pre_bias;
+  float alpha, eps;
+  void* residual_out;
+  uint16_t* h;
+} qgemm_residual_norm_t;
+qgemm_status_t qgemm_residual_norm(const qgemm_residual_norm_t* a, void* stream);
+
 /* ---- baselines and probes (bench harness; not on the product path) ------- */
 /* cuBLAS BF16 dense Y[M,N] = X[M,K] . W[N,K]^T (bench_cublas.cu:144-151 with
  * CUDA_R_16BF in place of CUDA_R_16F, COMPUTE_32F). */

@@ -97,8 +97,6 @@ _sig("qgemm_ipc_handle", _i32, [C.c_void_p, C.POINTER(C.c_uint8), C.POINTER(_sz)
 _sig("qgemm_ipc_open", _i32, [C.POINTER(C.c_uint8), C.POINTER(C.c_void_p)])
 _sig("qgemm_ipc_close", _i32, [C.c_void_p])
 
-EXPORTED = [n for n in dir(_lib) if n.startswith("qgemm_")]
-
 
 class QGemmError(RuntimeError):
     def __init__(self, status: int, where: str):
@@ -560,3 +558,11 @@ def device_info() -> tuple[int, int]:
     sm, l2 = _i32(0), _sz(0)
     _check(_lib.qgemm_device_info(C.byref(sm), C.byref(l2)), "device_info")
     return sm.value, l2.value
+
+
+# ---- serving operators (serving.py) ---------------------------------------------
+
+from .serving import (KV_E4M3, KV_INT8, KVCache, KVPlan, kv_append, kv_attention,  # noqa: E402
+                      kv_attention_workspace, kv_plan, make_kv_cache, make_kv_workspace, residual_norm)
+
+EXPORTED = [n for n in dir(_lib) if n.startswith("qgemm_")]

@@ -1,0 +1,233 @@
+// kv_plan.cu -- block tables and slot maps of a paged KV cache, built on the
+// GPU from the requests' lengths (no counterpart in titoatwork/qgemm-mx, which
+// stops at the GEMMs).
+//
+// With P tokens per block, request r holding len_r tokens and bringing n_r:
+//   starts = exclusive prefix sum of n
+//   need_r = ceil((len_r + n_r) / P) - ceil(len_r / P)   new blocks
+//   upto_r = inclusive prefix sum of need
+// and r's j-th new block is free_list[count - 1 - (upto_r - need_r + j)]: the
+// free list is a stack, taken from its end in request order.
+//
+// What bounds it: latency.  A step's lengths are a few KB and its slot map 12
+// bytes a token; the dependent chain is lengths -> scan -> block id -> slot.
+// So it is one launch: every CTA scans all requests itself (chunks of 1024
+// from L2) instead of waiting for another CTA's prefix, and then fills its own
+// range of 256-token rows, finding each token's request by binary search in
+// shared memory.
+#include "kv.cuh"
+
+namespace qg {
+
+constexpr int kPlanThreads = 256;
+constexpr int kPlanItems = 4;                          // requests per thread and chunk
+constexpr int kPlanChunk = kPlanThreads * kPlanItems;
+
+struct PlanArgs {
+  const int32_t *lens, *news;
+  int32_t* table;
+  const int32_t *free_list, *free_count;
+  int32_t requests, width, block_log2, tokens, max_runs;
+  int32_t *lens_out, *starts;
+  int64_t* slots;
+  int32_t *positions, *runs, *counts;
+};
+
+// One request's sizes.
+struct PlanSize {
+  int len, n, have, need, touched;
+  bool fits;  // its tokens fit its row of the table
+};
+// Blocks that n tokens after the first len touch.
+__device__ __forceinline__ int runs_of(int len, int n, int lg) {
+  return n > 0 ? (int)(((long long)len + n - 1) >> lg) - (len >> lg) + 1 : 0;
+}
+__device__ __forceinline__ PlanSize plan_size(int len, int n, int width, int lg) {
+  PlanSize s;
+  const int P1 = (1 << lg) - 1;
+  s.len = max(len, 0);
+  s.n = max(n, 0);
+  s.have = (int)(((long long)s.len + P1) >> lg);
+  const long long last = ((long long)s.len + s.n + P1) >> lg;
+  s.fits = last <= width && len >= 0;
+  s.need = s.fits ? (int)last - s.have : 0;
+  s.touched = runs_of(s.len, s.n, lg);
+  return s;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) k_kv_plan(const PlanArgs a) {
+  __shared__ int s_start[kPlanChunk + 1], s_upto[kPlanChunk], s_run[kPlanChunk], s_len[kPlanChunk];
+  __shared__ int s_warp[3][kPlanThreads / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int lg = a.block_log2;
+  const int count = a.free_list ? max(*a.free_count, 0) : 0;
+  // this CTA's rows
+  const int t0 = (int)((long long)blockIdx.x * a.tokens / gridDim.x);
+  const int t1 = (int)((long long)(blockIdx.x + 1) * a.tokens / gridDim.x);
+  long long base_tok = 0;
+  int base_need = 0, base_run = 0;  // needs stop mattering past `count`, so they saturate below
+  int used = 0, refused = 0, leads = 0;
+  for (int r0 = 0; r0 < a.requests; r0 += kPlanChunk) {
+    PlanSize z[kPlanItems];
+    long long tok = 0;
+    int need = 0, run = 0;
+#pragma unroll
+    for (int i = 0; i < kPlanItems; ++i) {
+      const int r = r0 + tid * kPlanItems + i;
+      z[i] = r < a.requests ? plan_size(a.lens[r], a.news[r], a.width, lg) : PlanSize{0, 0, 0, 0, 0, true};
+      tok += z[i].n; need += z[i].need; run += z[i].touched;
+    }
+    // Sums saturate at 2^30: rows past `tokens` are never written.
+    int sums[3] = {(int)min(tok, (long long)kKvMaxTokens), min(need, kKvMaxTokens), min(run, kKvMaxTokens)};
+    int incl[3];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      int v = sums[k];
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int u = __shfl_up_sync(0xFFFFFFFFu, v, d);
+        if (lane >= d) v = min(v + u, kKvMaxTokens);
+      }
+      incl[k] = v;
+      if (lane == 31) s_warp[k][warp] = v;
+    }
+    __syncthreads();
+    int before[3], total[3];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      int b = 0, t = 0;
+#pragma unroll
+      for (int w = 0; w < kPlanThreads / 32; ++w) {
+        if (w == warp) b = t;
+        t = min(t + s_warp[k][w], kKvMaxTokens);
+      }
+      const int up = __shfl_up_sync(0xFFFFFFFFu, incl[k], 1);
+      before[k] = min(b + (lane ? up : 0), kKvMaxTokens);
+      total[k] = t;
+    }
+    long long at = base_tok + before[0];
+    int upto = min(base_need + before[1], kKvMaxTokens), runs = min(base_run + before[2], kKvMaxTokens);
+#pragma unroll
+    for (int i = 0; i < kPlanItems; ++i) {
+      const int j = tid * kPlanItems + i, r = r0 + j;
+      upto = min(upto + z[i].need, kKvMaxTokens);
+      const bool granted = z[i].fits && at + z[i].n <= a.tokens && (z[i].need == 0 || upto <= count);
+      s_start[j] = (int)min(at, (long long)kKvMaxTokens);
+      s_upto[j] = granted ? upto - z[i].need : -1;
+      s_run[j] = runs;
+      s_len[j] = z[i].len;
+      if (r < a.requests) {
+        leads += runs_of(z[i].len, (int)min((long long)z[i].n, max(a.tokens - at, 0ll)), lg);  // of rows that exist
+        if (granted) used = max(used, upto);
+        else ++refused;
+        if (blockIdx.x == 0) {
+          a.starts[r] = s_start[j];
+          a.lens_out[r] = granted ? z[i].len + z[i].n : a.lens[r];
+        }
+      }
+      at = min(at + z[i].n, (long long)kKvMaxTokens);
+      runs = min(runs + z[i].touched, kKvMaxTokens);
+    }
+    base_tok = min(base_tok + total[0], (long long)kKvMaxTokens);
+    if (tid == kPlanThreads - 1) s_start[kPlanChunk] = (int)base_tok;
+    base_need = min(base_need + total[1], kKvMaxTokens);
+    base_run = min(base_run + total[2], kKvMaxTokens);
+    __syncthreads();
+    // tokens of this chunk in this CTA's range
+    const int lo = max(t0, s_start[0]), hi = min(t1, s_start[kPlanChunk]);
+    for (int t = lo + tid; t < hi; t += kPlanThreads) {
+      int b = 0;  // the last request with start <= t: empty requests share a start with the next
+#pragma unroll
+      for (int step = kPlanChunk / 2; step; step >>= 1)
+        if (s_start[b + step] <= t) b += step;
+      const int r = r0 + b, len = s_len[b];
+      const int at_t = len + (t - s_start[b]), blk = at_t >> lg, off = at_t & ((1 << lg) - 1);
+      const int taken = s_upto[b];
+      int64_t slot = -1;
+      if (taken >= 0) {
+        const int have = (len + (1 << lg) - 1) >> lg;
+        int id;
+        if (blk < have) {
+          id = a.table[(size_t)r * a.width + blk];
+        } else {
+          id = a.free_list[count - 1 - (taken + blk - have)];
+          if (off == 0) a.table[(size_t)r * a.width + blk] = id;  // a new block starts with a new token
+        }
+        slot = ((int64_t)id << lg) + off;
+      }
+      a.slots[t] = slot;
+      a.positions[t] = taken >= 0 ? at_t : -1;
+      if (t == s_start[b] || off == 0) {
+        const int k = s_run[b] + blk - (len >> lg);
+        if (k < a.max_runs) a.runs[k] = t;
+      }
+    }
+    __syncthreads();
+  }
+  // rows no request covers, the runs' end marks, and the totals
+  const int total = (int)min(base_tok, (long long)a.tokens);
+  for (int t = max(t0, total) + tid; t < t1; t += kPlanThreads) {
+    a.slots[t] = -1;
+    a.positions[t] = -1;
+  }
+  if (blockIdx.x != 0) return;
+  __shared__ int s_used, s_refused, s_leads;
+  if (tid == 0) { s_used = 0; s_refused = 0; s_leads = 0; }
+  __syncthreads();
+  if (used) atomicMax(&s_used, used);
+  if (refused) atomicAdd(&s_refused, refused);
+  if (leads) atomicAdd(&s_leads, leads);
+  __syncthreads();
+  for (int k = s_leads + tid; k <= a.max_runs; k += kPlanThreads) a.runs[k] = total;
+  if (tid == 0) {
+    a.starts[a.requests] = (int)base_tok;
+    a.counts[0] = count - s_used;
+    a.counts[1] = s_leads;
+    a.counts[2] = total;
+    a.counts[3] = s_refused;
+  }
+}
+
+}  // namespace qg
+
+using namespace qg;
+
+extern "C" {
+
+int32_t qgemm_kv_max_runs(int32_t requests, int32_t tokens, int32_t block) {
+  if (requests < 0 || tokens < 0 || !kv_block_ok(block)) return -1;
+  const long long b = 2ll * requests + tokens / block;
+  return (int32_t)(b < tokens ? b : tokens);
+}
+
+qgemm_status_t qgemm_kv_plan(int32_t block, int32_t requests, const int32_t* lens, const int32_t* news,
+                             int32_t* table, int32_t table_width, const int32_t* free_list,
+                             const int32_t* free_count, int32_t tokens, int32_t* lens_out, int32_t* starts,
+                             int64_t* slots, int32_t* positions, int32_t* runs, int32_t* counts, void* stream) {
+  if (!kv_block_ok(block)) return fail(QGEMM_ERR_INVALID_ARG, "kv_plan: block must be 16, 32, 64 or 128 tokens");
+  if (requests < 0 || tokens < 0 || table_width < 0)
+    return fail(QGEMM_ERR_INVALID_ARG, "kv_plan: negative size");
+  if (tokens >= kKvMaxTokens) return fail(QGEMM_ERR_INVALID_ARG, "kv_plan: at most 2^30 - 1 rows");
+  if (!free_count || !starts || !runs || !counts || (requests && (!lens || !news || !lens_out)) ||
+      (requests && table_width && !table) || (tokens && (!slots || !positions)))
+    return fail(QGEMM_ERR_INVALID_ARG, "kv_plan: null pointer");
+  if (lens_out && lens_out == lens)
+    return fail(QGEMM_ERR_INVALID_ARG, "kv_plan: lens_out must not be lens: CTAs read lens while others write");
+  PlanArgs a;
+  a.lens = lens; a.news = news; a.table = table; a.free_list = free_list; a.free_count = free_count;
+  a.requests = requests; a.width = table_width; a.tokens = tokens;
+  a.block_log2 = block == 16 ? 4 : block == 32 ? 5 : block == 64 ? 6 : 7;
+  a.max_runs = qgemm_kv_max_runs(requests, tokens, block);
+  a.lens_out = lens_out; a.starts = starts; a.slots = slots; a.positions = positions; a.runs = runs;
+  a.counts = counts;
+  DevProps dp;
+  qgemm_status_t st = device_props(&dp);
+  if (st != QGEMM_OK) return st;
+  int grid = (tokens + kPlanThreads - 1) / kPlanThreads;
+  grid = grid < 1 ? 1 : grid > dp.sm_count ? dp.sm_count : grid;
+  k_kv_plan<<<grid, kPlanThreads, 0, as_stream(stream)>>>(a);
+  QG_LAUNCH_RET();
+  return QGEMM_OK;
+}
+
+}  // extern "C"
