@@ -19,6 +19,8 @@
 
 namespace qg {
 
+constexpr int kKvMaxRequests = 2048;  // per launch: the line's prefix sums live in shared memory
+
 struct KvAttnArgs {
   const uint8_t *k, *v, *ks, *vs;
   const uint16_t* q;
@@ -28,6 +30,7 @@ struct KvAttnArgs {
   int64_t blocks;
   int requests, tokens, heads, group;  // group: query heads per KV head
   int max_new;
+  int rows_min, rows_max;  // rows per KV head of the requests this launch takes
   float scale_log2;  // scale * log2(e)
   int window, causal;
   uint16_t* out;
@@ -45,6 +48,11 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&b);
+}
+
 // Tokens row i of n sees: [lo, hi).
 __device__ __forceinline__ int row_hi(const KvAttnArgs& a, int len, int n, int i) {
   return a.causal ? min(max(len - n + i + 1, 0), len) : len;
@@ -53,8 +61,10 @@ __device__ __forceinline__ int row_lo(const KvAttnArgs& a, int len, int n, int i
   return a.window > 0 ? (int)max((long long)len - n + i - a.window + 1, 0ll) : 0;
 }
 
-// A request's rows and length as the kernels take them (rows past max_new or
-// past the row count are not computed, lengths end with the table).
+// A request's rows and length as the kernels take them: rows past max_new or
+// past the row count are not computed, lengths end with the table, and a
+// request whose rows per KV head are not in (rows_min, rows_max] belongs to
+// the other kernel and has none here.
 struct KvRequest {
   int start, n, len, n_all;
 };
@@ -63,9 +73,135 @@ __device__ __forceinline__ KvRequest kv_request(const KvAttnArgs& a, int r) {
   q.start = a.starts[r];
   q.n_all = a.starts[r + 1] - q.start;
   q.n = min(min(q.n_all, a.max_new), a.tokens - q.start);
-  if (q.start < 0 || q.n < 0) q.n = 0;
+  const long long rows = (long long)q.n * a.group;
+  if (q.start < 0 || q.n < 0 || rows <= a.rows_min || rows > a.rows_max) q.n = 0;
   q.len = (int)min((long long)max(a.lens[r], 0), (long long)a.width << a.block_log2);
   return q;
+}
+
+// ---- the line: all pairs' tiles, one after another ---------------------------
+// A pair is (request, KV head, group of RG rows); its tokens are tiles of
+// T = 2^TL.  The line gives group g of a request S(g + 1) - S(g) places,
+//   S(g) = floor(sum over k < g of (h0 + (k + 1) slope) / T + 1),
+// where h0 + (g + 1) slope bounds the tokens the group sees: slope is RG / group
+// tokens for causal rows, 0 otherwise.  floor(a + x) - floor(a) >= floor(x), so
+// the places suffice for the group's tiles; the spare one stands for the cost
+// of starting a pair.  A closed form keeps causal prompts balanced (their
+// groups see from few to all tokens) without a list of groups.
+template <int RG, int TL>
+struct KvLine {
+  long long c0, c1, den;  // S(g) = (c0 g + c1 g (g + 1)) / den
+  int groups;
+  __device__ __forceinline__ KvLine(const KvAttnArgs& a, const KvRequest& q) {
+    long long h0 = q.len, slope = 0;
+    if (a.causal) {
+      h0 = max(q.len - q.n_all, 0) + 1;
+      slope = RG;
+      const int span = min(q.n, (RG + a.group - 2) / a.group + 1);  // tokens of one group
+      if (a.window > 0 && (long long)a.window + span - 1 + (1 << TL) < q.len) {
+        h0 = (long long)a.window + span - 1 + (1 << TL);
+        slope = 0;
+      }
+    }
+    c0 = 2 * a.group * (h0 + (1 << TL));
+    c1 = slope;
+    den = (2ll * a.group) << TL;
+    groups = (q.n * a.group + RG - 1) / RG;
+  }
+  __device__ __forceinline__ int upto(int g) const { return (int)((c0 * g + c1 * g * (g + 1ll)) / den); }
+};
+
+// One stretch of one pair's tiles.
+struct KvSeg {
+  int pair_v, pair_end;  // the pair's range on the line
+  int r, h, row0, rows;  // rows: the request's n * group
+  int start, n, n_all, len;
+  int tile, tile_end;    // absolute tiles to visit
+};
+
+template <int RG, int TL>
+__device__ __forceinline__ void kv_seg(const KvAttnArgs& a, const int* prefix, int& r, int v, int v_end, KvSeg& s) {
+  while (prefix[r + 1] <= v) ++r;
+  const KvRequest q = kv_request(a, r);
+  const KvLine<RG, TL> line(a, q);
+  const int per_head = line.upto(line.groups);
+  s.r = r;
+  s.h = (v - prefix[r]) / per_head;
+  const int head_v = prefix[r] + s.h * per_head;
+  int g = 0;
+  for (int hi = line.groups; hi - g > 1;) {
+    const int mid = (g + hi) >> 1;
+    if (head_v + line.upto(mid) <= v) g = mid; else hi = mid;
+  }
+  s.row0 = g * RG;
+  s.rows = q.n * a.group;
+  s.start = q.start; s.n = q.n; s.n_all = q.n_all; s.len = q.len;
+  s.pair_v = head_v + line.upto(g);
+  s.pair_end = head_v + line.upto(g + 1);
+  const int i0 = s.row0 / a.group, i1 = (min(s.row0 + RG, s.rows) - 1) / a.group;
+  const int lo = row_lo(a, q.len, q.n_all, i0) >> TL;
+  const int hi = (int)(((long long)row_hi(a, q.len, q.n_all, i1) + (1 << TL) - 1) >> TL);
+  s.tile = lo + (v - s.pair_v);
+  s.tile_end = min(hi, lo + min(s.pair_end, v_end) - s.pair_v);
+}
+
+// Most places one request can take on the line (host).
+inline long long kv_line_most(const KvAttnArgs& a, int rg, int tl) {
+  const long long rows = (long long)a.max_new * a.group < a.rows_max ? (long long)a.max_new * a.group : a.rows_max;
+  const long long groups = (rows + rg - 1) / rg;
+  const long long tokens = ((long long)a.width << a.block_log2) + a.max_new + rg + (2ll << tl);
+  const long long per_head = groups * ((tokens >> tl) + 2);
+  return per_head > (1ll << 40) ? per_head : per_head * a.heads;
+}
+
+// The request whose pairs hold line position v (empty ones hold none).
+__device__ __forceinline__ int kv_find(const int* prefix, int requests, int v) {
+  int lo = 0, hi = requests;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (prefix[mid] <= v) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// The line's prefix sums (exclusive, prefix[requests] = its length) by a CTA of
+// at least WARPS warps; the first WARPS take part, all threads must call it.
+template <int RG, int TL, int WARPS>
+__device__ __forceinline__ int kv_line(const KvAttnArgs& a, int* prefix, int* scan) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int base = 0;
+  for (int r0 = 0; r0 < a.requests; r0 += WARPS * 32) {
+    const int r = r0 + tid;
+    const bool on = tid < WARPS * 32 && r < a.requests;
+    int c = 0;
+    if (on) {
+      const KvRequest q = kv_request(a, r);
+      if (q.n > 0) {
+        const KvLine<RG, TL> line(a, q);
+        c = a.heads * line.upto(line.groups);
+      }
+    }
+    int v = c;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int u = __shfl_up_sync(0xFFFFFFFFu, v, d);
+      if (lane >= d) v += u;
+    }
+    if (lane == 31 && warp < WARPS) scan[warp] = v;
+    __syncthreads();
+    int before = base, total = base;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      if (w == warp) before = total;
+      total += scan[w];
+    }
+    if (on) prefix[r] = before + v - c;
+    base = total;
+    __syncthreads();
+  }
+  if (tid == 0) prefix[a.requests] = base;
+  __syncthreads();
+  return base;
 }
 
 }  // namespace qg

@@ -30,7 +30,6 @@
 namespace qg {
 
 constexpr int kDecWarps = 8;
-constexpr int kDecMaxRequests = 2048;  // per launch: the line's prefix sums live in shared memory
 constexpr int kDecMinTiles = 2;        // tiles per warp below which the grid shrinks
 
 template <int HD, int NT>
@@ -71,101 +70,20 @@ __device__ __forceinline__ uint2 lds8(uint32_t p) {
   return v;
 }
 
-// Tiles each pair of a request takes on the line (the same for its row
-// groups, by a bound on what one group sees), and its number of groups.
-template <int RG>
-__device__ __forceinline__ int dec_tiles(const KvAttnArgs& a, const KvRequest& q) {
-  int t = (q.len + 15) >> 4;
-  if (a.window > 0 && a.causal) {
-    const int span = min(q.n, (RG + a.group - 2) / a.group + 1);
-    t = (int)min((long long)t, ((long long)a.window + span + 14) / 16 + 1);
-  }
-  return max(t, 1);
-}
-template <int RG>
-__device__ __forceinline__ int dec_groups(const KvAttnArgs& a, const KvRequest& q) {
-  return (q.n * a.group + RG - 1) / RG;
-}
-
-// One stretch of one pair's tiles.
-struct DecSeg {
-  int pair_v, pair_end;  // the pair's range on the line
-  int r, h, row0, rows;  // rows: the request's n * group
-  int start, n, n_all, len;
-  int tile, tile_end;    // absolute tiles to visit
-};
-
-template <int RG>
-__device__ __forceinline__ void dec_seg(const KvAttnArgs& a, const int* prefix, int& r, int v, int v_end, DecSeg& s) {
-  while (prefix[r + 1] <= v) ++r;
-  const KvRequest q = kv_request(a, r);
-  const int tiles = dec_tiles<RG>(a, q), groups = dec_groups<RG>(a, q);
-  const int pair = (v - prefix[r]) / tiles;
-  s.r = r;
-  s.h = pair / groups;
-  s.row0 = (pair - s.h * groups) * RG;
-  s.rows = q.n * a.group;
-  s.start = q.start; s.n = q.n; s.n_all = q.n_all; s.len = q.len;
-  s.pair_v = prefix[r] + pair * tiles;
-  s.pair_end = s.pair_v + tiles;
-  const int i0 = s.row0 / a.group, i1 = (min(s.row0 + RG, s.rows) - 1) / a.group;
-  const int lo = row_lo(a, q.len, q.n_all, i0) >> 4, hi = (row_hi(a, q.len, q.n_all, i1) + 15) >> 4;
-  s.tile = lo + (v - s.pair_v);
-  s.tile_end = min(hi, lo + min(s.pair_end, v_end) - s.pair_v);
-}
-
-// The request whose pairs hold line position v (empty ones hold none).
-__device__ __forceinline__ int dec_find(const int* prefix, int requests, int v) {
-  int lo = 0, hi = requests;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (prefix[mid] <= v) lo = mid; else hi = mid;
-  }
-  return lo;
-}
-
 template <int TYPE, int HD, int NT>
 __global__ void __launch_bounds__(kDecWarps * 32, 1) k_kv_decode(const KvAttnArgs a) {
   using Cfg = DecCfg<HD, NT>;
   constexpr int RG = 8 * NT, CPR = HD / 16, KJ = HD / 64, MT = HD / 16, ST = Cfg::kStages;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int s_prefix[kDecMaxRequests + 1];
+  __shared__ int s_prefix[kKvMaxRequests + 1];
   __shared__ int s_scan[kDecWarps];
   __shared__ int2 s_part[kDecWarps][2];  // the pair range each partial belongs to
   __shared__ unsigned s_ticket;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
 
-  // The line: exclusive prefix sums of the requests' tiles.
-  int base = 0;
-  for (int r0 = 0; r0 < a.requests; r0 += kDecWarps * 32) {
-    const int r = r0 + tid;
-    int c = 0;
-    if (r < a.requests) {
-      const KvRequest q = kv_request(a, r);
-      if (q.n > 0) c = a.heads * dec_groups<RG>(a, q) * dec_tiles<RG>(a, q);
-    }
-    int v = c;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int u = __shfl_up_sync(0xFFFFFFFFu, v, d);
-      if (lane >= d) v += u;
-    }
-    if (lane == 31) s_scan[warp] = v;
-    __syncthreads();
-    int before = base, total = base;
-#pragma unroll
-    for (int w = 0; w < kDecWarps; ++w) {
-      if (w == warp) before = total;
-      total += s_scan[w];
-    }
-    if (r < a.requests) s_prefix[r] = before + v - c;
-    base = total;
-    __syncthreads();
-  }
-  if (tid == 0) s_prefix[a.requests] = base;
+  const int V = kv_line<RG, 4, kDecWarps>(a, s_prefix, s_scan);
   if (tid < 2 * kDecWarps) s_part[tid >> 1][tid & 1] = make_int2(-1, -1);
   __syncthreads();
-  const int V = base;
   const int E = max(1, min((int)gridDim.x * kDecWarps, V / kDecMinTiles));  // shares
   const int k0 = blockIdx.x * kDecWarps;
   if (V == 0 || k0 >= E) return;
@@ -181,16 +99,16 @@ __global__ void __launch_bounds__(kDecWarps * 32, 1) k_kv_decode(const KvAttnArg
   if (k0 + warp < E) {
     const int v0 = cut(k0 + warp), v1 = cut(k0 + warp + 1);
     // ---- producer state: runs ST tiles ahead of the arithmetic --------------
-    int p_v = v0, p_r = dec_find(s_prefix, a.requests, v0);
+    int p_v = v0, p_r = kv_find(s_prefix, a.requests, v0);
     int c_r = p_r;  // the arithmetic's place
-    DecSeg ps;
+    KvSeg ps;
     ps.tile = 0; ps.tile_end = 0; ps.pair_end = v0;
     int win = -1, win_id = 0;  // 32 block ids from `win` on, one per lane, and their exponents
     uint32_t win_meta = 0;
     const int lg = a.block_log2;
     auto issue = [&](int stage) {
       while (ps.tile >= ps.tile_end && p_v < v1) {
-        dec_seg<RG>(a, s_prefix, p_r, p_v, v1, ps);
+        kv_seg<RG, 4>(a, s_prefix, p_r, p_v, v1, ps);
         p_v = min(ps.pair_end, v1);
         win = -1;
       }
@@ -247,8 +165,8 @@ __global__ void __launch_bounds__(kDecWarps * 32, 1) k_kv_decode(const KvAttnArg
     int stage = 0;
     bool first = true;
     for (int v = v0; v < v1;) {
-      DecSeg s;
-      dec_seg<RG>(a, s_prefix, c_r, v, v1, s);
+      KvSeg s;
+      kv_seg<RG, 4>(a, s_prefix, c_r, v, v1, s);
       const int seg_v0 = v;
       v = min(s.pair_end, v1);
       // ---- queries: f16 fragments and score factors --------------------------
@@ -443,10 +361,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 1) k_kv_decode(const KvAttnArg
             const float f = l[nt][c] == 0.0f ? 0.0f : 1.0f / l[nt][c];
             uint32_t w[MT];
 #pragma unroll
-            for (int z = 0; z < MT; ++z) {
-              const __nv_bfloat162 b = __floats2bfloat162_rn(o[nt][z][c] * f, o[nt][z][2 + c] * f);
-              w[z] = *reinterpret_cast<const uint32_t*>(&b);
-            }
+            for (int z = 0; z < MT; ++z) w[z] = pack_bf16(o[nt][z][c] * f, o[nt][z][2 + c] * f);
             uint4* dst = reinterpret_cast<uint4*>(a.out + at * HD + g * MT * 2);
 #pragma unroll
             for (int z = 0; z < MT / 4; ++z) dst[z] = make_uint4(w[4 * z], w[4 * z + 1], w[4 * z + 2], w[4 * z + 3]);
@@ -500,18 +415,17 @@ __global__ void __launch_bounds__(kDecWarps * 32, 1) k_kv_decode(const KvAttnArg
     const bool whole = pr.x >= cta0 && pr.y <= cta1;
     const int c_first = share_of(pr.x) / kDecWarps, c_last = share_of(pr.y - 1) / kDecWarps;
     float* gp = a.partials + (size_t)(blockIdx.x * 2 + ((int)blockIdx.x == c_first ? 1 : 0)) * Cfg::kSlot;
-    DecSeg s;
-    int join_r = dec_find(s_prefix, a.requests, pr.x);
-    dec_seg<RG>(a, s_prefix, join_r, pr.x, pr.y, s);
+    KvSeg s;
+    int join_r = kv_find(s_prefix, a.requests, pr.x);
+    kv_seg<RG, 4>(a, s_prefix, join_r, pr.x, pr.y, s);
     auto finish = [&](int e4, float4 acc, float M, float L) {
       const int qr = e4 * 4 / HD, d = e4 * 4 % HD, row = s.row0 + qr;
       if (row >= s.rows) return;
       const int i = row / a.group, gh = row - i * a.group;
       const int64_t at = (int64_t)(s.start + i) * a.heads * a.group + s.h * a.group + gh;
       const float f = L == 0.0f ? 0.0f : 1.0f / L;
-      const __nv_bfloat162 b0 = __floats2bfloat162_rn(acc.x * f, acc.y * f), b1 = __floats2bfloat162_rn(acc.z * f, acc.w * f);
       *reinterpret_cast<uint2*>(a.out + at * HD + d) =
-          make_uint2(*reinterpret_cast<const uint32_t*>(&b0), *reinterpret_cast<const uint32_t*>(&b1));
+          make_uint2(pack_bf16(acc.x * f, acc.y * f), pack_bf16(acc.z * f, acc.w * f));
       if (a.lse && d == 0) a.lse[at] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
     };
     for (int e4 = tid; e4 < RG * HD / 4; e4 += kDecWarps * 32) {
@@ -594,40 +508,58 @@ static cudaError_t launch_decode(const KvAttnArgs& a, int grid, cudaStream_t s) 
 }
 
 // Two row tiles of 8 when a request brings more than 8 rows per KV head.
-static int dec_nt(int group, int max_new) { return (long long)group * max_new > 8 ? 2 : 1; }
+static int dec_nt(long long rows) { return rows > 8 ? 2 : 1; }
 
-size_t kv_decode_workspace(const qgemm_kv_cache_t* c, int group, int max_new, int sm_count) {
-  const size_t slot = (size_t)8 * dec_nt(group, max_new) * (c->head_dim + 2) * sizeof(float);
-  return 4096 + (size_t)sm_count * 2 * slot;
+cudaError_t kv_decode_launch(int type, int head_dim, int nt, const KvAttnArgs& a, int grid, cudaStream_t s) {
+#define QG_DEC(T_, H_) nt == 1 ? launch_decode<T_, H_, 1>(a, grid, s) : launch_decode<T_, H_, 2>(a, grid, s)
+  if (type == QGEMM_KV_E4M3) return head_dim == 64 ? QG_DEC(QGEMM_KV_E4M3, 64) : QG_DEC(QGEMM_KV_E4M3, 128);
+  return head_dim == 64 ? QG_DEC(QGEMM_KV_INT8, 64) : QG_DEC(QGEMM_KV_INT8, 128);
+#undef QG_DEC
 }
 
-qgemm_status_t kv_decode(const qgemm_kv_cache_t* c, KvAttnArgs a, void* ws, int sm_count, cudaStream_t s) {
-  const int nt = dec_nt(a.group, a.max_new);
-  a.tickets = static_cast<unsigned*>(ws);
-  a.partials = reinterpret_cast<float*>(static_cast<char*>(ws) + 4096);
-  // requests per launch: the prefix sums fit shared memory and the line 31 bits
-  const long long groups = ((long long)a.max_new * a.group + 8 * nt - 1) / (8 * nt);
-  const long long tiles = ((long long)a.width << a.block_log2) / 16 + 1;
-  const long long per = groups * a.heads * tiles;
-  if (per > INT32_MAX) return fail(QGEMM_ERR_UNSUPPORTED_SHAPE, "kv_attention: rows x heads x tokens of a request exceed 2^31 tiles");
-  long long most = INT32_MAX / per;
-  if (most > kDecMaxRequests) most = kDecMaxRequests;
+size_t kv_prefill_workspace(int head_dim, int sm_count);
+cudaError_t kv_prefill_launch(int type, int head_dim, const KvAttnArgs& a, int grid, cudaStream_t s);
+
+// Requests with more rows per KV head than this run on the tcgen05 kernel.
+constexpr int kKvPrefillRows = 32;
+
+// Workspace: 4 KiB of tickets for each kernel, then their partials.
+struct KvWorkspace {
+  size_t decode, prefill, total;  // byte offsets of the partials
+  KvWorkspace(int head_dim, long long rows, int sm_count) {
+    const size_t slot = (size_t)8 * dec_nt(rows) * (head_dim + 2) * sizeof(float);
+    decode = 8192;
+    prefill = decode + (size_t)sm_count * 2 * slot;
+    total = prefill + (rows > kKvPrefillRows ? kv_prefill_workspace(head_dim, sm_count) : 0);
+  }
+};
+
+static qgemm_status_t kv_attention_run(const qgemm_kv_cache_t* c, KvAttnArgs a, void* ws, int sm_count, cudaStream_t s) {
+  const long long rows = (long long)a.max_new * a.group;
+  const KvWorkspace w(c->head_dim, rows, sm_count);
   const int all = a.requests;
   const int32_t *starts = a.starts, *lens = a.lens, *table = a.table;
-  for (int r0 = 0; r0 < all; r0 += (int)most) {
-    a.requests = all - r0 < most ? all - r0 : (int)most;
-    a.starts = starts + r0;
-    a.lens = lens + r0;
-    a.table = table + (size_t)r0 * a.width;
-    cudaError_t e;
-#define QG_DEC(T_, H_) e = nt == 1 ? launch_decode<T_, H_, 1>(a, sm_count, s) : launch_decode<T_, H_, 2>(a, sm_count, s)
-    if (c->type == QGEMM_KV_E4M3) {
-      if (c->head_dim == 64) QG_DEC(QGEMM_KV_E4M3, 64); else QG_DEC(QGEMM_KV_E4M3, 128);
-    } else {
-      if (c->head_dim == 64) QG_DEC(QGEMM_KV_INT8, 64); else QG_DEC(QGEMM_KV_INT8, 128);
+  for (int kernel = rows > kKvPrefillRows ? 1 : 0; kernel >= 0; --kernel) {
+    a.rows_min = kernel ? kKvPrefillRows : 0;
+    a.rows_max = kernel ? INT32_MAX : kKvPrefillRows;
+    a.tickets = reinterpret_cast<unsigned*>(static_cast<char*>(ws) + 4096 * kernel);
+    a.partials = reinterpret_cast<float*>(static_cast<char*>(ws) + (kernel ? w.prefill : w.decode));
+    const int nt = dec_nt(rows);
+    // requests per launch: the prefix sums fit shared memory and the line 31 bits
+    const long long per = kernel ? kv_line_most(a, 256, 7) : kv_line_most(a, 8 * nt, 4);
+    if (per > INT32_MAX)
+      return fail(QGEMM_ERR_UNSUPPORTED_SHAPE, "kv_attention: a request's rows x heads x tokens exceed 2^31 tiles");
+    long long most = INT32_MAX / per;
+    if (most > kKvMaxRequests) most = kKvMaxRequests;
+    for (int r0 = 0; r0 < all; r0 += (int)most) {
+      a.requests = all - r0 < most ? all - r0 : (int)most;
+      a.starts = starts + r0;
+      a.lens = lens + r0;
+      a.table = table + (size_t)r0 * a.width;
+      const cudaError_t e = kernel ? kv_prefill_launch(c->type, c->head_dim, a, sm_count, s)
+                                   : kv_decode_launch(c->type, c->head_dim, nt, a, sm_count, s);
+      if (e != cudaSuccess) return fail(QGEMM_ERR_CUDA, "kv_attention: launch: %s", cudaGetErrorString(e));
     }
-#undef QG_DEC
-    if (e != cudaSuccess) return fail(QGEMM_ERR_CUDA, "kv_attention: launch: %s", cudaGetErrorString(e));
   }
   return QGEMM_OK;
 }
@@ -643,7 +575,7 @@ size_t qgemm_kv_attention_workspace(const qgemm_kv_cache_t* c, int32_t q_heads, 
   if (kv_cache_error(c) || q_heads < 1 || q_heads % c->heads || max_new < 1) return 0;
   DevProps dp;
   if (device_props(&dp) != QGEMM_OK) return 0;
-  return kv_decode_workspace(c, q_heads / c->heads, max_new, dp.sm_count);
+  return KvWorkspace(c->head_dim, (long long)max_new * (q_heads / c->heads), dp.sm_count).total;
 }
 
 qgemm_status_t qgemm_kv_attention(const qgemm_kv_cache_t* c, const uint16_t* q, int64_t q_stride,
@@ -671,7 +603,9 @@ qgemm_status_t qgemm_kv_attention(const qgemm_kv_cache_t* c, const uint16_t* q, 
   qgemm_status_t st = device_props(&dp);
   if (st != QGEMM_OK) return st;
   const int group = q_heads / c->heads;
-  const size_t need = kv_decode_workspace(c, group, max_new, dp.sm_count);
+  if ((long long)max_new * group > INT32_MAX - 256)
+    return fail(QGEMM_ERR_UNSUPPORTED_SHAPE, "kv_attention: a request's rows x grouped heads exceed 2^31");
+  const size_t need = KvWorkspace(c->head_dim, (long long)max_new * group, dp.sm_count).total;
   if (!workspace || ws_bytes < need)
     return fail(QGEMM_ERR_WORKSPACE, "kv_attention: workspace of %zu bytes needed, %zu given", need, workspace ? ws_bytes : 0);
   KvAttnArgs a;
@@ -682,7 +616,7 @@ qgemm_status_t qgemm_kv_attention(const qgemm_kv_cache_t* c, const uint16_t* q, 
   a.max_new = max_new < tokens ? max_new : tokens;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.window = window; a.causal = causal != 0; a.out = out; a.lse = lse;
-  return kv_decode(c, a, workspace, dp.sm_count, as_stream(stream));
+  return kv_attention_run(c, a, workspace, dp.sm_count, as_stream(stream));
 }
 
 }  // extern "C"

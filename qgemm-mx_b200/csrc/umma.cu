@@ -532,9 +532,11 @@ qgemm_status_t gemm_umma_ts(const qgemm_weights_t* w, const __half* Xh, const fl
 unsigned umma_sk_fault();
 unsigned gemv_tma_fault();
 unsigned umma_bs_fault();
+unsigned kv_prefill_fault();
 cudaError_t umma_sk_fault_clear();
 cudaError_t gemv_tma_fault_clear();
 cudaError_t umma_bs_fault_clear();
+cudaError_t kv_prefill_fault_clear();
 cudaError_t tp_fault_clear();
 cudaError_t probe_fault_clear();
 
@@ -547,16 +549,17 @@ extern "C" {
 qgemm_status_t qgemm_umma_status(int32_t* faulted) {
   unsigned f = 0;
   QG_CUDA_RET(cudaMemcpyFromSymbol(&f, g_umma_fault, sizeof(f)));
-  const unsigned g = umma_sk_fault(), h = gemv_tma_fault(), b = umma_bs_fault();
-  if (g == 0xFFFFFFFFu || h == 0xFFFFFFFFu || b == 0xFFFFFFFFu)
+  const unsigned g = umma_sk_fault(), h = gemv_tma_fault(), b = umma_bs_fault(), k = kv_prefill_fault();
+  if (g == 0xFFFFFFFFu || h == 0xFFFFFFFFu || b == 0xFFFFFFFFu || k == 0xFFFFFFFFu)
     return fail(QGEMM_ERR_CUDA, "umma: reading a fault flag failed");
-  if (faulted) *faulted = (int32_t)(f | g | h | b);
-  if (!(f | g | h | b)) return QGEMM_OK;
+  if (faulted) *faulted = (int32_t)(f | g | h | b | k);
+  if (!(f | g | h | b | k)) return QGEMM_OK;
   // each flag holds where its kernel's first wait gave up (0x8wwcccbb: warp,
   // CTA, barrier index) or 1
   return fail(QGEMM_ERR_TIMEOUT,
-              "umma: a bounded barrier wait gave up (sites: tile %08x, stream-K %08x, decode %08x, block-scaled %08x)",
-              f, g, h, b);
+              "umma: a bounded barrier wait gave up (sites: tile %08x, stream-K %08x, decode %08x, block-scaled %08x, "
+              "attention %08x)",
+              f, g, h, b, k);
 }
 
 qgemm_status_t qgemm_clear_faults(void) {
@@ -566,6 +569,7 @@ qgemm_status_t qgemm_clear_faults(void) {
   QG_CUDA_RET(umma_sk_fault_clear());
   QG_CUDA_RET(gemv_tma_fault_clear());
   QG_CUDA_RET(umma_bs_fault_clear());
+  QG_CUDA_RET(kv_prefill_fault_clear());
   QG_CUDA_RET(tp_fault_clear());
   QG_CUDA_RET(probe_fault_clear());
   return QGEMM_OK;
