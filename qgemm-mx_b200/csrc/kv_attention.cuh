@@ -19,7 +19,7 @@
 
 namespace qg {
 
-constexpr int kKvMaxRequests = 2048;  // per launch: the line's prefix sums live in shared memory
+constexpr int kKvMaxRequests = 1024;  // per launch: they are kept in shared memory
 
 struct KvAttnArgs {
   const uint8_t *k, *v, *ks, *vs;
@@ -53,6 +53,10 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&b);
 }
 
+__device__ __forceinline__ float kv_lse(float m, float l) {
+  return l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+
 // Tokens row i of n sees: [lo, hi).
 __device__ __forceinline__ int row_hi(const KvAttnArgs& a, int len, int n, int i) {
   return a.causal ? min(max(len - n + i + 1, 0), len) : len;
@@ -68,16 +72,24 @@ __device__ __forceinline__ int row_lo(const KvAttnArgs& a, int len, int n, int i
 struct KvRequest {
   int start, n, len, n_all;
 };
-__device__ __forceinline__ KvRequest kv_request(const KvAttnArgs& a, int r) {
+__device__ __forceinline__ KvRequest kv_request(const KvAttnArgs& a, int start, int end, int len) {
   KvRequest q;
-  q.start = a.starts[r];
-  q.n_all = a.starts[r + 1] - q.start;
-  q.n = min(min(q.n_all, a.max_new), a.tokens - q.start);
+  q.start = start;
+  q.n_all = end - start;
+  q.n = min(min(q.n_all, a.max_new), a.tokens - start);
   const long long rows = (long long)q.n * a.group;
-  if (q.start < 0 || q.n < 0 || rows <= a.rows_min || rows > a.rows_max) q.n = 0;
-  q.len = (int)min((long long)max(a.lens[r], 0), (long long)a.width << a.block_log2);
+  if (start < 0 || q.n < 0 || rows <= a.rows_min || rows > a.rows_max) q.n = 0;
+  q.len = (int)min((long long)max(len, 0), (long long)a.width << a.block_log2);
   return q;
 }
+// A launch's requests in shared memory: prefix sums of their places on the
+// line (below), row starts and lengths.
+struct KvBatch {
+  int prefix[kKvMaxRequests + 1], start[kKvMaxRequests + 1], len[kKvMaxRequests];
+  __device__ __forceinline__ KvRequest at(const KvAttnArgs& a, int r) const {
+    return kv_request(a, start[r], start[r + 1], len[r]);
+  }
+};
 
 // ---- the line: all pairs' tiles, one after another ---------------------------
 // A pair is (request, KV head, group of RG rows); its tokens are tiles of
@@ -90,25 +102,26 @@ __device__ __forceinline__ KvRequest kv_request(const KvAttnArgs& a, int r) {
 // groups see from few to all tokens) without a list of groups.
 template <int RG, int TL>
 struct KvLine {
-  long long c0, c1, den;  // S(g) = (c0 g + c1 g (g + 1)) / den
+  long long c0, den;  // S(g) = (c0 g + RG g (g + 1)) / den, or c0 g / T without a slope
   int groups;
   __device__ __forceinline__ KvLine(const KvAttnArgs& a, const KvRequest& q) {
-    long long h0 = q.len, slope = 0;
-    if (a.causal) {
+    long long h0 = q.len;
+    den = 0;
+    const int span = min(q.n, (RG + a.group - 2) / a.group + 1);  // tokens of one group
+    const long long near = (long long)a.window + span - 1 + (1 << TL);
+    if (a.window > 0 && a.causal && near < q.len) {
+      h0 = near;
+    } else if (a.causal && q.n > 1) {
       h0 = max(q.len - q.n_all, 0) + 1;
-      slope = RG;
-      const int span = min(q.n, (RG + a.group - 2) / a.group + 1);  // tokens of one group
-      if (a.window > 0 && (long long)a.window + span - 1 + (1 << TL) < q.len) {
-        h0 = (long long)a.window + span - 1 + (1 << TL);
-        slope = 0;
-      }
+      den = (2ll * a.group) << TL;
     }
-    c0 = 2 * a.group * (h0 + (1 << TL));
-    c1 = slope;
-    den = (2ll * a.group) << TL;
+    c0 = h0 + (1 << TL);
+    if (den) c0 *= 2 * a.group;
     groups = (q.n * a.group + RG - 1) / RG;
   }
-  __device__ __forceinline__ int upto(int g) const { return (int)((c0 * g + c1 * g * (g + 1ll)) / den); }
+  __device__ __forceinline__ int upto(int g) const {
+    return den ? (int)((c0 * g + (long long)RG * g * (g + 1ll)) / den) : (int)((c0 * g) >> TL);
+  }
 };
 
 // One stretch of one pair's tiles.
@@ -120,14 +133,14 @@ struct KvSeg {
 };
 
 template <int RG, int TL>
-__device__ __forceinline__ void kv_seg(const KvAttnArgs& a, const int* prefix, int& r, int v, int v_end, KvSeg& s) {
-  while (prefix[r + 1] <= v) ++r;
-  const KvRequest q = kv_request(a, r);
+__device__ __forceinline__ void kv_seg(const KvAttnArgs& a, const KvBatch& b, int& r, int v, int v_end, KvSeg& s) {
+  while (b.prefix[r + 1] <= v) ++r;
+  const KvRequest q = b.at(a, r);
   const KvLine<RG, TL> line(a, q);
   const int per_head = line.upto(line.groups);
   s.r = r;
-  s.h = (v - prefix[r]) / per_head;
-  const int head_v = prefix[r] + s.h * per_head;
+  s.h = (v - b.prefix[r]) / per_head;
+  const int head_v = b.prefix[r] + s.h * per_head;
   int g = 0;
   for (int hi = line.groups; hi - g > 1;) {
     const int mid = (g + hi) >> 1;
@@ -155,19 +168,19 @@ inline long long kv_line_most(const KvAttnArgs& a, int rg, int tl) {
 }
 
 // The request whose pairs hold line position v (empty ones hold none).
-__device__ __forceinline__ int kv_find(const int* prefix, int requests, int v) {
+__device__ __forceinline__ int kv_find(const KvBatch& b, int requests, int v) {
   int lo = 0, hi = requests;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (prefix[mid] <= v) lo = mid; else hi = mid;
+    if (b.prefix[mid] <= v) lo = mid; else hi = mid;
   }
   return lo;
 }
 
-// The line's prefix sums (exclusive, prefix[requests] = its length) by a CTA of
-// at least WARPS warps; the first WARPS take part, all threads must call it.
+// Fills the batch and returns the line's length.  The first WARPS warps do the
+// work; all threads must call it.
 template <int RG, int TL, int WARPS>
-__device__ __forceinline__ int kv_line(const KvAttnArgs& a, int* prefix, int* scan) {
+__device__ __forceinline__ int kv_line(const KvAttnArgs& a, KvBatch& b, int* scan) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int base = 0;
   for (int r0 = 0; r0 < a.requests; r0 += WARPS * 32) {
@@ -175,7 +188,11 @@ __device__ __forceinline__ int kv_line(const KvAttnArgs& a, int* prefix, int* sc
     const bool on = tid < WARPS * 32 && r < a.requests;
     int c = 0;
     if (on) {
-      const KvRequest q = kv_request(a, r);
+      const int start = a.starts[r], end = a.starts[r + 1], len = a.lens[r];
+      b.start[r] = start;
+      b.len[r] = len;
+      if (r == a.requests - 1) b.start[r + 1] = end;
+      const KvRequest q = kv_request(a, start, end, len);
       if (q.n > 0) {
         const KvLine<RG, TL> line(a, q);
         c = a.heads * line.upto(line.groups);
@@ -195,13 +212,64 @@ __device__ __forceinline__ int kv_line(const KvAttnArgs& a, int* prefix, int* sc
       if (w == warp) before = total;
       total += scan[w];
     }
-    if (on) prefix[r] = before + v - c;
+    if (on) b.prefix[r] = before + v - c;
     base = total;
     __syncthreads();
   }
-  if (tid == 0) prefix[a.requests] = base;
+  if (tid == 0) b.prefix[a.requests] = base;
   __syncthreads();
   return base;
+}
+
+// The last CTA of a pair that crosses CTAs joins their partials, in CTA order:
+// values 4 e4 .. 4 e4 + 3 of the group's RG x HD.  BATCH partials' loads are
+// in flight before the first is used; one at a time this was a chain of L2
+// trips as long as the contributors.
+struct KvJoined {
+  float4 acc;
+  float M, L;
+};
+template <int RG, int HD, int BATCH>
+__device__ __forceinline__ KvJoined kv_join(const float* partials, size_t slot, int c_first, int c_last, int e4) {
+  const int qr = e4 * 4 / HD;
+  KvJoined j{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
+  for (int c0 = c_first; c0 <= c_last; c0 += BATCH) {
+    float mx[BATCH], lx[BATCH];
+    float4 ov[BATCH];
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      lx[i] = 0.0f;
+      if (c0 + i <= c_last) {
+        const float* p = partials + (size_t)((c0 + i) * 2 + (c0 + i == c_first ? 1 : 0)) * slot;
+        mx[i] = __ldcg(p + RG * HD + qr);
+        lx[i] = __ldcg(p + RG * HD + RG + qr);
+        ov[i] = __ldcg(reinterpret_cast<const float4*>(p) + e4);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      if (lx[i] == 0.0f) continue;
+      const float mn = fmaxf(j.M, mx[i]), f0 = j.M == -INFINITY ? 0.0f : ex2(j.M - mn), f1 = ex2(mx[i] - mn);
+      j.acc.x = fmaf(ov[i].x, f1, j.acc.x * f0); j.acc.y = fmaf(ov[i].y, f1, j.acc.y * f0);
+      j.acc.z = fmaf(ov[i].z, f1, j.acc.z * f0); j.acc.w = fmaf(ov[i].w, f1, j.acc.w * f0);
+      j.L = fmaf(lx[i], f1, j.L * f0);
+      j.M = mn;
+    }
+  }
+  if (j.L == 0.0f) j.M = 0.0f;
+  return j;
+}
+// Stores values 4 e4 .. of a finished group (and its rows' lse).
+template <int HD>
+__device__ __forceinline__ void kv_store(const KvAttnArgs& a, const KvSeg& s, int e4, const KvJoined& j) {
+  const int row = s.row0 + e4 * 4 / HD, d = e4 * 4 % HD;
+  if (row >= s.rows) return;
+  const int i = row / a.group, gh = row - i * a.group;
+  const int64_t at = (int64_t)(s.start + i) * a.heads * a.group + s.h * a.group + gh;
+  const float f = j.L == 0.0f ? 0.0f : 1.0f / j.L;
+  *reinterpret_cast<uint2*>(a.out + at * HD + d) =
+      make_uint2(pack_bf16(j.acc.x * f, j.acc.y * f), pack_bf16(j.acc.z * f, j.acc.w * f));
+  if (a.lse && d == 0) a.lse[at] = kv_lse(j.M, j.L);
 }
 
 }  // namespace qg

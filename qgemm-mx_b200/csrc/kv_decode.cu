@@ -75,14 +75,15 @@ __global__ void __launch_bounds__(kDecWarps * 32, 1) k_kv_decode(const KvAttnArg
   using Cfg = DecCfg<HD, NT>;
   constexpr int RG = 8 * NT, CPR = HD / 16, KJ = HD / 64, MT = HD / 16, ST = Cfg::kStages;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int s_prefix[kKvMaxRequests + 1];
+  __shared__ KvBatch s_batch;
   __shared__ int s_scan[kDecWarps];
-  __shared__ int2 s_part[kDecWarps][2];  // the pair range each partial belongs to
+  __shared__ int4 s_part[kDecWarps][2];  // the pair each partial belongs to: its range on the line, its request
+  __shared__ float s_wt[2 * kDecWarps + 2][RG];  // the partials' factors, then the joined m and l
   __shared__ unsigned s_ticket;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
 
-  const int V = kv_line<RG, 4, kDecWarps>(a, s_prefix, s_scan);
-  if (tid < 2 * kDecWarps) s_part[tid >> 1][tid & 1] = make_int2(-1, -1);
+  const int V = kv_line<RG, 4, kDecWarps>(a, s_batch, s_scan);
+  if (tid < 2 * kDecWarps) s_part[tid >> 1][tid & 1] = make_int4(-1, -1, 0, 0);
   __syncthreads();
   const int E = max(1, min((int)gridDim.x * kDecWarps, V / kDecMinTiles));  // shares
   const int k0 = blockIdx.x * kDecWarps;
@@ -99,7 +100,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 1) k_kv_decode(const KvAttnArg
   if (k0 + warp < E) {
     const int v0 = cut(k0 + warp), v1 = cut(k0 + warp + 1);
     // ---- producer state: runs ST tiles ahead of the arithmetic --------------
-    int p_v = v0, p_r = kv_find(s_prefix, a.requests, v0);
+    int p_v = v0, p_r = kv_find(s_batch, a.requests, v0);
     int c_r = p_r;  // the arithmetic's place
     KvSeg ps;
     ps.tile = 0; ps.tile_end = 0; ps.pair_end = v0;
@@ -108,7 +109,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 1) k_kv_decode(const KvAttnArg
     const int lg = a.block_log2;
     auto issue = [&](int stage) {
       while (ps.tile >= ps.tile_end && p_v < v1) {
-        kv_seg<RG, 4>(a, s_prefix, p_r, p_v, v1, ps);
+        kv_seg<RG, 4>(a, s_batch, p_r, p_v, v1, ps);
         p_v = min(ps.pair_end, v1);
         win = -1;
       }
@@ -166,7 +167,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 1) k_kv_decode(const KvAttnArg
     bool first = true;
     for (int v = v0; v < v1;) {
       KvSeg s;
-      kv_seg<RG, 4>(a, s_prefix, c_r, v, v1, s);
+      kv_seg<RG, 4>(a, s_batch, c_r, v, v1, s);
       const int seg_v0 = v;
       v = min(s.pair_end, v1);
       // ---- queries: f16 fragments and score factors --------------------------
@@ -366,7 +367,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 1) k_kv_decode(const KvAttnArg
 #pragma unroll
             for (int z = 0; z < MT / 4; ++z) dst[z] = make_uint4(w[4 * z], w[4 * z + 1], w[4 * z + 2], w[4 * z + 3]);
             if (a.lse && g == 0)
-              a.lse[at] = l[nt][c] == 0.0f ? -INFINITY : (m[nt][c] + log2f(l[nt][c])) * 0.6931471805599453f;
+              a.lse[at] = kv_lse(m[nt][c], l[nt][c]);
           }
       } else {
         // a warp has at most two: its first pair's end and its last pair's beginning
@@ -389,7 +390,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 1) k_kv_decode(const KvAttnArg
               slot[RG * HD + RG + qr] = l[nt][c];
             }
           }
-        if (lane == 0) s_part[warp][first ? 0 : 1] = make_int2(s.pair_v, s.pair_end);
+        if (lane == 0) s_part[warp][first ? 0 : 1] = make_int4(s.pair_v, s.pair_end, s.r, 0);
         first = false;
       }
     }
@@ -405,84 +406,62 @@ __global__ void __launch_bounds__(kDecWarps * 32, 1) k_kv_decode(const KvAttnArg
   };
 #pragma unroll 1
   for (int k = 0; k < 2 * kDecWarps;) {
-    const int2 pr = s_part[k >> 1][k & 1];
+    const int4 pr = s_part[k >> 1][k & 1];
     if (pr.x < 0) { ++k; continue; }
     int kend = k + 1;  // partials of one pair are neighbours, with unused slots between
-    for (int x = k + 1; x < 2 * kDecWarps; ++x) {
-      const int px = s_part[x >> 1][x & 1].x;
-      if (px == pr.x) kend = x + 1;
-    }
+    for (int x = k + 1; x < 2 * kDecWarps; ++x)
+      if (s_part[x >> 1][x & 1].x == pr.x) kend = x + 1;
     const bool whole = pr.x >= cta0 && pr.y <= cta1;
     const int c_first = share_of(pr.x) / kDecWarps, c_last = share_of(pr.y - 1) / kDecWarps;
     float* gp = a.partials + (size_t)(blockIdx.x * 2 + ((int)blockIdx.x == c_first ? 1 : 0)) * Cfg::kSlot;
     KvSeg s;
-    int join_r = kv_find(s_prefix, a.requests, pr.x);
-    kv_seg<RG, 4>(a, s_prefix, join_r, pr.x, pr.y, s);
-    auto finish = [&](int e4, float4 acc, float M, float L) {
-      const int qr = e4 * 4 / HD, d = e4 * 4 % HD, row = s.row0 + qr;
-      if (row >= s.rows) return;
-      const int i = row / a.group, gh = row - i * a.group;
-      const int64_t at = (int64_t)(s.start + i) * a.heads * a.group + s.h * a.group + gh;
-      const float f = L == 0.0f ? 0.0f : 1.0f / L;
-      *reinterpret_cast<uint2*>(a.out + at * HD + d) =
-          make_uint2(pack_bf16(acc.x * f, acc.y * f), pack_bf16(acc.z * f, acc.w * f));
-      if (a.lse && d == 0) a.lse[at] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
-    };
+    int join_r = pr.z;
+    kv_seg<RG, 4>(a, s_batch, join_r, pr.x, pr.y, s);
+    if (tid < RG) {
+      float M = -INFINITY, L = 0.0f;
+      for (int x = k; x < kend; ++x) {
+        const float* p = part_of(x);
+        if (s_part[x >> 1][x & 1].x == pr.x && p[RG * HD + RG + tid] != 0.0f) M = fmaxf(M, p[RG * HD + tid]);
+      }
+      for (int x = k; x < kend; ++x) {
+        const float* p = part_of(x);
+        const float lx = s_part[x >> 1][x & 1].x == pr.x ? p[RG * HD + RG + tid] : 0.0f;
+        const float f = lx != 0.0f ? ex2(p[RG * HD + tid] - M) : 0.0f;
+        s_wt[x][tid] = f;
+        L = fmaf(lx, f, L);
+      }
+      s_wt[2 * kDecWarps][tid] = L == 0.0f ? 0.0f : M;
+      s_wt[2 * kDecWarps + 1][tid] = L;
+    }
+    __syncthreads();
     for (int e4 = tid; e4 < RG * HD / 4; e4 += kDecWarps * 32) {
       const int qr = e4 * 4 / HD;
-      float M = -INFINITY, L = 0.0f;
-      for (int x = k; x < kend; ++x)
-        if (s_part[x >> 1][x & 1].x == pr.x) {
-          const float* p = part_of(x);
-          if (p[RG * HD + RG + qr] != 0.0f) M = fmaxf(M, p[RG * HD + qr]);
-        }
-      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      for (int x = k; x < kend; ++x)
-        if (s_part[x >> 1][x & 1].x == pr.x) {
-          const float* p = part_of(x);
-          const float lx = p[RG * HD + RG + qr];
-          if (lx == 0.0f) continue;
-          const float f = ex2(p[RG * HD + qr] - M);
-          const float4 ov = *reinterpret_cast<const float4*>(p + e4 * 4);
-          acc.x = fmaf(ov.x, f, acc.x); acc.y = fmaf(ov.y, f, acc.y);
-          acc.z = fmaf(ov.z, f, acc.z); acc.w = fmaf(ov.w, f, acc.w);
-          L = fmaf(lx, f, L);
-        }
-      if (L == 0.0f) M = 0.0f;
+      KvJoined j{make_float4(0.0f, 0.0f, 0.0f, 0.0f), s_wt[2 * kDecWarps][qr], s_wt[2 * kDecWarps + 1][qr]};
+      for (int x = k; x < kend; ++x) {
+        const float f = s_wt[x][qr];
+        if (f == 0.0f) continue;  // unused, or a share that saw no token
+        const float4 ov = *reinterpret_cast<const float4*>(part_of(x) + e4 * 4);
+        j.acc.x = fmaf(ov.x, f, j.acc.x); j.acc.y = fmaf(ov.y, f, j.acc.y);
+        j.acc.z = fmaf(ov.z, f, j.acc.z); j.acc.w = fmaf(ov.w, f, j.acc.w);
+      }
       if (whole) {
-        finish(e4, acc, M, L);
+        kv_store<HD>(a, s, e4, j);
       } else {
-        __stcg(reinterpret_cast<float4*>(gp) + e4, acc);
+        __stcg(reinterpret_cast<float4*>(gp) + e4, j.acc);
         if (e4 * 4 % HD == 0) {
-          __stcg(gp + RG * HD + qr, M);
-          __stcg(gp + RG * HD + RG + qr, L);
+          __stcg(gp + RG * HD + qr, j.M);
+          __stcg(gp + RG * HD + RG + qr, j.L);
         }
       }
     }
+    __syncthreads();
     if (!whole) {
       // the pair crosses CTAs: the last of its CTAs to arrive joins them in order
-      __syncthreads();
       if (tid == 0) s_ticket = ticket_acq_rel(a.tickets + c_first);
       __syncthreads();
       if (s_ticket == (unsigned)(c_last - c_first)) {
-        for (int e4 = tid; e4 < RG * HD / 4; e4 += kDecWarps * 32) {
-          const int qr = e4 * 4 / HD;
-          float M = -INFINITY, L = 0.0f;
-          float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          for (int c = c_first; c <= c_last; ++c) {
-            const float* p = a.partials + (size_t)(c * 2 + (c == c_first ? 1 : 0)) * Cfg::kSlot;
-            const float mx = __ldcg(p + RG * HD + qr), lx = __ldcg(p + RG * HD + RG + qr);
-            const float4 ov = __ldcg(reinterpret_cast<const float4*>(p) + e4);
-            if (lx == 0.0f) continue;
-            const float mn = fmaxf(M, mx), f0 = M == -INFINITY ? 0.0f : ex2(M - mn), f1 = ex2(mx - mn);
-            acc.x = fmaf(ov.x, f1, acc.x * f0); acc.y = fmaf(ov.y, f1, acc.y * f0);
-            acc.z = fmaf(ov.z, f1, acc.z * f0); acc.w = fmaf(ov.w, f1, acc.w * f0);
-            L = fmaf(lx, f1, L * f0);
-            M = mn;
-          }
-          if (L == 0.0f) M = 0.0f;
-          finish(e4, acc, M, L);
-        }
+        for (int e4 = tid; e4 < RG * HD / 4; e4 += kDecWarps * 32)
+          kv_store<HD>(a, s, e4, kv_join<RG, HD, 8>(a.partials, Cfg::kSlot, c_first, c_last, e4));
         if (tid == 0) a.tickets[c_first] = 0u;
       }
       __syncthreads();

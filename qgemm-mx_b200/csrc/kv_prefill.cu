@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
   using Cfg = PreCfg<HD>;
   constexpr int RG = kPreRows, TL = kPreTokLog2, AT = Cfg::kAtoms, TILE = Cfg::kTile;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ int s_prefix[kKvMaxRequests + 1];
+  __shared__ KvBatch s_batch;
   __shared__ int s_scan[16];
   __shared__ __align__(1024) uint64_t s_bars[32];
   __shared__ PreMeta s_meta[4][8];   // by tile, four deep: read after the tile's stage may be refilled
@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
   constexpr int K_FULL = 0, K_EMPTY = 2, V_FULL = 4, V_EMPTY = 6, Q_FULL = 8, Q_EMPTY = 9, S_FULL = 10, P_FULL = 12,
                 O_FULL = 14;
 
-  const int V = kv_line<RG, TL, 16>(a, s_prefix, s_scan);
+  const int V = kv_line<RG, TL, 16>(a, s_batch, s_scan);
   const int E = max(1, min((int)gridDim.x, V));
   const int cta = blockIdx.x;
   if (V == 0 || cta >= E) return;
@@ -152,10 +152,10 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
     constexpr int TSTEP = kPreLoaders / CPR;     // tokens between a thread's pieces
     const int ch = lt % CPR, tok0 = lt / CPR;
     const int lg = a.block_log2;
-    int n_tile = 0, n_seg = 0, r = kv_find(s_prefix, a.requests, v0);
+    int n_tile = 0, n_seg = 0, r = kv_find(s_batch, a.requests, v0);
     for (int v = v0; v < v1 && ok;) {
       KvSeg s;
-      kv_seg<RG, TL>(a, s_prefix, r, v, v1, s);
+      kv_seg<RG, TL>(a, s_batch, r, v, v1, s);
       v = min(s.pair_end, v1);
       if (s.tile >= s.tile_end) continue;
       const int32_t* row_table = a.table + (size_t)s.r * a.width;
@@ -275,11 +275,11 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
   } else if (warp == kPreMma) {
     if (lane == 0) {
       constexpr uint32_t id_qk = idesc_f16(128, kPreTok), id_pv = idesc_f16(128, HD) | (1u << 16);
-      int n_tile = 0, n_seg = 0, r = kv_find(s_prefix, a.requests, v0);
+      int n_tile = 0, n_seg = 0, r = kv_find(s_batch, a.requests, v0);
       uint32_t p_par[2] = {0, 0};
       for (int v = v0; v < v1 && ok;) {
         KvSeg s;
-        kv_seg<RG, TL>(a, s_prefix, r, v, v1, s);
+        kv_seg<RG, TL>(a, s_batch, r, v, v1, s);
         v = min(s.pair_end, v1);
         const int nt = s.tile_end - s.tile;
         if (nt <= 0) continue;
@@ -337,11 +337,11 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
     const uint32_t quad = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t sc = s_col(x) + quad, oc = o_col(x) + quad;
     const int rr = x * 128 + (warp & 3) * 32 + lane;
-    int n_tile = 0, n_seg = 0, r = kv_find(s_prefix, a.requests, v0);
+    int n_tile = 0, n_seg = 0, r = kv_find(s_batch, a.requests, v0);
     uint32_t s_par = 0, o_par = 0;
     for (int v = v0; v < v1;) {
       KvSeg s;
-      kv_seg<RG, TL>(a, s_prefix, r, v, v1, s);
+      kv_seg<RG, TL>(a, s_batch, r, v, v1, s);
       const int seg_v0 = v;
       v = min(s.pair_end, v1);
       const int nt = max(s.tile_end - s.tile, 0);
@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
         __stcg(slot + RG * HD + rr, m);
         __stcg(slot + RG * HD + RG + rr, l);
       } else if (on && a.lse) {
-        a.lse[at] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+        a.lse[at] = kv_lse(m, l);
       }
       tc_fence_before();  // O's reads are done before the next stretch's MMAs write it (through W full)
       if (!whole) {
@@ -489,29 +489,8 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
         if (tid == 0) s_ticket = ticket_acq_rel(a.tickets + c_first);
         asm volatile("bar.sync 1, 256;" ::: "memory");
         if (s_ticket == (unsigned)(c_last - c_first)) {
-          for (int e4 = tid; e4 < RG * HD / 4; e4 += 256) {
-            const int qr = e4 * 4 / HD, jrow = s.row0 + qr;
-            if (jrow >= s.rows) break;
-            float M = -INFINITY, L = 0.0f;
-            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (int c = c_first; c <= c_last; ++c) {
-              const float* p = a.partials + (size_t)(c * 2 + (c == c_first ? 1 : 0)) * Cfg::kSlot;
-              const float mx = __ldcg(p + RG * HD + qr), lx = __ldcg(p + RG * HD + RG + qr);
-              const float4 ov = __ldcg(reinterpret_cast<const float4*>(p) + e4);
-              if (lx == 0.0f) continue;
-              const float mn = fmaxf(M, mx), f0 = M == -INFINITY ? 0.0f : ex2(M - mn), f1 = ex2(mx - mn);
-              acc.x = fmaf(ov.x, f1, acc.x * f0); acc.y = fmaf(ov.y, f1, acc.y * f0);
-              acc.z = fmaf(ov.z, f1, acc.z * f0); acc.w = fmaf(ov.w, f1, acc.w * f0);
-              L = fmaf(lx, f1, L * f0);
-              M = mn;
-            }
-            const int ji = jrow / a.group, jg = jrow - ji * a.group, d = e4 * 4 % HD;
-            const int64_t jat = (int64_t)(s.start + ji) * a.heads * a.group + s.h * a.group + jg;
-            const float jf = L == 0.0f ? 0.0f : 1.0f / L;
-            *reinterpret_cast<uint2*>(a.out + jat * HD + d) =
-                make_uint2(pack_bf16(acc.x * jf, acc.y * jf), pack_bf16(acc.z * jf, acc.w * jf));
-            if (a.lse && d == 0) a.lse[jat] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
-          }
+          for (int e4 = tid; e4 < RG * HD / 4; e4 += 256)
+            kv_store<HD>(a, s, e4, kv_join<RG, HD, 2>(a.partials, Cfg::kSlot, c_first, c_last, e4));
           if (tid == 0) a.tickets[c_first] = 0u;
         }
       }
