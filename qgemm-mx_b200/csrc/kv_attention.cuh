@@ -48,13 +48,23 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&b);
 }
 
+// 1 / l, 0 for a row that saw no token (l is 2^-112 or more otherwise, or NaN)
+__device__ __forceinline__ float kv_inv(float l) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(l));
+  return l == 0.0f ? 0.0f : y;
+}
 __device__ __forceinline__ float kv_lse(float m, float l) {
-  return l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+  return l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
 }
 
 // Tokens row i of n sees: [lo, hi).
@@ -96,31 +106,28 @@ struct KvBatch {
 // T = 2^TL.  The line gives group g of a request S(g + 1) - S(g) places,
 //   S(g) = floor(sum over k < g of (h0 + (k + 1) slope) / T + 1),
 // where h0 + (g + 1) slope bounds the tokens the group sees: slope is RG / group
-// tokens for causal rows, 0 otherwise.  floor(a + x) - floor(a) >= floor(x), so
-// the places suffice for the group's tiles; the spare one stands for the cost
-// of starting a pair.  A closed form keeps causal prompts balanced (their
-// groups see from few to all tokens) without a list of groups.
+// tokens, rounded up, for causal rows and 0 otherwise.  floor(a + x) - floor(a)
+// >= floor(x), so the places suffice for the group's tiles; the spare one
+// stands for the cost of starting a pair.  A closed form keeps causal prompts
+// balanced (their groups see from few to all tokens) without a list of groups.
 template <int RG, int TL>
 struct KvLine {
-  long long c0, den;  // S(g) = (c0 g + RG g (g + 1)) / den, or c0 g / T without a slope
-  int groups;
+  int h0, slope, groups;
   __device__ __forceinline__ KvLine(const KvAttnArgs& a, const KvRequest& q) {
-    long long h0 = q.len;
-    den = 0;
-    const int span = min(q.n, (RG + a.group - 2) / a.group + 1);  // tokens of one group
-    const long long near = (long long)a.window + span - 1 + (1 << TL);
+    h0 = q.len;
+    slope = 0;
+    const int per = (RG + a.group - 1) / a.group;
+    const long long near = (long long)a.window + min(q.n, per + 1) - 1 + (1 << TL);  // a group spans per + 1 tokens at most
     if (a.window > 0 && a.causal && near < q.len) {
-      h0 = near;
+      h0 = (int)near;
     } else if (a.causal && q.n > 1) {
       h0 = max(q.len - q.n_all, 0) + 1;
-      den = (2ll * a.group) << TL;
+      slope = per;
     }
-    c0 = h0 + (1 << TL);
-    if (den) c0 *= 2 * a.group;
-    groups = (q.n * a.group + RG - 1) / RG;
+    groups = (int)(((unsigned)q.n * (unsigned)a.group + RG - 1u) / RG);
   }
   __device__ __forceinline__ int upto(int g) const {
-    return den ? (int)((c0 * g + (long long)RG * g * (g + 1ll)) / den) : (int)((c0 * g) >> TL);
+    return (int)(((long long)g * h0 + (long long)slope * ((long long)g * (g + 1) / 2)) >> TL) + g;
   }
 };
 
@@ -132,16 +139,21 @@ struct KvSeg {
   int tile, tile_end;    // absolute tiles to visit
 };
 
+// The stretch that begins at place v of the line and ends with its pair or at
+// v_end; r: a request at or before v's, moved to it.  Its loops are not
+// unrolled: code that runs once a stretch costs its instruction fetches.
 template <int RG, int TL>
 __device__ __forceinline__ void kv_seg(const KvAttnArgs& a, const KvBatch& b, int& r, int v, int v_end, KvSeg& s) {
+#pragma unroll 1
   while (b.prefix[r + 1] <= v) ++r;
   const KvRequest q = b.at(a, r);
   const KvLine<RG, TL> line(a, q);
   const int per_head = line.upto(line.groups);
   s.r = r;
-  s.h = (v - b.prefix[r]) / per_head;
+  s.h = (int)((unsigned)(v - b.prefix[r]) / (unsigned)per_head);
   const int head_v = b.prefix[r] + s.h * per_head;
   int g = 0;
+#pragma unroll 1
   for (int hi = line.groups; hi - g > 1;) {
     const int mid = (g + hi) >> 1;
     if (head_v + line.upto(mid) <= v) g = mid; else hi = mid;
@@ -167,9 +179,21 @@ inline long long kv_line_most(const KvAttnArgs& a, int rg, int tl) {
   return per_head > (1ll << 40) ? per_head : per_head * a.heads;
 }
 
+// The line cut into E shares of V / E or one more places.
+struct KvCuts {
+  unsigned size, longer;  // the first `longer` shares have size + 1 places
+  __device__ __forceinline__ KvCuts(int V, int E) : size((unsigned)V / (unsigned)E), longer((unsigned)V % (unsigned)E) {}
+  __device__ __forceinline__ int at(int k) const { return (int)(k * size + min((unsigned)k, longer)); }
+  __device__ __forceinline__ int share_of(int v) const {
+    const unsigned u = (unsigned)v, edge = longer * (size + 1);
+    return (int)(u < edge ? u / (size + 1) : longer + (u - edge) / size);
+  }
+};
+
 // The request whose pairs hold line position v (empty ones hold none).
 __device__ __forceinline__ int kv_find(const KvBatch& b, int requests, int v) {
   int lo = 0, hi = requests;
+#pragma unroll 1
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (b.prefix[mid] <= v) lo = mid; else hi = mid;
@@ -177,16 +201,19 @@ __device__ __forceinline__ int kv_find(const KvBatch& b, int requests, int v) {
   return lo;
 }
 
-// Fills the batch and returns the line's length.  The first WARPS warps do the
+// Fills the batch and returns the line's length; longest: the most places a
+// pair has, at most 2^15.  The first WARPS warps do the
 // work; all threads must call it.
 template <int RG, int TL, int WARPS>
-__device__ __forceinline__ int kv_line(const KvAttnArgs& a, KvBatch& b, int* scan) {
+__device__ __forceinline__ int kv_line(const KvAttnArgs& a, KvBatch& b, int* scan, int& longest) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int base = 0;
+  longest = 0;
+#pragma unroll 1
   for (int r0 = 0; r0 < a.requests; r0 += WARPS * 32) {
     const int r = r0 + tid;
     const bool on = tid < WARPS * 32 && r < a.requests;
-    int c = 0;
+    int c = 0, most = 0;
     if (on) {
       const int start = a.starts[r], end = a.starts[r + 1], len = a.lens[r];
       b.start[r] = start;
@@ -196,6 +223,7 @@ __device__ __forceinline__ int kv_line(const KvAttnArgs& a, KvBatch& b, int* sca
       if (q.n > 0) {
         const KvLine<RG, TL> line(a, q);
         c = a.heads * line.upto(line.groups);
+        most = min(line.upto(line.groups) - line.upto(line.groups - 1), 1 << 15);  // the last group's is the largest
       }
     }
     int v = c;
@@ -204,13 +232,15 @@ __device__ __forceinline__ int kv_line(const KvAttnArgs& a, KvBatch& b, int* sca
       const int u = __shfl_up_sync(0xFFFFFFFFu, v, d);
       if (lane >= d) v += u;
     }
-    if (lane == 31 && warp < WARPS) scan[warp] = v;
+    most = __reduce_max_sync(0xFFFFFFFFu, most);
+    if (lane == 31 && warp < WARPS) { scan[warp] = v; scan[WARPS + warp] = most; }
     __syncthreads();
     int before = base, total = base;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
       if (w == warp) before = total;
       total += scan[w];
+      longest = max(longest, scan[WARPS + w]);
     }
     if (on) b.prefix[r] = before + v - c;
     base = total;
@@ -221,55 +251,82 @@ __device__ __forceinline__ int kv_line(const KvAttnArgs& a, KvBatch& b, int* sca
   return base;
 }
 
-// The last CTA of a pair that crosses CTAs joins their partials, in CTA order:
-// values 4 e4 .. 4 e4 + 3 of the group's RG x HD.  BATCH partials' loads are
-// in flight before the first is used; one at a time this was a chain of L2
-// trips as long as the contributors.
+// One row (of RG) of a pair that crosses CTAs, joined by a warp from the CTAs'
+// partials in CTA order: lane i takes dims 4 i .. 4 i + 3 (HD = 128), or 2 i,
+// 2 i + 1.  Lanes first take a contributor's (m, l) each, so that the chain of
+// L2 trips is short: two, and one for every eight contributors' values.
+template <int RG, int HD>
 struct KvJoined {
-  float4 acc;
-  float M, L;
+  float acc[HD / 32], M, L;
 };
-template <int RG, int HD, int BATCH>
-__device__ __forceinline__ KvJoined kv_join(const float* partials, size_t slot, int c_first, int c_last, int e4) {
-  const int qr = e4 * 4 / HD;
-  KvJoined j{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
-  for (int c0 = c_first; c0 <= c_last; c0 += BATCH) {
-    float mx[BATCH], lx[BATCH];
-    float4 ov[BATCH];
+template <int RG, int HD>
+__device__ __forceinline__ KvJoined<RG, HD> kv_join(const float* partials, int slot, int c_first, int c_last, int row) {
+  constexpr int N = HD / 32;
+  const int lane = threadIdx.x & 31;
+  auto part = [&](int c) { return partials + (c == c_first ? 2 * c + 1 : 2 * c) * slot; };
+  KvJoined<RG, HD> j;
+  j.M = -INFINITY;
+  j.L = 0.0f;
 #pragma unroll
-    for (int i = 0; i < BATCH; ++i) {
-      lx[i] = 0.0f;
-      if (c0 + i <= c_last) {
-        const float* p = partials + (size_t)((c0 + i) * 2 + (c0 + i == c_first ? 1 : 0)) * slot;
-        mx[i] = __ldcg(p + RG * HD + qr);
-        lx[i] = __ldcg(p + RG * HD + RG + qr);
-        ov[i] = __ldcg(reinterpret_cast<const float4*>(p) + e4);
-      }
+  for (int i = 0; i < N; ++i) j.acc[i] = 0.0f;
+#pragma unroll 1
+  for (int c0 = c_first; c0 <= c_last; c0 += 32) {
+    const int n = min(c_last - c0 + 1, 32);
+    float m = -INFINITY, l = 0.0f;
+    if (lane < n) {
+      l = __ldcg(part(c0 + lane) + RG * HD + RG + row);
+      m = l != 0.0f ? __ldcg(part(c0 + lane) + RG * HD + row) : -INFINITY;
     }
+    float top = m;
 #pragma unroll
-    for (int i = 0; i < BATCH; ++i) {
-      if (lx[i] == 0.0f) continue;
-      const float mn = fmaxf(j.M, mx[i]), f0 = j.M == -INFINITY ? 0.0f : ex2(j.M - mn), f1 = ex2(mx[i] - mn);
-      j.acc.x = fmaf(ov[i].x, f1, j.acc.x * f0); j.acc.y = fmaf(ov[i].y, f1, j.acc.y * f0);
-      j.acc.z = fmaf(ov[i].z, f1, j.acc.z * f0); j.acc.w = fmaf(ov[i].w, f1, j.acc.w * f0);
-      j.L = fmaf(lx[i], f1, j.L * f0);
-      j.M = mn;
+    for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+    top = fmaxf(top, j.M);
+    const float mu = top == -INFINITY ? 0.0f : top;
+    const float f = l != 0.0f ? ex2(m - mu) : 0.0f, f0 = ex2(j.M - mu);
+    float sum = l * f;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+    j.L = fmaf(j.L, f0, sum);
+    j.M = top;
+#pragma unroll
+    for (int i = 0; i < N; ++i) j.acc[i] *= f0;
+#pragma unroll 1
+    for (int c = 0; c < n; c += 8) {
+      float x[8][N];
+#pragma unroll
+      for (int y = 0; y < 8; ++y) {
+        const float* p = part(c0 + min(c + y, n - 1)) + row * HD + lane * N;
+        if (N == 4) {
+          const float4 o = __ldcg(reinterpret_cast<const float4*>(p));
+          x[y][0] = o.x; x[y][1] = o.y; x[y][N - 2] = o.z; x[y][N - 1] = o.w;
+        } else {
+          const float2 o = __ldcg(reinterpret_cast<const float2*>(p));
+          x[y][0] = o.x; x[y][1] = o.y;
+        }
+      }
+#pragma unroll
+      for (int y = 0; y < 8; ++y) {
+        const float w = __shfl_sync(0xFFFFFFFFu, f, c + y);  // lanes from n on hold 0
+        if (w != 0.0f) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) j.acc[i] = fmaf(x[y][i], w, j.acc[i]);
+        }
+      }
     }
   }
   if (j.L == 0.0f) j.M = 0.0f;
   return j;
 }
-// Stores values 4 e4 .. of a finished group (and its rows' lse).
-template <int HD>
-__device__ __forceinline__ void kv_store(const KvAttnArgs& a, const KvSeg& s, int e4, const KvJoined& j) {
-  const int row = s.row0 + e4 * 4 / HD, d = e4 * 4 % HD;
-  if (row >= s.rows) return;
-  const int i = row / a.group, gh = row - i * a.group;
-  const int64_t at = (int64_t)(s.start + i) * a.heads * a.group + s.h * a.group + gh;
-  const float f = j.L == 0.0f ? 0.0f : 1.0f / j.L;
-  *reinterpret_cast<uint2*>(a.out + at * HD + d) =
-      make_uint2(pack_bf16(j.acc.x * f, j.acc.y * f), pack_bf16(j.acc.z * f, j.acc.w * f));
-  if (a.lse && d == 0) a.lse[at] = kv_lse(j.M, j.L);
+// Stores that row: query row `token` (of the batch), query head `head`.
+template <int RG, int HD>
+__device__ __forceinline__ void kv_store(const KvAttnArgs& a, int token, int head, const KvJoined<RG, HD>& j) {
+  const int lane = threadIdx.x & 31;
+  const int64_t at = (int64_t)token * (a.heads * a.group) + head;
+  const float f = kv_inv(j.L);
+  uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + at * HD) + lane * (HD / 64);
+#pragma unroll
+  for (int i = 0; i < HD / 64; ++i) dst[i] = pack_bf16(j.acc[2 * i] * f, j.acc[2 * i + 1] * f);
+  if (a.lse && lane == 0) a.lse[at] = kv_lse(j.M, j.L);
 }
 
 }  // namespace qg

@@ -4,56 +4,70 @@
 //
 // What bounds it: HBM.  Every K and V code is read once, one byte for 2 to
 // 2 x rows multiply-adds, so the kernel is built around the copy: each warp
-// streams its own tiles of 16 tokens through a private ring of cp.async stages
-// and never meets a barrier until its work is done.
+// streams its own tiles of 16 tokens through a private ring that one lane
+// fills by TMA (2 copies a tile, swizzled), and meets no barrier of the CTA
+// until its tokens are done.
 //
-// Split.  A pair is (request, group of 8 NT rows, KV head); its tokens are
+// Split.  A pair is (request, KV head, group of 8 NT rows); its tokens are
 // tiles of 16.  All pairs' tiles form one line that is cut into equal shares,
 // one per warp of the grid, wherever the cuts fall, so ragged batches and a
 // single long request load the GPU alike.  A share that holds a whole pair
-// writes its output; the others leave (m, l, O) partials that the CTA joins in
-// shared memory, and pairs that cross CTAs are joined by the last CTA to
-// arrive at a ticket, in CTA order, so results do not depend on timing.
+// writes its output; the others leave (O, m, l) partials that the CTA
+// joins in shared memory, and pairs that cross CTAs are joined by the
+// last CTA to arrive at a ticket, in CTA order, so results do not depend on
+// timing.
 //
 // Tile arithmetic (transposed, so that 8 query rows fill an MMA's N side):
 //   S^T[16 tokens x 8 rows] = K . q^T     A = K codes widened to f16
 //   O^T[dims x 8 rows]     += V^T . W^T   A = V codes, pairs of tokens by prmt
 // mma.sync m16n8k16 with 32-bit accumulators.  The token order inside a tile
 // and the dims inside an MMA are permuted so that every shared-memory read is
-// a conflict-free 128-bit (64-bit for V at 64 dims) load of bytes as they lie
-// in the cache.  With 2 x 8 rows per byte the tensor work is an eighth of what
-// the legacy MMA path sustains beside the copy, so tcgen05's TMEM round trips
+// a conflict-free 128-bit (64-bit for V at 64 dims) load of the swizzled
+// bytes.  With 2 x 8 rows per byte the tensor work is an eighth of what the
+// legacy MMA path sustains beside the copy, so tcgen05's TMEM round trips
 // would buy nothing here.
+//
+// Every mbarrier wait is bounded; on a timeout the kernel sets
+// g_kv_decode_fault, finishes its joins without waiting and returns
+// (qgemm_umma_status reports it).
 #include "gemv_core.cuh"
 #include "kv_attention.cuh"
+#include "tc.cuh"
 
 namespace qg {
 
-constexpr int kDecWarps = 8;
-constexpr int kDecMinTiles = 2;        // tiles per warp below which the grid shrinks
+__device__ unsigned g_kv_decode_fault = 0;
+
+constexpr int kDecMinTiles = 2;   // tiles per warp below which the grid shrinks
+constexpr int kDecSnapTiles = 16;  // longest pair for which shares end with whole pairs
+constexpr float kDecLow = -1e30f;  // m before a row has seen a token
 
 template <int HD, int NT>
 struct DecCfg {
-  static constexpr int kStage = 2 * 16 * HD;             // K and V of 16 tokens
-  static constexpr int kStages = HD == 128 ? (NT == 1 ? 5 : 4) : 8;
-  static constexpr int kSlot = 8 * NT * (HD + 2);        // floats of a partial: O, m, l
+  static constexpr int kStage = 2 * 16 * HD;  // K and V of 16 tokens
+  static constexpr int kWarps = NT == 1 ? 12 : 8;
+  static constexpr int kStages = HD == 128 ? (NT == 1 ? 3 : 4) : (NT == 1 ? 6 : 8);
+  static constexpr int kSlot = 8 * NT * (HD + 2);  // floats of a partial: O, m, l
   static constexpr int kRing = kStages * kStage;
-  // ring (a warp's last partial reuses it) | first partials | block exponents
-  static constexpr int kSmem = kDecWarps * (kRing + kSlot * 4 + kStages * 4);
+  // alignment | rings (a warp's last partial reuses its own) | first partials
+  static constexpr int kSmem = 1024 + kWarps * (kRing + kSlot * 4);
 };
 
-// Byte of 16-byte chunk `ch` of token row `row` in a tile: chunks are permuted
-// so that both the K reads (rows tau(g), chunks t) and the V reads (rows
-// t-dependent, chunk by g) of 8 or 16 lanes cover all banks once.
+// Byte of 16-byte chunk `ch` of token row `row` in a tile, as TMA's 128-byte
+// (64-byte) swizzle leaves it.
 template <int HD>
 __device__ __forceinline__ int tile_off(int row, int ch) {
-  if (HD == 128) return row * 128 + ((ch ^ ((((row ^ (row >> 1)) & 1) << 2) | (((row >> 2) & 1) << 1))) << 4);
-  return ((row & ~1) | ((row ^ (row >> 1)) & 1)) * 64 + ((ch ^ (((row >> 2) & 1) << 1)) << 4);
+  return HD == 128 ? row * 128 + ((ch ^ (row & 7)) << 4) : row * 64 + ((ch ^ ((row >> 1) & 3)) << 4);
+}
+// Token row of MMA row (and k index) i < 8; 8 + i is 8 rows on.  K's reads take
+// rows tau(2i), tau(2i + 1) and chunks 0-3 (4-7) together, V's rows tau(2t) of
+// four t and two chunks: these orders give them 8 bank groups each.
+template <int HD>
+__device__ __forceinline__ int tau(int i) {
+  const int r = HD == 128 ? (i & 6) : ((i >> 1) & 1) | (i & 4);  // tau(2t): 0 2 4 6, or 0 1 4 5
+  return (i & 1) ? (HD == 128 ? r ^ 5 : r ^ 3) : r;
 }
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
@@ -71,105 +85,140 @@ __device__ __forceinline__ uint2 lds8(uint32_t p) {
 }
 
 template <int TYPE, int HD, int NT>
-__global__ void __launch_bounds__(kDecWarps * 32, 1) k_kv_decode(const KvAttnArgs a) {
+__global__ void __launch_bounds__(DecCfg<HD, NT>::kWarps * 32, 1)
+k_kv_decode(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const KvAttnArgs a) {
   using Cfg = DecCfg<HD, NT>;
-  constexpr int RG = 8 * NT, CPR = HD / 16, KJ = HD / 64, MT = HD / 16, ST = Cfg::kStages;
-  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int RG = 8 * NT, KJ = HD / 64, MT = HD / 16, ST = Cfg::kStages, W = Cfg::kWarps;
+  extern __shared__ uint8_t smem_raw[];
   __shared__ KvBatch s_batch;
-  __shared__ int s_scan[kDecWarps];
-  __shared__ int4 s_part[kDecWarps][2];  // the pair each partial belongs to: its range on the line, its request
-  __shared__ float s_wt[2 * kDecWarps + 2][RG];  // the partials' factors, then the joined m and l
-  __shared__ unsigned s_ticket;
+  __shared__ int s_scan[2 * W];
+  __shared__ __align__(1024) uint64_t s_bars[W * ST];
+  __shared__ int s_cell[W * ST];   // a stage's (block, head)
+  __shared__ int2 s_part[2 * W];   // the pair each partial belongs to: its range on the line
+  __shared__ int4 s_rows[2 * W];   // and its rows: first token row, first row, rows, head
+  __shared__ int4 s_cross[2];              // pairs that cross CTAs: begun before this CTA, begun in it
+  __shared__ unsigned s_ticket[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const uint32_t raw = su32(smem_raw), base = (raw + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw);
 
-  const int V = kv_line<RG, 4, kDecWarps>(a, s_batch, s_scan);
-  if (tid < 2 * kDecWarps) s_part[tid >> 1][tid & 1] = make_int4(-1, -1, 0, 0);
-  __syncthreads();
-  const int E = max(1, min((int)gridDim.x * kDecWarps, V / kDecMinTiles));  // shares
-  const int k0 = blockIdx.x * kDecWarps;
+  if (tid < 2 * W) s_part[tid] = make_int2(-1, -1);
+  if (tid < 2) s_cross[tid] = make_int4(-1, -1, 0, 0);
+  if (lane == 0) {
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(su32(&s_bars[warp * ST + i]), 1);
+      s_cell[warp * ST + i] = 0;
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  int longest;
+  const int V = kv_line<RG, 4, W>(a, s_batch, s_scan, longest);
+  // Short pairs are not cut: a share takes the pairs that begin in it.  One pair
+  // more in some shares costs less than joining nearly every pair.
+  const bool snap = longest <= kDecSnapTiles;
+  const int E = max(1, min((int)gridDim.x * W, V / kDecMinTiles));  // shares
+  const int k0 = blockIdx.x * W;
   if (V == 0 || k0 >= E) return;
-  auto cut = [&](int k) { return (int)((long long)k * V / E); };
-  auto share_of = [&](int v) { return (int)((((long long)v + 1) * E - 1) / V); };
-  const int cta0 = cut(k0), cta1 = cut(min(k0 + kDecWarps, E));
+  const KvCuts cuts(V, E);
 
-  uint8_t* ring = smem + warp * Cfg::kRing;
-  const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
-  float* first_part = reinterpret_cast<float*>(smem + kDecWarps * Cfg::kRing) + warp * Cfg::kSlot;
-  uint32_t* meta = reinterpret_cast<uint32_t*>(smem + kDecWarps * (Cfg::kRing + Cfg::kSlot * 4)) + warp * ST;
+  const uint32_t ring = base + warp * Cfg::kRing;
+  float* const last_part = reinterpret_cast<float*>(smem + warp * Cfg::kRing);
+  float* const first_part = reinterpret_cast<float*>(smem + W * Cfg::kRing) + warp * Cfg::kSlot;
+  const float inv_group = 1.0f / (float)a.group;
+  // row / group for the few rows of this kernel (exact below 2^21)
+  auto token_of = [&](int row) { return (int)(((float)row + 0.5f) * inv_group); };
+  bool ok = true;
 
   if (k0 + warp < E) {
-    const int v0 = cut(k0 + warp), v1 = cut(k0 + warp + 1);
+    const int v0 = cuts.at(k0 + warp), v1 = cuts.at(k0 + warp + 1);
     // ---- producer state: runs ST tiles ahead of the arithmetic --------------
     int p_v = v0, p_r = kv_find(s_batch, a.requests, v0);
     int c_r = p_r;  // the arithmetic's place
-    KvSeg ps;
-    ps.tile = 0; ps.tile_end = 0; ps.pair_end = v0;
-    int win = -1, win_id = 0;  // 32 block ids from `win` on, one per lane, and their exponents
-    uint32_t win_meta = 0;
+    KvSeg s;
+    kv_seg<RG, 4>(a, s_batch, c_r, v0, snap ? INT32_MAX : v1, s);
+    const bool skip = snap && s.pair_v < v0;  // begun in the share before
+    if (skip) p_v = s.pair_end;
+    KvSeg ps = s;
+    ps.tile = 0; ps.tile_end = 0;
+    int win = 0, win_end = 0, win_id = -1;  // 32 block ids from `win` on, one per lane
     const int lg = a.block_log2;
     auto issue = [&](int stage) {
-      while (ps.tile >= ps.tile_end && p_v < v1) {
-        kv_seg<RG, 4>(a, s_batch, p_r, p_v, v1, ps);
-        p_v = min(ps.pair_end, v1);
-        win = -1;
+      while (ps.tile >= ps.tile_end) {
+        if (p_v >= v1) return;
+        kv_seg<RG, 4>(a, s_batch, p_r, p_v, snap ? INT32_MAX : v1, ps);
+        p_v = snap ? ps.pair_end : min(ps.pair_end, v1);
+        win_end = 0;
       }
-      if (ps.tile < ps.tile_end) {
-        const int tok = ps.tile * 16, page = tok >> lg;
-        if (win < 0 || page - win >= 32) {
-          win = page;
-          const int p = page + lane;
-          win_id = ((long long)p << lg) < ps.len ? a.table[(size_t)ps.r * a.width + p] : -1;
-          if (win_id < 0 || win_id >= a.blocks) {
-            win_id = -1;
-            win_meta = 127u | (127u << 8);
-          } else {
-            const size_t cell = (size_t)win_id * a.heads + ps.h;
-            win_meta = (uint32_t)a.ks[cell] | ((uint32_t)a.vs[cell] << 8);
-          }
-        }
-        const int id = __shfl_sync(0xFFFFFFFFu, win_id, page - win);
-        const uint32_t mt = __shfl_sync(0xFFFFFFFFu, win_meta, page - win);
-        if (lane == 0) meta[stage] = mt;
-        const size_t cell = id < 0 ? 0 : (size_t)id * a.heads + ps.h;
-        const size_t off = (cell << lg) * HD + (size_t)(tok & ((1 << lg) - 1)) * HD;
-        const uint8_t* k = a.k + off;
-        const uint8_t* v = a.v + off;
-        const uint32_t dst = ring_s + stage * Cfg::kStage;
-#pragma unroll
-        for (int j = 0; j < CPR / 2; ++j) {
-          const int c = j * 32 + lane, row = c / CPR, ch = c % CPR;
-          // tokens past the end (the rest of the last block) arrive as zeros
-          const int bytes = id >= 0 && tok + row < ps.len ? 16 : 0;
-          cp16(dst + tile_off<HD>(row, ch), k + c * 16, bytes);
-          cp16(dst + 16 * HD + tile_off<HD>(row, ch), v + c * 16, bytes);
-        }
-        ++ps.tile;
+      const int tok = ps.tile * 16, page = tok >> lg;
+      if (page >= win_end) {
+        win = page;
+        win_end = page + 32;
+        const int p = page + lane;
+        win_id = ((long long)p << lg) < ps.len ? a.table[(size_t)ps.r * a.width + p] : -1;
+        if (win_id >= a.blocks) win_id = -1;
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
+      const int id = __shfl_sync(0xFFFFFFFFu, win_id, page - win);
+      if (lane == 0) {
+        const uint32_t bar = su32(&s_bars[warp * ST + stage]), dst = ring + stage * Cfg::kStage;
+        const int cell = id * a.heads + ps.h;
+        // a block outside the pool: rows in front of it, which TMA fills with zeros
+        const int y = id < 0 ? -16 : (cell << lg) + (tok & ((1 << lg) - 1));
+        s_cell[warp * ST + stage] = max(cell, 0);
+        mbar_expect_tx(bar, Cfg::kStage);
+        tma_load_2d(dst, &map_k, 0, y, bar);
+        tma_load_2d(dst + 16 * HD, &map_v, 0, y, bar);
+      }
+      ++ps.tile;
     };
+    // queries of a stretch: this lane's part of row g of each tile of 8
+    auto load_q = [&](const KvSeg& s, uint4 (&w)[NT][KJ][2]) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int row = s.row0 + nt * 8 + g, i = token_of(row), gh = row - i * a.group;
+        const uint16_t* qp = a.q + (int64_t)(s.start + i) * a.q_stride + (int64_t)(s.h * a.group + gh) * a.q_head_stride;
+#pragma unroll
+        for (int j = 0; j < KJ; ++j)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            w[nt][j][x] = row < s.rows ? __ldg(reinterpret_cast<const uint4*>(qp + (t + 4 * j) * 16) + x)
+                                       : make_uint4(0, 0, 0, 0);
+      }
+    };
+    uint4 qw[NT][KJ][2];
+    if (!skip) load_q(s, qw);  // in flight while the ring fills
 #pragma unroll 1
     for (int i = 0; i < ST; ++i) issue(i);
 
     // ---- fixed shared-memory offsets of this lane ---------------------------
-    const int tau = (g & 4) | ((g & 1) << 1) | ((g >> 1) & 1);  // token row of MMA row g (+8: tau + 8)
+    const int tg = tau<HD>(g);  // token row of MMA row g
     uint32_t k_off[2][KJ], v_off[4];
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-      for (int j = 0; j < KJ; ++j) k_off[hh][j] = tile_off<HD>(tau + 8 * hh, t + 4 * j);
+      for (int j = 0; j < KJ; ++j) k_off[hh][j] = tile_off<HD>(tg + 8 * hh, t + 4 * j);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int row = (t & 1) + 4 * (t >> 1) + (i & 1) * 2 + (i >> 1) * 8;
+      const int row = tau<HD>(2 * t + (i & 1)) + (i >> 1) * 8;
       v_off[i] = 16 * HD + (HD == 128 ? tile_off<HD>(row, g) : tile_off<HD>(row, g >> 1) + (g & 1) * 8);
     }
 
     int stage = 0;
+    uint32_t parity = 0;
     bool first = true;
-    for (int v = v0; v < v1;) {
-      KvSeg s;
-      kv_seg<RG, 4>(a, s_batch, c_r, v, v1, s);
+    // exponents of a stage's blocks, K's | V's << 8: loaded a tile ahead
+    auto load_exp = [&](int stage) {
+      const int cell = s_cell[warp * ST + stage];
+      return (uint32_t)__ldg(a.ks + cell) | ((uint32_t)__ldg(a.vs + cell) << 8);
+    };
+    __syncwarp();
+    uint32_t mt_next = load_exp(0);
+    for (int v = skip ? s.pair_end : v0; v < v1;) {
       const int seg_v0 = v;
-      v = min(s.pair_end, v1);
+      if (v > v0) {
+        kv_seg<RG, 4>(a, s_batch, c_r, v, snap ? INT32_MAX : v1, s);
+        load_q(s, qw);
+      }
+      v = snap ? s.pair_end : min(s.pair_end, v1);
       // ---- queries: f16 fragments and score factors --------------------------
       uint32_t qf[NT][KJ][8];
       float fac[NT][2], m[NT][2], l[NT][2];
@@ -177,18 +226,12 @@ __global__ void __launch_bounds__(kDecWarps * 32, 1) k_kv_decode(const KvAttnArg
       float o[NT][MT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const int row = s.row0 + nt * 8 + g;
-        const bool on = row < s.rows;
-        const int i = row / a.group, gh = row - i * a.group;
-        const uint16_t* qp = a.q + (int64_t)(s.start + i) * a.q_stride + (int64_t)(s.h * a.group + gh) * a.q_head_stride;
-        uint4 w[KJ][2];
         uint32_t mx = 0;
 #pragma unroll
         for (int j = 0; j < KJ; ++j)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            w[j][x] = on ? __ldg(reinterpret_cast<const uint4*>(qp + (t + 4 * j) * 16) + x) : make_uint4(0, 0, 0, 0);
-            const uint32_t u[4] = {w[j][x].x, w[j][x].y, w[j][x].z, w[j][x].w};
+            const uint32_t u[4] = {qw[nt][j][x].x, qw[nt][j][x].y, qw[nt][j][x].z, qw[nt][j][x].w};
 #pragma unroll
             for (int y = 0; y < 4; ++y) mx = max(mx, max(u[y] & 0x7FFFu, (u[y] >> 16) & 0x7FFFu));
           }
@@ -201,23 +244,20 @@ __global__ void __launch_bounds__(kDecWarps * 32, 1) k_kv_decode(const KvAttnArg
         for (int j = 0; j < KJ; ++j)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const uint32_t u[4] = {w[j][x].x, w[j][x].y, w[j][x].z, w[j][x].w};
+            const uint32_t u[4] = {qw[nt][j][x].x, qw[nt][j][x].y, qw[nt][j][x].z, qw[nt][j][x].w};
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              const __half2 hv = __floats2half2_rn(u2f(u[y] << 16) * down, u2f(u[y] & 0xFFFF0000u) * down);
-              qf[nt][j][x * 4 + y] = *reinterpret_cast<const uint32_t*>(&hv);
-            }
+            for (int y = 0; y < 4; ++y)
+              qf[nt][j][x * 4 + y] = pack_f16(u2f(u[y] << 16) * down, u2f(u[y] & 0xFFFF0000u) * down);
           }
         const float fq = a.scale_log2 * pow2f(e);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const int col = 2 * t + c;
           fac[nt][c] = __shfl_sync(0xFFFFFFFFu, fq, col * 4);
-          const int crow = s.row0 + nt * 8 + col;
-          const int ci = min(crow, s.rows - 1) / a.group;
+          const int ci = token_of(min(s.row0 + nt * 8 + col, s.rows - 1));
           lo_t[nt][c] = row_lo(a, s.len, s.n_all, ci);
           hi_t[nt][c] = row_hi(a, s.len, s.n_all, ci);
-          m[nt][c] = -INFINITY;
+          m[nt][c] = kDecLow;
           l[nt][c] = 0.0f;
         }
 #pragma unroll
@@ -226,23 +266,17 @@ __global__ void __launch_bounds__(kDecWarps * 32, 1) k_kv_decode(const KvAttnArg
           for (int y = 0; y < 4; ++y) o[nt][x][y] = 0.0f;
       }
       // tiles every row of the group sees whole need no mask
-      const int last_i = (min(s.row0 + RG, s.rows) - 1) / a.group;
-      const int full_lo = row_lo(a, s.len, s.n_all, last_i), full_hi = row_hi(a, s.len, s.n_all, s.row0 / a.group);
+      const int full_lo = row_lo(a, s.len, s.n_all, token_of(min(s.row0 + RG, s.rows) - 1));
+      const int full_hi = row_hi(a, s.len, s.n_all, token_of(s.row0));
 
       // ---- tiles ----------------------------------------------------------------
 #pragma unroll 1
-      for (int tile = s.tile; tile < s.tile_end; ++tile) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
-        __syncwarp();
-        const uint32_t sb = ring_s + stage * Cfg::kStage;
-        const uint32_t mt = meta[stage];
+      for (int tile = s.tile; tile < s.tile_end && ok; ++tile) {
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait_flag(su32(&s_bars[warp * ST + stage]), parity, &g_kv_decode_fault));
+        if (!ok) break;
+        const uint32_t sb = ring + stage * Cfg::kStage;
+        const uint32_t mt = mt_next;
         float sc[NT][2][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int y = 0; y < 4; ++y) sc[nt][x][y] = 0.0f;
 #pragma unroll
         for (int j = 0; j < KJ; ++j) {
           const uint4 k0v = lds16(sb + k_off[0][j]), k1v = lds16(sb + k_off[1][j]);
@@ -253,67 +287,12 @@ __global__ void __launch_bounds__(kDecWarps * 32, 1) k_kv_decode(const KvAttnArg
             codes4_to_f16<TYPE>(kw[0][i], a0, a2);
             codes4_to_f16<TYPE>(kw[1][i], a1, a3);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              mma_f16(sc[nt][i & 1], a0, a1, a2, a3, qf[nt][j][2 * i], qf[nt][j][2 * i + 1]);
-          }
-        }
-        const float ksc = u2f((mt & 0xFFu) << 23);
-        const int vexp = (int)((mt >> 8) & 0xFFu) - 127;
-        const float ev = (float)vexp, inv = pow2f(-vexp);
-        const int tok = tile * 16 + tau;
-        const bool mask = tile * 16 < full_lo || tile * 16 + 16 > full_hi;
-        float p[NT][4];
-        bool grow = false;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const int c = y & 1;
-            p[nt][y] = fmaf(sc[nt][0][y] + sc[nt][1][y], fac[nt][c] * ksc, ev);
-            if (mask) {
-              const int at = tok + (y >> 1) * 8;
-              if (at < lo_t[nt][c] || at >= hi_t[nt][c]) p[nt][y] = -INFINITY;
+            for (int nt = 0; nt < NT; ++nt) {
+              if (j == 0 && i < 2) mma_f16_z(sc[nt][i], a0, a1, a2, a3, qf[nt][j][2 * i], qf[nt][j][2 * i + 1]);
+              else mma_f16(sc[nt][i & 1], a0, a1, a2, a3, qf[nt][j][2 * i], qf[nt][j][2 * i + 1]);
             }
-            grow |= p[nt][y] > m[nt][c] + kKvGrow;
-          }
-        if (__any_sync(0xFFFFFFFFu, grow)) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              float x = fmaxf(p[nt][c], p[nt][2 + c]);
-#pragma unroll
-              for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, d));
-              const float mn = x > m[nt][c] + kKvGrow ? x - kKvTop : m[nt][c];
-              const float al = m[nt][c] == -INFINITY ? 0.0f : ex2(m[nt][c] - mn);
-              if (mn != m[nt][c]) {
-                l[nt][c] *= al;
-#pragma unroll
-                for (int z = 0; z < MT; ++z) {
-                  o[nt][z][c] *= al;
-                  o[nt][z][2 + c] *= al;
-                }
-                m[nt][c] = mn;
-              }
-            }
-        }
-        uint32_t bw[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const float mm = m[nt][y & 1];
-            p[nt][y] = ex2(p[nt][y] - (mm == -INFINITY ? 0.0f : mm));
-          }
-#pragma unroll
-          for (int c = 0; c < 2; ++c) l[nt][c] = fmaf(p[nt][c] + p[nt][2 + c], inv, l[nt][c]);
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const __half2 hv = __floats2half2_rn(p[nt][2 * x], p[nt][2 * x + 1]);
-            bw[nt][x] = movmatrix(*reinterpret_cast<const uint32_t*>(&hv));
           }
         }
-        // ---- O^T += V^T . W^T
         uint32_t vw[4][HD / 32];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -325,8 +304,84 @@ __global__ void __launch_bounds__(kDecWarps * 32, 1) k_kv_decode(const KvAttnArg
             vw[i][0] = x.x; vw[i][1] = x.y;
           }
         }
+        const float ksc = u2f((mt & 0xFFu) << 23);
+        const int vexp = (int)((mt >> 8) & 0xFFu) - 127;
+        const float ev = (float)vexp, inv = pow2f(-vexp);
+        float f[NT][2], p[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) f[nt][c] = fac[nt][c] * ksc;
+#pragma unroll
+          for (int y = 0; y < 4; ++y) sc[nt][0][y] += sc[nt][1][y];
+        }
+        const int tok = tile * 16;
+        const bool mask = tok < full_lo || tok + 16 > full_hi;
+        bool hide[NT][4];
+        if (mask) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const int at = tok + tg + (y >> 1) * 8;
+              hide[nt][y] = at < lo_t[nt][y & 1] || at >= hi_t[nt][y & 1];
+            }
+          // what lies behind the last token is not the request's: its codes may be NaN
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (tok + tau<HD>(2 * t + (i & 1)) + (i >> 1) * 8 >= s.len) {
+#pragma unroll
+              for (int w = 0; w < HD / 32; ++w) vw[i][w] = 0u;
+            }
+        }
+        bool grow = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            p[nt][y] = fmaf(sc[nt][0][y], f[nt][y & 1], ev - m[nt][y & 1]);
+            if (mask && hide[nt][y]) p[nt][y] = -INFINITY;
+            grow |= p[nt][y] > kKvGrow;
+          }
+        if (__any_sync(0xFFFFFFFFu, grow)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float x0 = fmaf(sc[nt][0][c], f[nt][c], ev), x1 = fmaf(sc[nt][0][2 + c], f[nt][c], ev);
+              if (mask && hide[nt][c]) x0 = -INFINITY;
+              if (mask && hide[nt][2 + c]) x1 = -INFINITY;
+              float x = fmaxf(x0, x1);
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, d));
+              if (x > m[nt][c] + kKvGrow) {
+                const float mn = x - kKvTop, al = ex2(m[nt][c] - mn);
+                l[nt][c] *= al;
+#pragma unroll
+                for (int z = 0; z < MT; ++z) {
+                  o[nt][z][c] *= al;
+                  o[nt][z][2 + c] *= al;
+                }
+                m[nt][c] = mn;
+              }
+              p[nt][c] = x0 - m[nt][c];
+              p[nt][2 + c] = x1 - m[nt][c];
+            }
+        }
+        uint32_t bw[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int y = 0; y < 4; ++y) p[nt][y] = ex2(p[nt][y]);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) l[nt][c] = fmaf(p[nt][c] + p[nt][2 + c], inv, l[nt][c]);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) bw[nt][x] = movmatrix(pack_f16(p[nt][2 * x], p[nt][2 * x + 1]));
+        }
         __syncwarp();
         issue(stage);  // the stage's bytes are in registers: refill it
+        mt_next = load_exp(stage + 1 == ST ? 0 : stage + 1);
+        // ---- O^T += V^T . W^T
 #pragma unroll
         for (int w = 0; w < HD / 32; ++w)
 #pragma unroll
@@ -338,7 +393,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 1) k_kv_decode(const KvAttnArg
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][2 * w + x], a0, a1, a2, a3, bw[nt][0], bw[nt][1]);
           }
-        stage = stage + 1 == ST ? 0 : stage + 1;
+        if (++stage == ST) { stage = 0; parity ^= 1u; }
       }
 
       // ---- the stretch's end -------------------------------------------------------
@@ -348,7 +403,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 1) k_kv_decode(const KvAttnArg
         for (int c = 0; c < 2; ++c) {
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) l[nt][c] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][c], d);
-          if (m[nt][c] == -INFINITY) m[nt][c] = 0.0f;  // l is 0, or NaN for a NaN score
+          if (m[nt][c] == kDecLow) m[nt][c] = 0.0f;  // l is 0, or NaN for a NaN score
         }
       if (seg_v0 == s.pair_v && v == s.pair_end) {
 #pragma unroll
@@ -357,25 +412,21 @@ __global__ void __launch_bounds__(kDecWarps * 32, 1) k_kv_decode(const KvAttnArg
           for (int c = 0; c < 2; ++c) {
             const int row = s.row0 + nt * 8 + 2 * t + c;
             if (row >= s.rows) continue;
-            const int i = row / a.group, gh = row - i * a.group;
+            const int i = token_of(row), gh = row - i * a.group;
             const int64_t at = (int64_t)(s.start + i) * a.heads * a.group + s.h * a.group + gh;
-            const float f = l[nt][c] == 0.0f ? 0.0f : 1.0f / l[nt][c];
+            const float f = kv_inv(l[nt][c]);
             uint32_t w[MT];
 #pragma unroll
             for (int z = 0; z < MT; ++z) w[z] = pack_bf16(o[nt][z][c] * f, o[nt][z][2 + c] * f);
             uint4* dst = reinterpret_cast<uint4*>(a.out + at * HD + g * MT * 2);
 #pragma unroll
             for (int z = 0; z < MT / 4; ++z) dst[z] = make_uint4(w[4 * z], w[4 * z + 1], w[4 * z + 2], w[4 * z + 3]);
-            if (a.lse && g == 0)
-              a.lse[at] = kv_lse(m[nt][c], l[nt][c]);
+            if (a.lse && g == 0) a.lse[at] = kv_lse(m[nt][c], l[nt][c]);
           }
       } else {
-        // a warp has at most two: its first pair's end and its last pair's beginning
-        if (!first) {
-          asm volatile("cp.async.wait_all;" ::: "memory");
-          __syncwarp();
-        }
-        float* slot = first ? first_part : reinterpret_cast<float*>(ring);
+        // a warp has at most two: its first pair's end and its last pair's
+        // beginning, when all its tiles have been read
+        float* slot = first ? first_part : last_part;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -390,88 +441,107 @@ __global__ void __launch_bounds__(kDecWarps * 32, 1) k_kv_decode(const KvAttnArg
               slot[RG * HD + RG + qr] = l[nt][c];
             }
           }
-        if (lane == 0) s_part[warp][first ? 0 : 1] = make_int4(s.pair_v, s.pair_end, s.r, 0);
+        if (lane == 0) {
+          s_part[2 * warp + (first ? 0 : 1)] = make_int2(s.pair_v, s.pair_end);
+          s_rows[2 * warp + (first ? 0 : 1)] = make_int4(s.start, s.row0, s.rows, s.h);
+        }
         first = false;
       }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (!ok && lane == 0) fault_drain();
   }
   __syncthreads();
 
-  // ---- join the partials -------------------------------------------------------------
-  auto part_of = [&](int k) -> const float* {
-    const int w = k >> 1;
-    return (k & 1) ? reinterpret_cast<const float*>(smem + w * Cfg::kRing)
-                   : reinterpret_cast<const float*>(smem + kDecWarps * Cfg::kRing) + w * Cfg::kSlot;
-  };
+  // ---- join the partials: a warp takes row `warp` (and 8 on) of every pair --------
+  const int cta0 = cuts.at(k0), cta1 = cuts.at(min(k0 + W, E));
+  constexpr int N = HD / 32;
+  const int pair_of = lane < 2 * W ? s_part[lane].x : -1;
+  unsigned left = __ballot_sync(0xFFFFFFFFu, pair_of >= 0);
 #pragma unroll 1
-  for (int k = 0; k < 2 * kDecWarps;) {
-    const int4 pr = s_part[k >> 1][k & 1];
-    if (pr.x < 0) { ++k; continue; }
-    int kend = k + 1;  // partials of one pair are neighbours, with unused slots between
-    for (int x = k + 1; x < 2 * kDecWarps; ++x)
-      if (s_part[x >> 1][x & 1].x == pr.x) kend = x + 1;
-    const bool whole = pr.x >= cta0 && pr.y <= cta1;
-    const int c_first = share_of(pr.x) / kDecWarps, c_last = share_of(pr.y - 1) / kDecWarps;
-    float* gp = a.partials + (size_t)(blockIdx.x * 2 + ((int)blockIdx.x == c_first ? 1 : 0)) * Cfg::kSlot;
-    KvSeg s;
-    int join_r = pr.z;
-    kv_seg<RG, 4>(a, s_batch, join_r, pr.x, pr.y, s);
-    if (tid < RG) {
-      float M = -INFINITY, L = 0.0f;
-      for (int x = k; x < kend; ++x) {
-        const float* p = part_of(x);
-        if (s_part[x >> 1][x & 1].x == pr.x && p[RG * HD + RG + tid] != 0.0f) M = fmaxf(M, p[RG * HD + tid]);
+  while (left) {
+    const int k = __ffs(left) - 1;
+    const int2 pr = s_part[k];
+    const unsigned members = __ballot_sync(0xFFFFFFFFu, pair_of == pr.x);
+    left &= ~members;
+    const int4 rw = s_rows[k];
+    const bool whole = pr.x >= cta0 && pr.y <= cta1, begun = pr.x >= cta0;
+#pragma unroll 1
+    for (int qr = warp; qr < RG; qr += W) {
+      // lane x takes slot x's m and l; then all slots' values are loaded at once
+      const float* const firsts = reinterpret_cast<const float*>(smem + W * Cfg::kRing);
+      float m = -INFINITY, l = 0.0f;
+      if (members >> lane & 1u) {
+        const float* p = (lane & 1 ? reinterpret_cast<const float*>(smem + (lane >> 1) * Cfg::kRing)
+                                   : firsts + (lane >> 1) * Cfg::kSlot) + RG * HD + qr;
+        l = p[RG];
+        if (l != 0.0f) m = p[0];  // 0: a share that saw no token
       }
-      for (int x = k; x < kend; ++x) {
-        const float* p = part_of(x);
-        const float lx = s_part[x >> 1][x & 1].x == pr.x ? p[RG * HD + RG + tid] : 0.0f;
-        const float f = lx != 0.0f ? ex2(p[RG * HD + tid] - M) : 0.0f;
-        s_wt[x][tid] = f;
-        L = fmaf(lx, f, L);
+      KvJoined<RG, HD> j;
+      j.M = m;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) j.M = fmaxf(j.M, __shfl_xor_sync(0xFFFFFFFFu, j.M, d));
+      if (j.M == -INFINITY) j.M = 0.0f;
+      const float f = l != 0.0f ? ex2(m - j.M) : 0.0f;
+      j.L = l * f;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) j.L += __shfl_xor_sync(0xFFFFFFFFu, j.L, d);
+#pragma unroll
+      for (int i = 0; i < N; ++i) j.acc[i] = 0.0f;
+#pragma unroll
+      for (int x = 0; x < 2 * W; ++x) {
+        const float fx = __shfl_sync(0xFFFFFFFFu, f, x);
+        const float* p = (x & 1 ? reinterpret_cast<const float*>(smem + (x >> 1) * Cfg::kRing)
+                                : firsts + (x >> 1) * Cfg::kSlot) + qr * HD + lane * N;
+        if (fx != 0.0f) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) j.acc[i] = fmaf(p[i], fx, j.acc[i]);
+        }
       }
-      s_wt[2 * kDecWarps][tid] = L == 0.0f ? 0.0f : M;
-      s_wt[2 * kDecWarps + 1][tid] = L;
-    }
-    __syncthreads();
-    for (int e4 = tid; e4 < RG * HD / 4; e4 += kDecWarps * 32) {
-      const int qr = e4 * 4 / HD;
-      KvJoined j{make_float4(0.0f, 0.0f, 0.0f, 0.0f), s_wt[2 * kDecWarps][qr], s_wt[2 * kDecWarps + 1][qr]};
-      for (int x = k; x < kend; ++x) {
-        const float f = s_wt[x][qr];
-        if (f == 0.0f) continue;  // unused, or a share that saw no token
-        const float4 ov = *reinterpret_cast<const float4*>(part_of(x) + e4 * 4);
-        j.acc.x = fmaf(ov.x, f, j.acc.x); j.acc.y = fmaf(ov.y, f, j.acc.y);
-        j.acc.z = fmaf(ov.z, f, j.acc.z); j.acc.w = fmaf(ov.w, f, j.acc.w);
-      }
+      const int row = rw.y + qr;
       if (whole) {
-        kv_store<HD>(a, s, e4, j);
+        if (row < rw.z) {
+          const int tk = token_of(row);
+          kv_store<RG, HD>(a, rw.x + tk, rw.w * a.group + row - tk * a.group, j);
+        }
       } else {
-        __stcg(reinterpret_cast<float4*>(gp) + e4, j.acc);
-        if (e4 * 4 % HD == 0) {
+        float* gp = a.partials + (size_t)(blockIdx.x * 2 + (begun ? 1 : 0)) * Cfg::kSlot;
+#pragma unroll
+        for (int i = 0; i < N; ++i) __stcg(gp + qr * HD + lane * N + i, j.acc[i]);
+        if (lane == 0) {
           __stcg(gp + RG * HD + qr, j.M);
           __stcg(gp + RG * HD + RG + qr, j.L);
         }
       }
     }
-    __syncthreads();
-    if (!whole) {
-      // the pair crosses CTAs: the last of its CTAs to arrive joins them in order
-      if (tid == 0) s_ticket = ticket_acq_rel(a.tickets + c_first);
-      __syncthreads();
-      if (s_ticket == (unsigned)(c_last - c_first)) {
-        for (int e4 = tid; e4 < RG * HD / 4; e4 += kDecWarps * 32)
-          kv_store<HD>(a, s, e4, kv_join<RG, HD, 8>(a.partials, Cfg::kSlot, c_first, c_last, e4));
-        if (tid == 0) a.tickets[c_first] = 0u;
-      }
-      __syncthreads();
+    if (!whole && tid == 0) s_cross[begun ? 1 : 0] = make_int4(pr.x, pr.y, k, 0);
+  }
+  __syncthreads();
+  // ---- pairs that cross CTAs: the last of their CTAs to arrive joins them ----------
+  if (tid < 2 && s_cross[tid].x >= 0) s_ticket[tid] = ticket_acq_rel(a.tickets + cuts.share_of(s_cross[tid].x) / W);
+  __syncthreads();
+#pragma unroll 1
+  for (int x = 0; x < 2; ++x) {
+    const int4 pr = s_cross[x];
+    if (pr.x < 0) continue;
+    const int c_first = cuts.share_of(pr.x) / W, c_last = cuts.share_of(pr.y - 1) / W;
+    if (s_ticket[x] != (unsigned)(c_last - c_first)) continue;
+    const int4 rw = s_rows[pr.z];
+#pragma unroll 1
+    for (int qr = warp; qr < min(RG, rw.z - rw.y); qr += W) {
+      const int row = rw.y + qr, tk = token_of(row);
+      kv_store<RG, HD>(a, rw.x + tk, rw.w * a.group + row - tk * a.group,
+                       kv_join<RG, HD>(a.partials, Cfg::kSlot, c_first, c_last, qr));
     }
-    k = kend;
+    if (tid == 0) a.tickets[c_first] = 0u;
   }
 }
 
+bool make_tma_map_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* ptr, uint64_t inner, uint64_t outer,
+                     uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle sw);
+
 template <int TYPE, int HD, int NT>
-static cudaError_t launch_decode(const KvAttnArgs& a, int grid, cudaStream_t s) {
+static cudaError_t launch_decode(const CUtensorMap& mk, const CUtensorMap& mv, const KvAttnArgs& a, int grid,
+                                 cudaStream_t s) {
   constexpr int BYTES = DecCfg<HD, NT>::kSmem;
   static bool attr[64] = {false};
   int dev = 0;
@@ -482,15 +552,17 @@ static cudaError_t launch_decode(const KvAttnArgs& a, int grid, cudaStream_t s) 
     if (e != cudaSuccess) return e;
     if (dev < 64) attr[dev] = true;
   }
-  k_kv_decode<TYPE, HD, NT><<<grid, kDecWarps * 32, BYTES, s>>>(a);
+  k_kv_decode<TYPE, HD, NT><<<grid, DecCfg<HD, NT>::kWarps * 32, BYTES, s>>>(mk, mv, a);
   return cudaGetLastError();
 }
 
 // Two row tiles of 8 when a request brings more than 8 rows per KV head.
 static int dec_nt(long long rows) { return rows > 8 ? 2 : 1; }
 
-cudaError_t kv_decode_launch(int type, int head_dim, int nt, const KvAttnArgs& a, int grid, cudaStream_t s) {
-#define QG_DEC(T_, H_) nt == 1 ? launch_decode<T_, H_, 1>(a, grid, s) : launch_decode<T_, H_, 2>(a, grid, s)
+static cudaError_t kv_decode_launch(int type, int head_dim, int nt, const CUtensorMap& mk, const CUtensorMap& mv,
+                                    const KvAttnArgs& a, int grid, cudaStream_t s) {
+#define QG_DEC(T_, H_) \
+  nt == 1 ? launch_decode<T_, H_, 1>(mk, mv, a, grid, s) : launch_decode<T_, H_, 2>(mk, mv, a, grid, s)
   if (type == QGEMM_KV_E4M3) return head_dim == 64 ? QG_DEC(QGEMM_KV_E4M3, 64) : QG_DEC(QGEMM_KV_E4M3, 128);
   return head_dim == 64 ? QG_DEC(QGEMM_KV_INT8, 64) : QG_DEC(QGEMM_KV_INT8, 128);
 #undef QG_DEC
@@ -498,6 +570,15 @@ cudaError_t kv_decode_launch(int type, int head_dim, int nt, const KvAttnArgs& a
 
 size_t kv_prefill_workspace(int head_dim, int sm_count);
 cudaError_t kv_prefill_launch(int type, int head_dim, const KvAttnArgs& a, int grid, cudaStream_t s);
+
+unsigned kv_decode_fault() {
+  unsigned f = 0;
+  return cudaMemcpyFromSymbol(&f, g_kv_decode_fault, sizeof(f)) == cudaSuccess ? f : 0xFFFFFFFFu;
+}
+cudaError_t kv_decode_fault_clear() {
+  const unsigned z = 0;
+  return cudaMemcpyToSymbol(g_kv_decode_fault, &z, sizeof(z));
+}
 
 // Requests with more rows per KV head than this run on the tcgen05 kernel.
 constexpr int kKvPrefillRows = 32;
@@ -516,6 +597,15 @@ struct KvWorkspace {
 static qgemm_status_t kv_attention_run(const qgemm_kv_cache_t* c, KvAttnArgs a, void* ws, int sm_count, cudaStream_t s) {
   const long long rows = (long long)a.max_new * a.group;
   const KvWorkspace w(c->head_dim, rows, sm_count);
+  // K and V as rows of head_dim codes, copied 16 at a time
+  const uint64_t code_rows = (uint64_t)c->blocks * c->heads * c->block;
+  if (code_rows > INT32_MAX)
+    return fail(QGEMM_ERR_UNSUPPORTED_SHAPE, "kv_attention: blocks x heads x block of the pool exceed 2^31 - 1");
+  CUtensorMap mk, mv;
+  const CUtensorMapSwizzle sw = c->head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+  if (!make_tma_map_2d(&mk, CU_TENSOR_MAP_DATA_TYPE_UINT8, c->k, c->head_dim, code_rows, c->head_dim, c->head_dim, 16, sw) ||
+      !make_tma_map_2d(&mv, CU_TENSOR_MAP_DATA_TYPE_UINT8, c->v, c->head_dim, code_rows, c->head_dim, c->head_dim, 16, sw))
+    return fail(QGEMM_ERR_CUDA, "kv_attention: cuTensorMapEncodeTiled failed");
   const int all = a.requests;
   const int32_t *starts = a.starts, *lens = a.lens, *table = a.table;
   for (int kernel = rows > kKvPrefillRows ? 1 : 0; kernel >= 0; --kernel) {
@@ -536,7 +626,7 @@ static qgemm_status_t kv_attention_run(const qgemm_kv_cache_t* c, KvAttnArgs a, 
       a.lens = lens + r0;
       a.table = table + (size_t)r0 * a.width;
       const cudaError_t e = kernel ? kv_prefill_launch(c->type, c->head_dim, a, sm_count, s)
-                                   : kv_decode_launch(c->type, c->head_dim, nt, a, sm_count, s);
+                                   : kv_decode_launch(c->type, c->head_dim, nt, mk, mv, a, sm_count, s);
       if (e != cudaSuccess) return fail(QGEMM_ERR_CUDA, "kv_attention: launch: %s", cudaGetErrorString(e));
     }
   }

@@ -43,7 +43,6 @@ constexpr int kPreLoaders = 256;
 
 template <int HD>
 struct PreCfg {
-  static constexpr int kAtoms = HD / 64;               // 64-dim swizzle atoms of a row
   static constexpr int kTile = 128 * HD * 2;           // one f16 operand tile: 128 rows
   static constexpr int kQ = 2 * kTile;
   static constexpr int kSmem = kQ + 4 * kTile + 1024;  // q, two stages of K and V, alignment
@@ -80,10 +79,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
 __device__ __forceinline__ void sts16(uint32_t p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(p), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 // Byte offset of 16-byte chunk c (0..7) of row r in a swizzled 128-byte-row tile.
 __device__ __forceinline__ uint32_t sw128_off(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
 
@@ -95,10 +90,10 @@ struct PreMeta {
 template <int TYPE, int HD>
 __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnArgs a) {
   using Cfg = PreCfg<HD>;
-  constexpr int RG = kPreRows, TL = kPreTokLog2, AT = Cfg::kAtoms, TILE = Cfg::kTile;
+  constexpr int RG = kPreRows, TL = kPreTokLog2, TILE = Cfg::kTile;
   extern __shared__ uint8_t smem_raw[];
   __shared__ KvBatch s_batch;
-  __shared__ int s_scan[16];
+  __shared__ int s_scan[32];
   __shared__ __align__(1024) uint64_t s_bars[32];
   __shared__ PreMeta s_meta[4][8];   // by tile, four deep: read after the tile's stage may be refilled
   __shared__ float s_fq[2][RG];      // by stretch: score factor of each row
@@ -114,13 +109,13 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
   constexpr int K_FULL = 0, K_EMPTY = 2, V_FULL = 4, V_EMPTY = 6, Q_FULL = 8, Q_EMPTY = 9, S_FULL = 10, P_FULL = 12,
                 O_FULL = 14;
 
-  const int V = kv_line<RG, TL, 16>(a, s_batch, s_scan);
+  int longest;
+  const int V = kv_line<RG, TL, 16>(a, s_batch, s_scan, longest);
   const int E = max(1, min((int)gridDim.x, V));
   const int cta = blockIdx.x;
   if (V == 0 || cta >= E) return;
-  auto cut = [&](int k) { return (int)((long long)k * V / E); };
-  auto share_of = [&](int v) { return (int)((((long long)v + 1) * E - 1) / V); };
-  const int v0 = cut(cta), v1 = cut(cta + 1);
+  const KvCuts cuts(V, E);
+  const int v0 = cuts.at(cta), v1 = cuts.at(cta + 1);
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -441,11 +436,11 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
       // that the barrier below is met and the tickets return to zero
       if (m == -INFINITY) m = 0.0f;  // l is 0, or NaN for a NaN score
       const bool whole = seg_v0 == s.pair_v && v == s.pair_end;
-      const int c_first = share_of(s.pair_v);
+      const int c_first = cuts.share_of(s.pair_v);
       float* slot = a.partials + (size_t)(cta * 2 + (cta == c_first ? 1 : 0)) * Cfg::kSlot;
       const int i = min(row, s.rows - 1) / a.group, gh = min(row, s.rows - 1) - i * a.group;
       const int64_t at = (int64_t)(s.start + i) * a.heads * a.group + s.h * a.group + gh;
-      const float f = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+      const float f = whole ? kv_inv(l) : 1.0f;
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
         uint32_t w[32];
@@ -484,13 +479,17 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
       tc_fence_before();  // O's reads are done before the next stretch's MMAs write it (through W full)
       if (!whole) {
         // the pair crosses CTAs: its last CTA to arrive joins them in order
-        const int c_last = share_of(s.pair_end - 1);
+        const int c_last = cuts.share_of(s.pair_end - 1);
         asm volatile("bar.sync 1, 256;" ::: "memory");
         if (tid == 0) s_ticket = ticket_acq_rel(a.tickets + c_first);
         asm volatile("bar.sync 1, 256;" ::: "memory");
         if (s_ticket == (unsigned)(c_last - c_first)) {
-          for (int e4 = tid; e4 < RG * HD / 4; e4 += 256)
-            kv_store<HD>(a, s, e4, kv_join<RG, HD, 2>(a.partials, Cfg::kSlot, c_first, c_last, e4));
+#pragma unroll 1
+          for (int qr = warp; qr < min(RG, s.rows - s.row0); qr += 8) {
+            const int jrow = s.row0 + qr, ji = jrow / a.group;
+            kv_store<RG, HD>(a, s.start + ji, s.h * a.group + jrow - ji * a.group,
+                             kv_join<RG, HD>(a.partials, Cfg::kSlot, c_first, c_last, qr));
+          }
           if (tid == 0) a.tickets[c_first] = 0u;
         }
       }

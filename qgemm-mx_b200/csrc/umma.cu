@@ -533,10 +533,12 @@ unsigned umma_sk_fault();
 unsigned gemv_tma_fault();
 unsigned umma_bs_fault();
 unsigned kv_prefill_fault();
+unsigned kv_decode_fault();
 cudaError_t umma_sk_fault_clear();
 cudaError_t gemv_tma_fault_clear();
 cudaError_t umma_bs_fault_clear();
 cudaError_t kv_prefill_fault_clear();
+cudaError_t kv_decode_fault_clear();
 cudaError_t tp_fault_clear();
 cudaError_t probe_fault_clear();
 
@@ -549,17 +551,19 @@ extern "C" {
 qgemm_status_t qgemm_umma_status(int32_t* faulted) {
   unsigned f = 0;
   QG_CUDA_RET(cudaMemcpyFromSymbol(&f, g_umma_fault, sizeof(f)));
-  const unsigned g = umma_sk_fault(), h = gemv_tma_fault(), b = umma_bs_fault(), k = kv_prefill_fault();
-  if (g == 0xFFFFFFFFu || h == 0xFFFFFFFFu || b == 0xFFFFFFFFu || k == 0xFFFFFFFFu)
+  const unsigned g = umma_sk_fault(), h = gemv_tma_fault(), b = umma_bs_fault(), k = kv_prefill_fault(),
+                 d = kv_decode_fault();
+  if (g == 0xFFFFFFFFu || h == 0xFFFFFFFFu || b == 0xFFFFFFFFu || k == 0xFFFFFFFFu ||
+      d == 0xFFFFFFFFu)
     return fail(QGEMM_ERR_CUDA, "umma: reading a fault flag failed");
-  if (faulted) *faulted = (int32_t)(f | g | h | b | k);
-  if (!(f | g | h | b | k)) return QGEMM_OK;
+  if (faulted) *faulted = (int32_t)(f | g | h | b | k | d);
+  if (!(f | g | h | b | k | d)) return QGEMM_OK;
   // each flag holds where its kernel's first wait gave up (0x8wwcccbb: warp,
   // CTA, barrier index) or 1
   return fail(QGEMM_ERR_TIMEOUT,
               "umma: a bounded barrier wait gave up (sites: tile %08x, stream-K %08x, decode %08x, block-scaled %08x, "
-              "attention %08x)",
-              f, g, h, b, k);
+              "attention %08x, decode attention %08x)",
+              f, g, h, b, k, d);
 }
 
 qgemm_status_t qgemm_clear_faults(void) {
@@ -570,6 +574,7 @@ qgemm_status_t qgemm_clear_faults(void) {
   QG_CUDA_RET(gemv_tma_fault_clear());
   QG_CUDA_RET(umma_bs_fault_clear());
   QG_CUDA_RET(kv_prefill_fault_clear());
+  QG_CUDA_RET(kv_decode_fault_clear());
   QG_CUDA_RET(tp_fault_clear());
   QG_CUDA_RET(probe_fault_clear());
   return QGEMM_OK;
