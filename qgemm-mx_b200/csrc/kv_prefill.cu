@@ -11,19 +11,22 @@
 //                  token rows lie (N-major operand)
 // and A's softmax runs while the tensor core works for B, and the reverse.
 //
-// Warps (17): 0-3 and 4-7 the softmax of A and B, one row per thread (TMEM
-// lane = row); 8 issues the MMAs; 9-16 widen q, K and V into the swizzled
-// operand tiles, their global loads one tile ahead in registers.  Widening
-// costs 2 conversions per 4 codes once per 256 rows.
+// Warps (20): 0-3 and 4-7 the softmax of A and B, one row per thread (TMEM
+// lane = row), 64 scores in registers at a time; 8-15 widen q, K and V into the
+// swizzled operand tiles, their global loads one tile ahead in registers; 16
+// issues the MMAs.  Widening costs 2 conversions per 4 codes once per 256 rows.
+// Registers go where the data waits: 128 a softmax thread, 80 a widening one,
+// 56 in the MMA warp's group (together no more than the launch's 640 x 96).
 //
 // What bounds it: exponentials.  A row and token cost one ex2, 16 a clock and
 // SM, as long as its 2 x 2 x 128 multiply-adds take the tensor core at 128
 // dims; at 64 dims the tensor core needs half of that.
 //
 // The line of all pairs' tiles is cut into one equal share per CTA
-// (kv_attention.cuh), so 148 CTAs finish together whatever the pair count; pairs that
-// cross CTAs leave (O, m, l) partials, joined in CTA order by the last CTA to
-// arrive at the pair's ticket.
+// (kv_attention.cuh), so all CTAs finish together whatever the pair count; pairs
+// that cross CTAs leave (O, m, l) partials, which a second kernel joins in CTA
+// order: 32 rows a CTA.  (By the last CTA to arrive, a pair's 256 rows took that
+// CTA 50 us.)
 //
 // Every mbarrier wait is bounded; on a timeout the kernel sets g_kv_fault,
 // drains, frees its TMEM and returns (qgemm_umma_status reports it).
@@ -38,7 +41,7 @@ namespace qg {
 __device__ unsigned g_kv_fault = 0;
 
 constexpr int kPreRows = 256, kPreTokLog2 = 7, kPreTok = 128;
-constexpr int kPreWarps = 17, kPreMma = 8, kPreLoad = 9;  // warps; first of each role
+constexpr int kPreWarps = 20, kPreLoad = 8, kPreMma = 16;  // warps; first of each role
 constexpr int kPreLoaders = 256;
 
 template <int HD>
@@ -52,19 +55,38 @@ struct PreCfg {
 __device__ __forceinline__ bool pre_wait(uint32_t bar, uint32_t parity) {
   return mbar_wait_flag(bar, parity, &g_kv_fault);
 }
+// The MMA warp runs its loop with all lanes and one of them issues (`one`), and
+// descriptors are passed as their low words (address and leading offset; the
+// high word, stride offset 1024 and the 128-byte swizzle, is the same for all):
+// so they live in uniform registers.  With 64-bit descriptors in a one-lane
+// branch, issuing took longer than the MMAs.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
 // D(tmem) (+)= A(smem) . B(smem)
-__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void umma_ss_one(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc, uint32_t one) {
   asm volatile(
-      "{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{ .reg .pred p, q; .reg .b64 x, y; setp.ne.b32 p, %4, 0; setp.ne.b32 q, %5, 0;\n"
+      "  mov.b64 x, {%1, %6}; mov.b64 y, {%2, %6};\n"
+      "  @q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p; }"
+      ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(one), "n"(kDescHigh)
       : "memory");
 }
-// N-major SWIZZLE_128B operand: rows of 64 n (128 bytes), one per k; 8 k to a
-// 1024-byte atom (stride offset), the next 64 n `atom` bytes on (leading offset).
-__device__ __forceinline__ uint64_t sw128_desc_mn(uint32_t addr, uint32_t atom) {
-  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(atom >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+// D(tmem) (+)= A(tmem) . B(smem)
+__device__ __forceinline__ void umma_ts_one(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc, uint32_t one) {
+  asm volatile(
+      "{ .reg .pred p, q; .reg .b64 y; setp.ne.b32 p, %4, 0; setp.ne.b32 q, %5, 0; mov.b64 y, {%2, %6};\n"
+      "  @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p; }"
+      ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(one), "n"(kDescHigh)
+      : "memory");
 }
+__device__ __forceinline__ void commit_one(uint32_t bar, uint32_t one) {
+  asm volatile(
+      "{ .reg .pred q; setp.ne.b32 q, %1, 0;\n"
+      "  @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0]; }" ::"r"(bar), "r"(one) : "memory");
+}
+// Low descriptor words.  q and K: rows of 64 k (128 bytes), 8 to an atom.  V is
+// N-major: rows of 64 n, one per k, 8 k to an atom, the next 64 n 16 KiB on.
+__device__ __forceinline__ uint32_t desc_k(uint32_t addr) { return ((addr & 0x3FFFFu) >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_mn(uint32_t addr) { return ((addr & 0x3FFFFu) >> 4) | ((16384u >> 4) << 16); }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
@@ -74,7 +96,23 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
         "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
         "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
       : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// (a, b) <- (a, b) f + c and (a, b) <- (a, b) + (c, d), both halves in one instruction
+__device__ __forceinline__ void fma2(float& a, float& b, float f, float c) {
+  asm("{ .reg .b64 x, y, z; mov.b64 x, {%0, %1}; mov.b64 y, {%2, %2}; mov.b64 z, {%3, %3};\n"
+      "  fma.rn.f32x2 x, x, y, z; mov.b64 {%0, %1}, x; }"
+      : "+f"(a), "+f"(b) : "f"(f), "f"(c));
+}
+__device__ __forceinline__ void add2(float& a, float& b, float c, float d) {
+  asm("{ .reg .b64 x, y; mov.b64 x, {%0, %1}; mov.b64 y, {%2, %3};\n"
+      "  add.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x; }"
+      : "+f"(a), "+f"(b) : "f"(c), "f"(d));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 __device__ __forceinline__ void sts16(uint32_t p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(p), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
@@ -97,8 +135,8 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
   __shared__ __align__(1024) uint64_t s_bars[32];
   __shared__ PreMeta s_meta[4][8];   // by tile, four deep: read after the tile's stage may be refilled
   __shared__ float s_fq[2][RG];      // by stretch: score factor of each row
+  __shared__ int s_seg[2];           // by stretch, for the MMA warp: tiles * 2 + B in use; 0: the end
   __shared__ uint32_t s_tmem;
-  __shared__ unsigned s_ticket;
   const uint32_t raw = su32(smem_raw), base = (raw + 1023u) & ~1023u;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   auto q_addr = [&](int x) { return base + (uint32_t)(x * TILE); };
@@ -139,14 +177,18 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
   auto o_col = [&](int x) { return tmem + 256u + (uint32_t)(x * 128); };
   bool ok = true;
 
-  if (warp >= kPreLoad) {
+  if (warp >= kPreLoad && warp < kPreMma) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     // ---- widening: codes -> f16 operand tiles ------------------------------------
     const int lt = tid - kPreLoad * 32;  // 0 .. 255
     constexpr int CPR = HD / 16;         // 16-code pieces per token
     constexpr int PC = 128 * CPR / kPreLoaders;  // pieces per thread of K (and of V)
-    constexpr int TSTEP = kPreLoaders / CPR;     // tokens between a thread's pieces
-    const int ch = lt % CPR, tok0 = lt / CPR;
+    constexpr int TSTEP = kPreLoaders / CPR;     // tokens between a thread's pieces: 32, or 64
+    // 8 neighbouring lanes take two tokens' 64 dims: their stores meet 8 bank groups
+    const int ch = (lt & 3) | (HD == 128 ? (lt >> 1) & 4 : 0);
+    const int tok0 = (HD == 128 ? (lt >> 4) << 1 : (lt >> 3) << 1) | ((lt >> 2) & 1);
     const int lg = a.block_log2;
+    const uint32_t block_bytes = (uint32_t)(a.heads << lg) * HD;
     int n_tile = 0, n_seg = 0, r = kv_find(s_batch, a.requests, v0);
     for (int v = v0; v < v1 && ok;) {
       KvSeg s;
@@ -154,94 +196,102 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
       v = min(s.pair_end, v1);
       if (s.tile >= s.tile_end) continue;
       const int32_t* row_table = a.table + (size_t)s.r * a.width;
-      // block ids of this thread's tokens in tile x; -1 past the end or outside the pool
-      auto load_ids = [&](int x, int (&id)[PC]) {
-#pragma unroll
-        for (int i = 0; i < PC; ++i) {
-          const long long t = (long long)x * kPreTok + tok0 + i * TSTEP;
-          id[i] = x < s.tile_end && t < s.len ? row_table[t >> lg] : -1;
-        }
+      const uint32_t head_off = (uint32_t)(s.h << lg) * HD + ch * 16;
+      // lane i < 8: block of the i-th 16 tokens of tile x; -1 past the end or
+      // outside the pool
+      auto load_id = [&](int x) {
+        const long long t = (long long)x * kPreTok + lane * 16;
+        int id = -1;
+        if (lane < 8 && x < s.tile_end && t < s.len) id = row_table[t >> lg];
+        return id < a.blocks ? id : -1;
       };
-      auto load_codes = [&](const uint8_t* src, int x, const int (&id)[PC], uint4 (&w)[PC]) {
+      // and its exponents, K's | V's << 8
+      auto load_exp = [&](int id) -> uint32_t {
+        if (id < 0) return 127u | (127u << 8);
+        const size_t cell = (size_t)id * a.heads + s.h;
+        return (uint32_t)__ldg(a.ks + cell) | ((uint32_t)__ldg(a.vs + cell) << 8);
+      };
+      auto load_codes = [&](const uint8_t* src, int x, int id, uint4 (&w)[PC]) {
+        const int room = s.len - x * kPreTok;  // tokens of tile x (and more)
 #pragma unroll
         for (int i = 0; i < PC; ++i) {
+          const int t = tok0 + i * TSTEP;
+          const int b = __shfl_sync(0xFFFFFFFFu, id, t >> 4);
           w[i] = make_uint4(0, 0, 0, 0);
-          if (id[i] >= 0 && id[i] < a.blocks) {
-            const int t = x * kPreTok + tok0 + i * TSTEP;
-            const size_t at = ((((size_t)id[i] * a.heads + s.h) << lg) + (t & ((1 << lg) - 1))) * HD + ch * 16;
-            w[i] = __ldg(reinterpret_cast<const uint4*>(src + at));
-          }
+          if (b >= 0 && t < room)
+            w[i] = __ldg(reinterpret_cast<const uint4*>(src + (uint64_t)(uint32_t)b * block_bytes + head_off +
+                                                        (t & ((1 << lg) - 1)) * HD));
         }
       };
       auto widen = [&](uint32_t dst, const uint4 (&w)[PC]) {
 #pragma unroll
         for (int i = 0; i < PC; ++i) {
           const int row = tok0 + i * TSTEP;
-          // lanes of odd atoms store their halves the other way round, so that
-          // 8 lanes meet 8 bank groups
-          const int sw = (ch >> 2) & 1, c = 2 * (ch & 3) + sw;
-          const uint32_t u[4] = {sw ? w[i].z : w[i].x, sw ? w[i].w : w[i].y, sw ? w[i].x : w[i].z, sw ? w[i].y : w[i].w};
+          const int c = 2 * (ch & 3);
+          const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
           uint32_t o[8];
 #pragma unroll
           for (int y = 0; y < 4; ++y) codes4_to_f16<TYPE>(u[y], o[2 * y], o[2 * y + 1]);
           const uint32_t p = dst + (uint32_t)(ch >> 2) * 16384u;
           sts16(p + sw128_off(row, c), o[0], o[1], o[2], o[3]);
-          sts16(p + sw128_off(row, c ^ 1), o[4], o[5], o[6], o[7]);
+          sts16(p + sw128_off(row, c + 1), o[4], o[5], o[6], o[7]);
         }
       };
-      // block exponents of group lt of tile x (threads 0..7): K's | V's << 8
-      auto meta_id = [&](int x) {
-        const long long t = (long long)x * kPreTok + lt * 16;
-        return lt < 8 && x < s.tile_end && t < s.len ? row_table[t >> lg] : -1;
-      };
-      auto meta_of = [&](int id) -> uint32_t {
-        if (id < 0 || id >= a.blocks) return 127u | (127u << 8);
-        const size_t cell = (size_t)id * a.heads + s.h;
-        return (uint32_t)a.ks[cell] | ((uint32_t)a.vs[cell] << 8);
-      };
       // codes and exponents are loaded one tile ahead, block ids two
-      int id[PC];
       uint4 wk[PC], wv[PC];
-      load_ids(s.tile, id);
-      int id_m = meta_id(s.tile);
+      int id = load_id(s.tile);
       load_codes(a.k, s.tile, id, wk);
       load_codes(a.v, s.tile, id, wv);
-      uint32_t meta = meta_of(id_m);
-      load_ids(s.tile + 1, id);
-      id_m = meta_id(s.tile + 1);
+      uint32_t exps = load_exp(id);
+      id = load_id(s.tile + 1);
       // q: 16 (8 for 64 dims) lanes a row
       if (n_seg > 0) ok = pre_wait(bar(Q_EMPTY), (n_seg - 1) & 1);
-      if (ok) {
+      if (!ok) break;
+      {
         constexpr int LPR = HD / 8;  // lanes per row
         constexpr int STEP = kPreLoaders / LPR;
         const int c8 = lt % LPR;
-#pragma unroll 4
-        for (int rr = lt / LPR; rr < RG; rr += STEP) {
-          const int row = s.row0 + rr;
-          uint4 w = make_uint4(0, 0, 0, 0);
-          if (row < s.rows) {
-            const int i = row / a.group, gh = row - i * a.group;
-            w = __ldg(reinterpret_cast<const uint4*>(a.q + (int64_t)(s.start + i) * a.q_stride +
-                                                     (int64_t)(s.h * a.group + gh) * a.q_head_stride + c8 * 8));
+        // row0 + x over group, x < 256: exact in float
+        const int i0 = s.row0 / a.group, g0 = s.row0 - i0 * a.group;
+        const float inv_group = 1.0f / (float)a.group;
+        const int rows = min(RG, s.rows - s.row0);
+#pragma unroll 1
+        for (int r0 = lt / LPR; r0 < RG; r0 += 4 * STEP) {
+          uint4 w[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const int rr = r0 + y * STEP;
+            const int i = (int)(((float)(g0 + rr) + 0.5f) * inv_group), gh = g0 + rr - i * a.group;
+            w[y] = make_uint4(0, 0, 0, 0);
+            if (rr < rows)
+              w[y] = __ldg(reinterpret_cast<const uint4*>(a.q + (int64_t)(s.start + i0 + i) * a.q_stride +
+                                                          (int64_t)(s.h * a.group + gh) * a.q_head_stride + c8 * 8));
           }
-          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-          uint32_t mx = 0;
 #pragma unroll
-          for (int y = 0; y < 4; ++y) mx = max(mx, max(u[y] & 0x7FFFu, (u[y] >> 16) & 0x7FFFu));
+          for (int y = 0; y < 4; ++y) {
+            const int rr = r0 + y * STEP;
+            const uint32_t u[4] = {w[y].x, w[y].y, w[y].z, w[y].w};
+            uint32_t mx = 0;
 #pragma unroll
-          for (int d = 1; d < LPR; d <<= 1) mx = max(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, d));
-          const int e = mx >= 0x7F80u || mx < 0x0080u ? 0 : min((int)(mx >> 7) - 127, 126);
-          // the sign of the scale goes into q, so that factors are never negative
-          const float down = a.scale_log2 < 0.0f ? -pow2f(-e) : pow2f(-e);
-          uint32_t o[4];
+            for (int z = 0; z < 4; ++z) mx = max(mx, max(u[z] & 0x7FFFu, (u[z] >> 16) & 0x7FFFu));
 #pragma unroll
-          for (int y = 0; y < 4; ++y) o[y] = pack_f16(u2f(u[y] << 16) * down, u2f(u[y] & 0xFFFF0000u) * down);
-          sts16(q_addr(rr >> 7) + (uint32_t)(c8 >> 3) * 16384u + sw128_off(rr & 127, c8 & 7), o[0], o[1], o[2], o[3]);
-          if (c8 == 0) s_fq[n_seg & 1][rr] = fabsf(a.scale_log2) * pow2f(e);
+            for (int d = 1; d < LPR; d <<= 1) mx = max(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, d));
+            const int e = mx >= 0x7F80u || mx < 0x0080u ? 0 : min((int)(mx >> 7) - 127, 126);
+            // the sign of the scale goes into q, so that factors are never negative
+            const float down = a.scale_log2 < 0.0f ? -pow2f(-e) : pow2f(-e);
+            uint32_t o[4];
+#pragma unroll
+            for (int z = 0; z < 4; ++z) o[z] = pack_f16(u2f(u[z] << 16) * down, u2f(u[z] & 0xFFFF0000u) * down);
+            sts16(q_addr(rr >> 7) + (uint32_t)(c8 >> 3) * 16384u + sw128_off(rr & 127, c8 & 7), o[0], o[1], o[2], o[3]);
+            if (c8 == 0) s_fq[n_seg & 1][rr] = fabsf(a.scale_log2) * pow2f(e);
+          }
         }
+        // the MMA warp's view of the stretch: tiles, and whether B has rows
+        if (lt == 0) s_seg[n_seg & 1] = (s.tile_end - s.tile) * 2 + (rows > 128 ? 1 : 0);
         fence_proxy_async();
         mbar_arrive(bar(Q_FULL));
       }
+#pragma unroll 1
       for (int x = s.tile; x < s.tile_end && ok; ++x, ++n_tile) {
         const int st = n_tile & 1;
         const uint32_t par = (uint32_t)(n_tile >> 1) & 1u;
@@ -249,84 +299,100 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
         if (!ok) break;
         widen(k_addr(st), wk);
         if (lt < 8) {
-          const int ev = (int)(meta >> 8) - 127;
-          s_meta[n_tile & 3][lt] = PreMeta{u2f((meta & 0xFFu) << 23), (float)ev, pow2f(-ev), 0.0f};
+          const int ev = (int)(exps >> 8) - 127;
+          s_meta[n_tile & 3][lt] = PreMeta{u2f((exps & 0xFFu) << 23), (float)ev, pow2f(-ev), 0.0f};
         }
         fence_proxy_async();
         mbar_arrive(bar(K_FULL + st));
         load_codes(a.k, x + 1, id, wk);
-        meta = meta_of(id_m);
+        exps = load_exp(id);
         if (n_tile >= 2) ok = pre_wait(bar(V_EMPTY + st), par ^ 1u);
         if (!ok) break;
         widen(v_addr(st), wv);
         fence_proxy_async();
         mbar_arrive(bar(V_FULL + st));
         load_codes(a.v, x + 1, id, wv);
-        load_ids(x + 2, id);
-        id_m = meta_id(x + 2);
+        id = load_id(x + 2);
       }
       ++n_seg;
     }
-  } else if (warp == kPreMma) {
-    if (lane == 0) {
+    // no stretch is left
+    if (n_seg > 0 && ok) ok = pre_wait(bar(Q_EMPTY), (n_seg - 1) & 1);
+    if (ok) {
+      if (lt == 0) s_seg[n_seg & 1] = 0;
+      mbar_arrive(bar(Q_FULL));
+    }
+  } else if (warp >= kPreMma) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == kPreMma) {
       constexpr uint32_t id_qk = idesc_f16(128, kPreTok), id_pv = idesc_f16(128, HD) | (1u << 16);
-      int n_tile = 0, n_seg = 0, r = kv_find(s_batch, a.requests, v0);
-      uint32_t p_par[2] = {0, 0};
-      for (int v = v0; v < v1 && ok;) {
-        KvSeg s;
-        kv_seg<RG, TL>(a, s_batch, r, v, v1, s);
-        v = min(s.pair_end, v1);
-        const int nt = s.tile_end - s.tile;
-        if (nt <= 0) continue;
-        const int nx = s.rows - s.row0 > 128 ? 2 : 1;  // row tiles in use
-        auto qk = [&](int x, int st) {
+      const uint32_t one = lane == 0, tm = __reduce_or_sync(0xFFFFFFFFu, tmem);  // uniform
+      auto wait = [&](int b, uint32_t parity) { return __all_sync(0xFFFFFFFFu, pre_wait(bar(b), parity)) != 0; };
+      auto qk = [&](int x, int st) {
+        const uint32_t q = desc_k(q_addr(x)), k = desc_k(k_addr(st));
 #pragma unroll
-          for (int kk = 0; kk < HD / 16; ++kk) {
-            const uint32_t o = (uint32_t)(kk >> 2) * 16384u + (uint32_t)(kk & 3) * 32u;
-            umma_f16_ss(s_col(x), sw128_desc(q_addr(x) + o), sw128_desc(k_addr(st) + o), id_qk, kk != 0);
-          }
-          umma_commit(bar(S_FULL + x));
-        };
-        auto pv = [&](int x, int st, bool first) {
-#pragma unroll
-          for (int kk = 0; kk < kPreTok / 16; ++kk)
-            umma_f16_ts(o_col(x), s_col(x) + (uint32_t)(kk * 8), sw128_desc_mn(v_addr(st) + (uint32_t)kk * 2048u, 16384u),
-                        id_pv, !(first && kk == 0));
-        };
-        ok = pre_wait(bar(Q_FULL), n_seg & 1) && pre_wait(bar(K_FULL + (n_tile & 1)), (n_tile >> 1) & 1);
-        if (!ok) break;
-        tc_fence_after();
-        for (int x = 0; x < nx; ++x) qk(x, n_tile & 1);
-        umma_commit(bar(K_EMPTY + (n_tile & 1)));
-        if (nt == 1) umma_commit(bar(Q_EMPTY));
-        for (int j = 0; j < nt && ok; ++j, ++n_tile) {
-          const int st = n_tile & 1, nst = (n_tile + 1) & 1;
-          ok = pre_wait(bar(V_FULL + st), (n_tile >> 1) & 1);
-          for (int x = 0; x < nx && ok; ++x) {
-            ok = pre_wait(bar(P_FULL + x), p_par[x]);
-            if (!ok) break;
-            p_par[x] ^= 1u;
-            tc_fence_after();
-            pv(x, st, j == 0);
-            if (j + 1 < nt) {
-              if (x == 0) {
-                ok = pre_wait(bar(K_FULL + nst), ((n_tile + 1) >> 1) & 1);
-                if (!ok) break;
-                tc_fence_after();
-              }
-              qk(x, nst);
-            } else {
-              umma_commit(bar(O_FULL + x));
-            }
-          }
-          umma_commit(bar(V_EMPTY + st));
-          if (j + 1 < nt) umma_commit(bar(K_EMPTY + nst));
-          if (j + 2 == nt) umma_commit(bar(Q_EMPTY));
+        for (int kk = 0; kk < HD / 16; ++kk) {
+          const uint32_t o = ((uint32_t)(kk >> 2) * 16384u + (uint32_t)(kk & 3) * 32u) >> 4;
+          umma_ss_one(tm + x * 128u, q + o, k + o, id_qk, kk != 0, one);
         }
-        ++n_seg;
+        commit_one(bar(S_FULL + x), one);
+      };
+      auto pv = [&](int x, int st, uint32_t acc) {
+        const uint32_t vd = desc_mn(v_addr(st));
+#pragma unroll
+        for (int kk = 0; kk < kPreTok / 16; ++kk)
+          umma_ts_one(tm + 256u + x * 128u, tm + x * 128u + (uint32_t)(kk * 8), vd + (uint32_t)(kk * 128), id_pv, kk > 0 ? 1u : acc, one);
+      };
+      uint32_t st = 0, par = 0;        // stage of the next tile's K, phase of its barrier
+      uint32_t pa = 0, pb = 0;         // phases of W full, A and B
+#pragma unroll 1
+      for (int n_seg = 0; ok; ++n_seg) {
+        ok = wait(Q_FULL, n_seg & 1);
+        if (!ok) break;
+        const int seg = (int)__reduce_or_sync(0xFFFFFFFFu, (unsigned)*const_cast<volatile int*>(&s_seg[n_seg & 1]));
+        const int nt = seg >> 1;
+        const bool two = seg & 1;
+        if (nt == 0) break;
+        // step j issues W.V of tile j - 1 and q.K of tile j, A's before B's
+#pragma unroll 1
+        for (int j = 0; j <= nt && ok; ++j) {
+          const uint32_t old = st ^ 1u, old_par = st ? par : par ^ 1u;  // the tile before
+          const bool more = j < nt;
+          if (j > 0) {
+            ok = wait(V_FULL + old, old_par) && wait(P_FULL, pa);
+            pa ^= 1u;
+            tc_fence_after();
+            pv(0, old, j > 1);
+          }
+          if (more) {
+            ok = ok && wait(K_FULL + st, par);
+            tc_fence_after();
+            qk(0, st);
+          } else {
+            commit_one(bar(O_FULL), one);
+          }
+          if (two) {
+            if (j > 0) {
+              ok = ok && wait(P_FULL + 1, pb);
+              pb ^= 1u;
+              tc_fence_after();
+              pv(1, old, j > 1);
+            }
+            if (more) qk(1, st);
+            else commit_one(bar(O_FULL + 1), one);
+          }
+          if (j > 0) commit_one(bar(V_EMPTY + old), one);
+          if (more) {
+            commit_one(bar(K_EMPTY + st), one);
+            if (j + 1 == nt) commit_one(bar(Q_EMPTY), one);
+            st ^= 1u;
+            par ^= st ^ 1u;
+          }
+        }
       }
     }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
     // ---- softmax: one row per thread -----------------------------------------------
     const int x = warp >> 2;  // row tile
     const uint32_t quad = (uint32_t)(32 * (warp & 3)) << 16;
@@ -343,7 +409,8 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
       const bool used = x * 128 < s.rows - s.row0;
       const int row = s.row0 + rr;
       const bool on = row < s.rows;
-      float m = -INFINITY, l = 0.0f;
+      float m = 0.0f, l = 0.0f;
+      bool fresh = true;  // no visible token yet
       if (nt > 0 && used) {
         const int i = min(row, s.rows - 1) / a.group;
         const int lo = row_lo(a, s.len, s.n_all, i), hi = row_hi(a, s.len, s.n_all, i);
@@ -362,64 +429,88 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
           const int t0 = (s.tile + j) * kPreTok;
           auto tile = [&](auto masked) {
             constexpr bool MASK = decltype(masked)::value;
-            const int from = lo - t0, to = hi - t0;
-            float mx = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              uint32_t w[32];
-              tmem_ld32(sc + 32u * c, w);
-#pragma unroll
-              for (int g = 0; g < 2; ++g) {
-                float gm = -INFINITY;
-#pragma unroll
-                for (int y = 0; y < 16; ++y) {
-                  const int t = 32 * c + 16 * g + y;
-                  if (!MASK || (t >= from && t < to)) gm = fmaxf(gm, u2f(w[16 * g + y]));
-                }
-                const PreMeta mt = meta[2 * c + g];
-                if (!MASK || gm != -INFINITY) mx = fmaxf(mx, fmaf(gm, fq * mt.ks, mt.ev));
+            for (int h = 0; h < 2; ++h) {  // 64 tokens at a time
+              float p[64];
+              {
+                uint32_t (&w)[2][32] = reinterpret_cast<uint32_t (&)[2][32]>(p);
+                tmem_ld32(sc + 64u * h, w[0]);
+                tmem_ld32(sc + 64u * h + 32u, w[1]);
+                tmem_ld_wait();
               }
-            }
-            if (__any_sync(0xFFFFFFFFu, mx > m + kKvGrow)) {
-              const float mn = mx > m + kKvGrow ? mx - kKvTop : m;
-              const float al = mn == m ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - mn);
-              m = mn;
-              l *= al;
-              if (j > 0) {
-#pragma unroll 1
-                for (int c = 0; c < HD / 32; ++c) {
-                  uint32_t w[32];
-                  tmem_ld32(oc + 32u * c, w);
+              // exponents relative to m, and their maximum
+              float mx = -INFINITY;
 #pragma unroll
-                  for (int y = 0; y < 32; ++y) w[y] = f2u(u2f(w[y]) * al);
-                  tmem_st32(oc + 32u * c, w);
-                }
-              }
-            }
-            const float mu = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              uint32_t w[32], p[16];
-              tmem_ld32(sc + 32u * c, w);
-#pragma unroll
-              for (int g = 0; g < 2; ++g) {
-                const PreMeta mt = meta[2 * c + g];
-                const float f = fq * mt.ks, b = mt.ev - mu;
-                float sum = 0.0f;
+              for (int g = 0; g < 4; ++g) {
+                const float f = fq * meta[4 * h + g].ks, b = meta[4 * h + g].ev - m;
 #pragma unroll
                 for (int y = 0; y < 16; y += 2) {
-                  float e0 = ex2(fmaf(u2f(w[16 * g + y]), f, b)), e1 = ex2(fmaf(u2f(w[16 * g + y + 1]), f, b));
+                  const int t = 16 * g + y;
+                  fma2(p[t], p[t + 1], f, b);
                   if (MASK) {
-                    const int t = 32 * c + 16 * g + y;
-                    if (t < from || t >= to) e0 = 0.0f;
-                    if (t + 1 < from || t + 1 >= to) e1 = 0.0f;
+                    const int at = t0 + 64 * h + t;
+                    if (at < lo || at >= hi) p[t] = -INFINITY;
+                    if (at + 1 < lo || at + 1 >= hi) p[t + 1] = -INFINITY;
                   }
-                  sum += e0 + e1;
-                  p[8 * g + y / 2] = pack_f16(e0, e1);
+                  mx = max3(mx, p[t], p[t + 1]);
                 }
-                l = fmaf(sum, mt.inv, l);
               }
-              tmem_st16(sc + 16u * c, p);
+              // m moves, by a whole number, when a weight would pass 2^15, and at a
+              // row's first visible token (fresh: nothing is summed yet)
+              const bool move = mx > kKvGrow || (fresh && mx > -INFINITY);
+              if (__any_sync(0xFFFFFFFFu, move)) {
+                const float by = move ? fminf(ceilf(mx) - kKvTop, 1e30f) : 0.0f;
+                const bool scale = move && !fresh;  // by > 0
+                const int k = scale ? (int)fminf(by, 126.0f) : 0;
+                if (move) fresh = false;
+                m += by;
+                l *= pow2f(-k);
+#pragma unroll
+                for (int t = 0; t < 64; t += 2) add2(p[t], p[t + 1], -by, -by);
+                if (__any_sync(0xFFFFFFFFu, scale)) {
+                  if (j > 0) {
+                    const float al = pow2f(-k);
+#pragma unroll 1
+                    for (int c = 0; c < HD / 16; ++c) {
+                      uint32_t w[16];
+                      tmem_ld16(oc + 16u * c, w);
+#pragma unroll
+                      for (int y = 0; y < 16; ++y) w[y] = f2u(u2f(w[y]) * al);
+                      tmem_st16(oc + 16u * c, w);
+                    }
+                  }
+                  if (h == 1) {  // the first half's weights, already stored
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    // in two steps: below 2^-24 a factor is 0, a weight times it need not be
+                    const uint32_t a0 = f16x2_pow2(-min(k, 20)), a1 = f16x2_pow2(min(k, 20) - k);
+#pragma unroll 1
+                    for (int c = 0; c < 2; ++c) {
+                      uint32_t w[16];
+                      tmem_ld16(sc + 16u * c, w);
+#pragma unroll
+                      for (int y = 0; y < 16; ++y) w[y] = hmul2_f16x2(hmul2_f16x2(w[y], a0), a1);
+                      tmem_st16(sc + 16u * c, w);
+                    }
+                  }
+                }
+              }
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                uint32_t w[16];
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                  float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+                  for (int y = 0; y < 16; y += 2) {
+                    const int t = 32 * c + 16 * g + y;
+                    const float e0 = ex2(p[t]), e1 = ex2(p[t + 1]);
+                    add2(s0, s1, e0, e1);
+                    w[8 * g + y / 2] = pack_f16(e0, e1);
+                  }
+                  l = fmaf(s0 + s1, meta[4 * h + 2 * c + g].inv, l);
+                }
+                tmem_st16(sc + 32u * h + 16u * c, w);
+              }
             }
           };
           if (t0 >= full_lo && t0 + kPreTok <= full_hi) tile(std::false_type{});
@@ -434,7 +525,6 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
       }
       // after a timeout the stretches that are left still go through the join, so
       // that the barrier below is met and the tickets return to zero
-      if (m == -INFINITY) m = 0.0f;  // l is 0, or NaN for a NaN score
       const bool whole = seg_v0 == s.pair_v && v == s.pair_end;
       const int c_first = cuts.share_of(s.pair_v);
       float* slot = a.partials + (size_t)(cta * 2 + (cta == c_first ? 1 : 0)) * Cfg::kSlot;
@@ -446,6 +536,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
         uint32_t w[32];
         if (nt > 0 && used) {
           tmem_ld32(oc + 32u * c, w);
+          tmem_ld_wait();
         } else {
 #pragma unroll
           for (int y = 0; y < 32; ++y) w[y] = 0u;
@@ -477,22 +568,6 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
         a.lse[at] = kv_lse(m, l);
       }
       tc_fence_before();  // O's reads are done before the next stretch's MMAs write it (through W full)
-      if (!whole) {
-        // the pair crosses CTAs: its last CTA to arrive joins them in order
-        const int c_last = cuts.share_of(s.pair_end - 1);
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        if (tid == 0) s_ticket = ticket_acq_rel(a.tickets + c_first);
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        if (s_ticket == (unsigned)(c_last - c_first)) {
-#pragma unroll 1
-          for (int qr = warp; qr < min(RG, s.rows - s.row0); qr += 8) {
-            const int jrow = s.row0 + qr, ji = jrow / a.group;
-            kv_store<RG, HD>(a, s.start + ji, s.h * a.group + jrow - ji * a.group,
-                             kv_join<RG, HD>(a.partials, Cfg::kSlot, c_first, c_last, qr));
-          }
-          if (tid == 0) a.tickets[c_first] = 0u;
-        }
-      }
       if (nt > 0) { n_tile += nt; ++n_seg; }
     }
   }
@@ -502,6 +577,69 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
   if (warp == kPreMma) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+// Joins the pairs that cross CTAs of k_kv_prefill (E of them, cut the same way):
+// CTA (c, y) takes rows 32 y .. of the pair that begins in CTA c and goes on.
+template <int HD>
+__global__ void __launch_bounds__(256) k_kv_prefill_join(const KvAttnArgs a, int grid) {
+  constexpr int RG = kPreRows, TL = kPreTokLog2, N4 = 32 * HD / 4 / 256;  // float4 per thread
+  __shared__ KvBatch s_batch;
+  __shared__ int s_scan[16];
+  const int tid = threadIdx.x;
+  int longest;
+  const int V = kv_line<RG, TL, 8>(a, s_batch, s_scan, longest);
+  const int E = max(1, min(grid, V)), c_first = blockIdx.x;
+  if (c_first + 1 >= E) return;
+  const KvCuts cuts(V, E);
+  const int v = cuts.at(c_first + 1);
+  KvSeg s;
+  int r = kv_find(s_batch, a.requests, v);
+  kv_seg<RG, TL>(a, s_batch, r, v, INT32_MAX, s);
+  const int rows = s.rows - s.row0 - (int)blockIdx.y * 32;  // of this CTA's 32
+  if (s.pair_v == v || s.pair_v < cuts.at(c_first) || rows <= 0) return;
+  const int c_last = cuts.share_of(s.pair_end - 1);
+  KvJoined<RG, 128> j[N4];  // 4 values each
+#pragma unroll
+  for (int i = 0; i < N4; ++i) {
+    j[i].M = -INFINITY;
+    j[i].L = 0.0f;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) j[i].acc[y] = 0.0f;
+  }
+#pragma unroll 1
+  for (int c = c_first; c <= c_last; ++c) {
+    const float* p = a.partials + (size_t)(c == c_first ? 2 * c + 1 : 2 * c) * PreCfg<HD>::kSlot;
+    float m[N4], l[N4];
+    float4 o[N4];
+#pragma unroll
+    for (int i = 0; i < N4; ++i) {
+      const int e4 = i * 256 + tid, qr = blockIdx.y * 32 + e4 * 4 / HD;
+      m[i] = __ldcg(p + RG * HD + qr);
+      l[i] = __ldcg(p + RG * HD + RG + qr);
+      o[i] = __ldcg(reinterpret_cast<const float4*>(p + blockIdx.y * 32 * HD) + e4);
+    }
+#pragma unroll
+    for (int i = 0; i < N4; ++i) {
+      if (l[i] == 0.0f) continue;
+      const float top = fmaxf(j[i].M, m[i]), f0 = ex2(j[i].M - top), f1 = ex2(m[i] - top);
+      j[i].M = top;
+      j[i].L = fmaf(l[i], f1, j[i].L * f0);
+      j[i].acc[0] = fmaf(o[i].x, f1, j[i].acc[0] * f0); j[i].acc[1] = fmaf(o[i].y, f1, j[i].acc[1] * f0);
+      j[i].acc[2] = fmaf(o[i].z, f1, j[i].acc[2] * f0); j[i].acc[3] = fmaf(o[i].w, f1, j[i].acc[3] * f0);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N4; ++i) {
+    const int e4 = i * 256 + tid, qr = e4 * 4 / HD, d = e4 * 4 % HD;
+    if (qr >= rows) continue;
+    const int row = s.row0 + blockIdx.y * 32 + qr, tk = row / a.group;
+    const int64_t at = (int64_t)(s.start + tk) * (a.heads * a.group) + s.h * a.group + row - tk * a.group;
+    const float f = kv_inv(j[i].L);
+    *reinterpret_cast<uint2*>(a.out + at * HD + d) =
+        make_uint2(pack_bf16(j[i].acc[0] * f, j[i].acc[1] * f), pack_bf16(j[i].acc[2] * f, j[i].acc[3] * f));
+    if (a.lse && d == 0) a.lse[at] = kv_lse(j[i].M, j[i].L);
   }
 }
 
@@ -518,6 +656,9 @@ static cudaError_t launch_prefill(const KvAttnArgs& a, int grid, cudaStream_t s)
     if (dev < 64) attr[dev] = true;
   }
   k_kv_prefill<TYPE, HD><<<grid, kPreWarps * 32, BYTES, s>>>(a);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  k_kv_prefill_join<HD><<<dim3((unsigned)grid, kPreRows / 32), 256, 0, s>>>(a, grid);
   return cudaGetLastError();
 }
 
