@@ -4,19 +4,24 @@
 //
 // A pair is (request, KV head, 256 rows), the rows being the request's new
 // tokens times the query heads that share the KV head, so grouped heads fill
-// the tile.  The rows are two TMEM tiles A and B of 128; per tile of 128
-// tokens
+// the tile.  The rows are two TMEM tiles A and B of 128; per 64 tokens
 //   S = q . K^T    kind::f16, q and K (codes widened to f16) in shared memory
 //   O += W . V     W from TMEM (over S's columns), V in shared memory as its
 //                  token rows lie (N-major operand)
-// and A's softmax runs while the tensor core works for B, and the reverse.
+// Each row tile has two S buffers, so the scores of the next 64 tokens are
+// there when a row's softmax gets to them: the tensor core issues, in turn for
+// A and B, W.V of step i - 2 and q.K of step i.  (With one buffer of 128 tokens
+// the softmax waited for its own W.V and q.K in every step: 351 us instead of
+// the 2048-row chunk's time below.)
 //
 // Warps (20): 0-3 and 4-7 the softmax of A and B, one row per thread (TMEM
 // lane = row), 64 scores in registers at a time; 8-15 widen q, K and V into the
 // swizzled operand tiles, their global loads one tile ahead in registers; 16
-// issues the MMAs.  Widening costs 2 conversions per 4 codes once per 256 rows.
+// and 17 issue the MMAs of A and B (a commit holds up the warp that issues it
+// for some 80 cycles: two warps overlap them).  Widening costs 2 conversions
+// per 4 codes once per 256 rows.
 // Registers go where the data waits: 128 a softmax thread, 80 a widening one,
-// 56 in the MMA warp's group (together no more than the launch's 640 x 96).
+// 56 in the MMA warps' group (together no more than the launch's 640 x 96).
 //
 // What bounds it: exponentials.  A row and token cost one ex2, 16 a clock and
 // SM, as long as its 2 x 2 x 128 multiply-adds take the tensor core at 128
@@ -55,7 +60,7 @@ struct PreCfg {
 __device__ __forceinline__ bool pre_wait(uint32_t bar, uint32_t parity) {
   return mbar_wait_flag(bar, parity, &g_kv_fault);
 }
-// The MMA warp runs its loop with all lanes and one of them issues (`one`), and
+// An MMA warp runs its loop with all lanes and one of them issues (`one`), and
 // descriptors are passed as their low words (address and leading offset; the
 // high word, stride offset 1024 and the 128-byte swizzle, is the same for all):
 // so they live in uniform registers.  With 64-bit descriptors in a one-lane
@@ -97,7 +102,17 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
         "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
       : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Waits for the loads into v (and all before).  v is an operand so that no use of
+// it can move in front of the wait.
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                 "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]),
+                 "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]),
+                 "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]),
+                 "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
+               :: "memory");
+}
 // (a, b) <- (a, b) f + c and (a, b) <- (a, b) + (c, d), both halves in one instruction
 __device__ __forceinline__ void fma2(float& a, float& b, float f, float c) {
   asm("{ .reg .b64 x, y, z; mov.b64 x, {%0, %1}; mov.b64 y, {%2, %2}; mov.b64 z, {%3, %3};\n"
@@ -135,7 +150,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
   __shared__ __align__(1024) uint64_t s_bars[32];
   __shared__ PreMeta s_meta[4][8];   // by tile, four deep: read after the tile's stage may be refilled
   __shared__ float s_fq[2][RG];      // by stretch: score factor of each row
-  __shared__ int s_seg[2];           // by stretch, for the MMA warp: tiles * 2 + B in use; 0: the end
+  __shared__ int s_seg[2];           // by stretch, for the MMA warps: tiles * 2 + B in use; 0: the end
   __shared__ uint32_t s_tmem;
   const uint32_t raw = su32(smem_raw), base = (raw + 1023u) & ~1023u;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -143,9 +158,11 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
   auto k_addr = [&](int st) { return base + (uint32_t)((2 + 2 * st) * TILE); };
   auto v_addr = [&](int st) { return base + (uint32_t)((3 + 2 * st) * TILE); };
   auto bar = [&](int i) { return su32(&s_bars[i]); };
-  // barriers: K and V stages full / empty, q full / empty, per row tile S full, W full, O full
-  constexpr int K_FULL = 0, K_EMPTY = 2, V_FULL = 4, V_EMPTY = 6, Q_FULL = 8, Q_EMPTY = 9, S_FULL = 10, P_FULL = 12,
-                O_FULL = 14;
+  // barriers: K and V stages full / empty, q full / empty; per row tile x
+  // and buffer h, 2 x + h: S full (and so the W.V before it done), W full, and the
+  // stretch's last two W.V done
+  constexpr int K_FULL = 0, K_EMPTY = 2, V_FULL = 4, V_EMPTY = 6, Q_FULL = 8, Q_EMPTY = 9, S_FULL = 10, P_FULL = 14,
+                O_DONE = 18;
 
   int longest;
   const int V = kv_line<RG, TL, 16>(a, s_batch, s_scan, longest);
@@ -158,11 +175,13 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(K_FULL + i), kPreLoaders); mbar_init(bar(V_FULL + i), kPreLoaders);
-      mbar_init(bar(K_EMPTY + i), 1); mbar_init(bar(V_EMPTY + i), 1);
-      mbar_init(bar(S_FULL + i), 1); mbar_init(bar(P_FULL + i), 128); mbar_init(bar(O_FULL + i), 1);
+      mbar_init(bar(K_EMPTY + i), 2); mbar_init(bar(V_EMPTY + i), 2);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(bar(S_FULL + i), 1); mbar_init(bar(P_FULL + i), 128); mbar_init(bar(O_DONE + i), 1);
     }
     mbar_init(bar(Q_FULL), kPreLoaders);
-    mbar_init(bar(Q_EMPTY), 1);
+    mbar_init(bar(Q_EMPTY), 2);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kPreMma) {
@@ -286,7 +305,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
             if (c8 == 0) s_fq[n_seg & 1][rr] = fabsf(a.scale_log2) * pow2f(e);
           }
         }
-        // the MMA warp's view of the stretch: tiles, and whether B has rows
+        // the MMA warps' view of the stretch: tiles, and whether B has rows
         if (lt == 0) s_seg[n_seg & 1] = (s.tile_end - s.tile) * 2 + (rows > 128 ? 1 : 0);
         fence_proxy_async();
         mbar_arrive(bar(Q_FULL));
@@ -324,69 +343,64 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
     }
   } else if (warp >= kPreMma) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == kPreMma) {
-      constexpr uint32_t id_qk = idesc_f16(128, kPreTok), id_pv = idesc_f16(128, HD) | (1u << 16);
+    if (warp < kPreMma + 2) {
+      constexpr uint32_t id_qk = idesc_f16(128, 64), id_pv = idesc_f16(128, HD) | (1u << 16);
       const uint32_t one = lane == 0, tm = __reduce_or_sync(0xFFFFFFFFu, tmem);  // uniform
-      auto wait = [&](int b, uint32_t parity) { return __all_sync(0xFFFFFFFFu, pre_wait(bar(b), parity)) != 0; };
-      auto qk = [&](int x, int st) {
-        const uint32_t q = desc_k(q_addr(x)), k = desc_k(k_addr(st));
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk) {
-          const uint32_t o = ((uint32_t)(kk >> 2) * 16384u + (uint32_t)(kk & 3) * 32u) >> 4;
-          umma_ss_one(tm + x * 128u, q + o, k + o, id_qk, kk != 0, one);
-        }
-        commit_one(bar(S_FULL + x), one);
-      };
-      auto pv = [&](int x, int st, uint32_t acc) {
-        const uint32_t vd = desc_mn(v_addr(st));
-#pragma unroll
-        for (int kk = 0; kk < kPreTok / 16; ++kk)
-          umma_ts_one(tm + 256u + x * 128u, tm + x * 128u + (uint32_t)(kk * 8), vd + (uint32_t)(kk * 128), id_pv, kk > 0 ? 1u : acc, one);
-      };
-      uint32_t st = 0, par = 0;        // stage of the next tile's K, phase of its barrier
-      uint32_t pa = 0, pb = 0;         // phases of W full, A and B
+      const uint32_t x = __reduce_or_sync(0xFFFFFFFFu, (unsigned)(warp - kPreMma));  // row tile
+      auto wait = [&](uint32_t b, uint32_t parity) { return __all_sync(0xFFFFFFFFu, pre_wait(bar(b), parity)) != 0; };
+      uint32_t st = 0, par = 0;   // stage and phase of the next tile's K
+      uint32_t sv = 0, parv = 0;  // and of the next tile's V
+      uint32_t pp = 0;            // phases of W full, one bit a buffer
 #pragma unroll 1
       for (int n_seg = 0; ok; ++n_seg) {
         ok = wait(Q_FULL, n_seg & 1);
         if (!ok) break;
         const int seg = (int)__reduce_or_sync(0xFFFFFFFFu, (unsigned)*const_cast<volatile int*>(&s_seg[n_seg & 1]));
-        const int nt = seg >> 1;
-        const bool two = seg & 1;
-        if (nt == 0) break;
-        // step j issues W.V of tile j - 1 and q.K of tile j, A's before B's
+        const int steps = seg & ~1;  // two to a tile
+        if (steps == 0) break;
+        const bool used = x == 0 || (seg & 1);
+        // step i: W.V of step i - 2, then q.K of step i into the buffer it frees
 #pragma unroll 1
-        for (int j = 0; j <= nt && ok; ++j) {
-          const uint32_t old = st ^ 1u, old_par = st ? par : par ^ 1u;  // the tile before
-          const bool more = j < nt;
-          if (j > 0) {
-            ok = wait(V_FULL + old, old_par) && wait(P_FULL, pa);
-            pa ^= 1u;
-            tc_fence_after();
-            pv(0, old, j > 1);
-          }
-          if (more) {
-            ok = ok && wait(K_FULL + st, par);
-            tc_fence_after();
-            qk(0, st);
-          } else {
-            commit_one(bar(O_FULL), one);
-          }
-          if (two) {
-            if (j > 0) {
-              ok = ok && wait(P_FULL + 1, pb);
-              pb ^= 1u;
+        for (int i = 0; i < steps + 2 && ok; ++i) {
+          const uint32_t h = (uint32_t)i & 1u, b = 2 * x + h;
+          if (i >= 2) {
+            if (h == 0) ok = wait(V_FULL + sv, parv);
+            if (used) {
+              ok = ok && wait(P_FULL + b, (pp >> h) & 1u);
+              pp ^= 1u << h;
               tc_fence_after();
-              pv(1, old, j > 1);
+              const uint32_t vd = desc_mn(v_addr(sv) + h * 8192u), acc = i > 2;
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                umma_ts_one(tm + 256u + x * 128u, tm + x * 128u + h * 64u + (uint32_t)(kk * 8), vd + (uint32_t)(kk * 128),
+                            id_pv, kk > 0 ? 1u : acc, one);
             }
-            if (more) qk(1, st);
-            else commit_one(bar(O_FULL + 1), one);
+            if (h == 1) {
+              commit_one(bar(V_EMPTY + sv), one);
+              sv ^= 1u;
+              parv ^= sv ^ 1u;
+            }
           }
-          if (j > 0) commit_one(bar(V_EMPTY + old), one);
-          if (more) {
-            commit_one(bar(K_EMPTY + st), one);
-            if (j + 1 == nt) commit_one(bar(Q_EMPTY), one);
-            st ^= 1u;
-            par ^= st ^ 1u;
+          if (i < steps) {
+            if (h == 0) ok = ok && wait(K_FULL + st, par);
+            if (used) {
+              tc_fence_after();
+              const uint32_t q = desc_k(q_addr(x)), k = desc_k(k_addr(st) + h * 8192u);
+#pragma unroll
+              for (int kk = 0; kk < HD / 16; ++kk) {
+                const uint32_t o = ((uint32_t)(kk >> 2) * 16384u + (uint32_t)(kk & 3) * 32u) >> 4;
+                umma_ss_one(tm + x * 128u + h * 64u, q + o, k + o, id_qk, kk != 0, one);
+              }
+              commit_one(bar(S_FULL + b), one);
+            }
+            if (h == 1) {
+              commit_one(bar(K_EMPTY + st), one);
+              if (i + 1 == steps) commit_one(bar(Q_EMPTY), one);
+              st ^= 1u;
+              par ^= st ^ 1u;
+            }
+          } else if (used) {
+            commit_one(bar(O_DONE + b), one);
           }
         }
       }
@@ -399,7 +413,8 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
     const uint32_t sc = s_col(x) + quad, oc = o_col(x) + quad;
     const int rr = x * 128 + (warp & 3) * 32 + lane;
     int n_tile = 0, n_seg = 0, r = kv_find(s_batch, a.requests, v0);
-    uint32_t s_par = 0, o_par = 0;
+    uint32_t s_par = 0;  // phases of S full, one bit per buffer
+    uint32_t o_par = 0;  // phase of W.V done, one a stretch
     for (int v = v0; v < v1;) {
       KvSeg s;
       kv_seg<RG, TL>(a, s_batch, r, v, v1, s);
@@ -414,112 +429,103 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
       if (nt > 0 && used) {
         const int i = min(row, s.rows - 1) / a.group;
         const int lo = row_lo(a, s.len, s.n_all, i), hi = row_hi(a, s.len, s.n_all, i);
-        // tiles that every row of this warp sees whole need no mask
+        // steps that every row of this warp sees whole need no mask
         const int wrow = s.row0 + x * 128 + (warp & 3) * 32;
         const int full_lo = row_lo(a, s.len, s.n_all, min(wrow + 31, s.rows - 1) / a.group);
         const int full_hi = row_hi(a, s.len, s.n_all, min(wrow, s.rows - 1) / a.group);
         float fq = 0.0f;
-        for (int j = 0; j < nt && ok; ++j) {
-          ok = pre_wait(bar(S_FULL + x), s_par);
+#pragma unroll 1
+        for (int j = 0; j < 2 * nt && ok; ++j) {
+          const int h = j & 1;
+          ok = pre_wait(bar(S_FULL + 2 * x + h), (s_par >> h) & 1u);
           if (!ok) break;
-          s_par ^= 1u;
+          s_par ^= 1u << h;
           tc_fence_after();
           if (j == 0) fq = s_fq[n_seg & 1][rr];
-          const PreMeta* meta = s_meta[(n_tile + j) & 3];
-          const int t0 = (s.tile + j) * kPreTok;
-          auto tile = [&](auto masked) {
+          const PreMeta* meta = s_meta[(n_tile + (j >> 1)) & 3] + 4 * h;
+          const int t0 = s.tile * kPreTok + j * 64;
+          const uint32_t scol = sc + 64u * h;
+          auto step = [&](auto masked) {
             constexpr bool MASK = decltype(masked)::value;
+            float p[64];
+            {
+              uint32_t (&w)[2][32] = reinterpret_cast<uint32_t (&)[2][32]>(p);
+              tmem_ld32(scol, w[0]);
+              tmem_ld32(scol + 32u, w[1]);
+              tmem_ld_wait(w[0]);
+              tmem_ld_wait(w[1]);
+            }
+            // exponents relative to m, and their maximum
+            float mx = -INFINITY;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {  // 64 tokens at a time
-              float p[64];
-              {
-                uint32_t (&w)[2][32] = reinterpret_cast<uint32_t (&)[2][32]>(p);
-                tmem_ld32(sc + 64u * h, w[0]);
-                tmem_ld32(sc + 64u * h + 32u, w[1]);
-                tmem_ld_wait();
-              }
-              // exponents relative to m, and their maximum
-              float mx = -INFINITY;
+            for (int g = 0; g < 4; ++g) {
+              const float f = fq * meta[g].ks, b = meta[g].ev - m;
 #pragma unroll
-              for (int g = 0; g < 4; ++g) {
-                const float f = fq * meta[4 * h + g].ks, b = meta[4 * h + g].ev - m;
-#pragma unroll
-                for (int y = 0; y < 16; y += 2) {
-                  const int t = 16 * g + y;
-                  fma2(p[t], p[t + 1], f, b);
-                  if (MASK) {
-                    const int at = t0 + 64 * h + t;
-                    if (at < lo || at >= hi) p[t] = -INFINITY;
-                    if (at + 1 < lo || at + 1 >= hi) p[t + 1] = -INFINITY;
-                  }
-                  mx = max3(mx, p[t], p[t + 1]);
+              for (int y = 0; y < 16; y += 2) {
+                const int t = 16 * g + y;
+                fma2(p[t], p[t + 1], f, b);
+                if (MASK) {
+                  if (t0 + t < lo || t0 + t >= hi) p[t] = -INFINITY;
+                  if (t0 + t + 1 < lo || t0 + t + 1 >= hi) p[t + 1] = -INFINITY;
                 }
-              }
-              // m moves, by a whole number, when a weight would pass 2^15, and at a
-              // row's first visible token (fresh: nothing is summed yet)
-              const bool move = mx > kKvGrow || (fresh && mx > -INFINITY);
-              if (__any_sync(0xFFFFFFFFu, move)) {
-                const float by = move ? fminf(ceilf(mx) - kKvTop, 1e30f) : 0.0f;
-                const bool scale = move && !fresh;  // by > 0
-                const int k = scale ? (int)fminf(by, 126.0f) : 0;
-                if (move) fresh = false;
-                m += by;
-                l *= pow2f(-k);
-#pragma unroll
-                for (int t = 0; t < 64; t += 2) add2(p[t], p[t + 1], -by, -by);
-                if (__any_sync(0xFFFFFFFFu, scale)) {
-                  if (j > 0) {
-                    const float al = pow2f(-k);
-#pragma unroll 1
-                    for (int c = 0; c < HD / 16; ++c) {
-                      uint32_t w[16];
-                      tmem_ld16(oc + 16u * c, w);
-#pragma unroll
-                      for (int y = 0; y < 16; ++y) w[y] = f2u(u2f(w[y]) * al);
-                      tmem_st16(oc + 16u * c, w);
-                    }
-                  }
-                  if (h == 1) {  // the first half's weights, already stored
-                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                    // in two steps: below 2^-24 a factor is 0, a weight times it need not be
-                    const uint32_t a0 = f16x2_pow2(-min(k, 20)), a1 = f16x2_pow2(min(k, 20) - k);
-#pragma unroll 1
-                    for (int c = 0; c < 2; ++c) {
-                      uint32_t w[16];
-                      tmem_ld16(sc + 16u * c, w);
-#pragma unroll
-                      for (int y = 0; y < 16; ++y) w[y] = hmul2_f16x2(hmul2_f16x2(w[y], a0), a1);
-                      tmem_st16(sc + 16u * c, w);
-                    }
-                  }
-                }
-              }
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                uint32_t w[16];
-#pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                  float s0 = 0.0f, s1 = 0.0f;
-#pragma unroll
-                  for (int y = 0; y < 16; y += 2) {
-                    const int t = 32 * c + 16 * g + y;
-                    const float e0 = ex2(p[t]), e1 = ex2(p[t + 1]);
-                    add2(s0, s1, e0, e1);
-                    w[8 * g + y / 2] = pack_f16(e0, e1);
-                  }
-                  l = fmaf(s0 + s1, meta[4 * h + 2 * c + g].inv, l);
-                }
-                tmem_st16(sc + 32u * h + 16u * c, w);
+                mx = max3(mx, p[t], p[t + 1]);
               }
             }
+            // m moves, by a whole number, when a weight would pass 2^15, and at a
+            // row's first visible token (fresh: nothing is summed yet)
+            const bool move = mx > kKvGrow || (fresh && mx > -INFINITY);
+            if (__any_sync(0xFFFFFFFFu, move)) {
+              const float by = move ? fminf(ceilf(mx) - kKvTop, 1e30f) : 0.0f;
+              const bool scale = move && !fresh;  // by > 0
+              const float al = pow2f(scale ? -(int)fminf(by, 126.0f) : 0);
+              if (move) fresh = false;
+              m += by;
+              l *= al;
+#pragma unroll
+              for (int t = 0; t < 64; t += 2) add2(p[t], p[t + 1], -by, -by);
+              if (j > 0 && __any_sync(0xFFFFFFFFu, scale)) {
+                // O holds the steps up to the last once its W.V is done: before the
+                // next step's q.K is, or for the last step, before the end is marked
+                const uint32_t b = 2 * x + (h ^ 1);
+                ok = __all_sync(0xFFFFFFFFu, j + 1 < 2 * nt ? pre_wait(bar(S_FULL + b), (s_par >> (h ^ 1)) & 1u)
+                                                            : pre_wait(bar(O_DONE + b), o_par));
+                tc_fence_after();
+#pragma unroll 1
+                for (int c = 0; c < HD / 32; ++c) {
+                  uint32_t w[32];
+                  tmem_ld32(oc + 32u * c, w);
+                  tmem_ld_wait(w);
+#pragma unroll
+                  for (int y = 0; y < 32; ++y) w[y] = f2u(u2f(w[y]) * al);
+                  tmem_st32(oc + 32u * c, w);
+                }
+              }
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              uint32_t w[16];
+#pragma unroll
+              for (int g = 0; g < 2; ++g) {
+                float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+                for (int y = 0; y < 16; y += 2) {
+                  const int t = 32 * c + 16 * g + y;
+                  const float e0 = ex2(p[t]), e1 = ex2(p[t + 1]);
+                  add2(s0, s1, e0, e1);
+                  w[8 * g + y / 2] = pack_f16(e0, e1);
+                }
+                l = fmaf(s0 + s1, meta[2 * c + g].inv, l);
+              }
+              tmem_st16(scol + 16u * c, w);
+            }
           };
-          if (t0 >= full_lo && t0 + kPreTok <= full_hi) tile(std::false_type{});
-          else tile(std::true_type{});
+          if (t0 >= full_lo && t0 + 64 <= full_hi) step(std::false_type{});
+          else step(std::true_type{});
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
           tc_fence_before();
-          mbar_arrive(bar(P_FULL + x));
+          mbar_arrive(bar(P_FULL + 2 * x + h));
         }
-        if (ok) ok = pre_wait(bar(O_FULL + x), o_par);
+        if (ok) ok = pre_wait(bar(O_DONE + 2 * x + 1), o_par);
         o_par ^= 1u;
         tc_fence_after();
       }
@@ -536,7 +542,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) k_kv_prefill(const KvAttnAr
         uint32_t w[32];
         if (nt > 0 && used) {
           tmem_ld32(oc + 32u * c, w);
-          tmem_ld_wait();
+          tmem_ld_wait(w);
         } else {
 #pragma unroll
           for (int y = 0; y < 32; ++y) w[y] = 0u;
