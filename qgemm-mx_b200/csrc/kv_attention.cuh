@@ -19,7 +19,6 @@
 
 namespace qg {
 
-constexpr int kKvMaxRequests = 1024;  // per launch: they are kept in shared memory
 
 struct KvAttnArgs {
   const uint8_t *k, *v, *ks, *vs;
@@ -94,8 +93,9 @@ __device__ __forceinline__ KvRequest kv_request(const KvAttnArgs& a, int start, 
 }
 // A launch's requests in shared memory: prefix sums of their places on the
 // line (below), row starts and lengths.
+template <int MOST>
 struct KvBatch {
-  int prefix[kKvMaxRequests + 1], start[kKvMaxRequests + 1], len[kKvMaxRequests];
+  int prefix[MOST + 1], start[MOST + 1], len[MOST];
   __device__ __forceinline__ KvRequest at(const KvAttnArgs& a, int r) const {
     return kv_request(a, start[r], start[r + 1], len[r]);
   }
@@ -142,8 +142,8 @@ struct KvSeg {
 // The stretch that begins at place v of the line and ends with its pair or at
 // v_end; r: a request at or before v's, moved to it.  Its loops are not
 // unrolled: code that runs once a stretch costs its instruction fetches.
-template <int RG, int TL>
-__device__ __forceinline__ void kv_seg(const KvAttnArgs& a, const KvBatch& b, int& r, int v, int v_end, KvSeg& s) {
+template <int RG, int TL, int MOST>
+__device__ __forceinline__ void kv_seg(const KvAttnArgs& a, const KvBatch<MOST>& b, int& r, int v, int v_end, KvSeg& s) {
 #pragma unroll 1
   while (b.prefix[r + 1] <= v) ++r;
   const KvRequest q = b.at(a, r);
@@ -191,7 +191,8 @@ struct KvCuts {
 };
 
 // The request whose pairs hold line position v (empty ones hold none).
-__device__ __forceinline__ int kv_find(const KvBatch& b, int requests, int v) {
+template <int MOST>
+__device__ __forceinline__ int kv_find(const KvBatch<MOST>& b, int requests, int v) {
   int lo = 0, hi = requests;
 #pragma unroll 1
   while (hi - lo > 1) {
@@ -204,8 +205,8 @@ __device__ __forceinline__ int kv_find(const KvBatch& b, int requests, int v) {
 // Fills the batch and returns the line's length; longest: the most places a
 // pair has, at most 2^15.  The first WARPS warps do the
 // work; all threads must call it.
-template <int RG, int TL, int WARPS>
-__device__ __forceinline__ int kv_line(const KvAttnArgs& a, KvBatch& b, int* scan, int& longest) {
+template <int RG, int TL, int WARPS, int MOST>
+__device__ __forceinline__ int kv_line(const KvAttnArgs& a, KvBatch<MOST>& b, int* scan, int& longest) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int base = 0;
   longest = 0;

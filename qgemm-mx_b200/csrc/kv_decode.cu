@@ -38,6 +38,7 @@ namespace qg {
 
 __device__ unsigned g_kv_decode_fault = 0;
 
+constexpr int kDecRequests = 1024;  // of a launch: they are kept in shared memory
 constexpr int kDecMinTiles = 2;   // tiles per warp below which the grid shrinks
 constexpr int kDecSnapTiles = 16;  // longest pair for which shares end with whole pairs
 constexpr float kDecLow = -1e30f;  // m before a row has seen a token
@@ -90,7 +91,7 @@ k_kv_decode(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
   using Cfg = DecCfg<HD, NT>;
   constexpr int RG = 8 * NT, KJ = HD / 64, MT = HD / 16, ST = Cfg::kStages, W = Cfg::kWarps;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ KvBatch s_batch;
+  __shared__ KvBatch<kDecRequests> s_batch;
   __shared__ int s_scan[2 * W];
   __shared__ __align__(1024) uint64_t s_bars[W * ST];
   __shared__ int s_cell[W * ST];   // a stage's (block, head)
@@ -568,8 +569,10 @@ static cudaError_t kv_decode_launch(int type, int head_dim, int nt, const CUtens
 #undef QG_DEC
 }
 
+extern const int kKvPrefillRequests;  // of a launch
 size_t kv_prefill_workspace(int head_dim, int sm_count);
-cudaError_t kv_prefill_launch(int type, int head_dim, const KvAttnArgs& a, int grid, cudaStream_t s);
+cudaError_t kv_prefill_launch(int type, int head_dim, const CUtensorMap& mk, const CUtensorMap& mv, const KvAttnArgs& a,
+                              int grid, cudaStream_t s);
 
 unsigned kv_decode_fault() {
   unsigned f = 0;
@@ -597,15 +600,11 @@ struct KvWorkspace {
 static qgemm_status_t kv_attention_run(const qgemm_kv_cache_t* c, KvAttnArgs a, void* ws, int sm_count, cudaStream_t s) {
   const long long rows = (long long)a.max_new * a.group;
   const KvWorkspace w(c->head_dim, rows, sm_count);
-  // K and V as rows of head_dim codes, copied 16 at a time
+  // K and V as rows of head_dim codes, copied 16 at a time: whole and swizzled for
+  // the decode kernel, 64 codes of a row for the prefill kernel
   const uint64_t code_rows = (uint64_t)c->blocks * c->heads * c->block;
   if (code_rows > INT32_MAX)
     return fail(QGEMM_ERR_UNSUPPORTED_SHAPE, "kv_attention: blocks x heads x block of the pool exceed 2^31 - 1");
-  CUtensorMap mk, mv;
-  const CUtensorMapSwizzle sw = c->head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
-  if (!make_tma_map_2d(&mk, CU_TENSOR_MAP_DATA_TYPE_UINT8, c->k, c->head_dim, code_rows, c->head_dim, c->head_dim, 16, sw) ||
-      !make_tma_map_2d(&mv, CU_TENSOR_MAP_DATA_TYPE_UINT8, c->v, c->head_dim, code_rows, c->head_dim, c->head_dim, 16, sw))
-    return fail(QGEMM_ERR_CUDA, "kv_attention: cuTensorMapEncodeTiled failed");
   const int all = a.requests;
   const int32_t *starts = a.starts, *lens = a.lens, *table = a.table;
   for (int kernel = rows > kKvPrefillRows ? 1 : 0; kernel >= 0; --kernel) {
@@ -614,18 +613,25 @@ static qgemm_status_t kv_attention_run(const qgemm_kv_cache_t* c, KvAttnArgs a, 
     a.tickets = reinterpret_cast<unsigned*>(static_cast<char*>(ws) + 4096 * kernel);
     a.partials = reinterpret_cast<float*>(static_cast<char*>(ws) + (kernel ? w.prefill : w.decode));
     const int nt = dec_nt(rows);
+    CUtensorMap mk, mv;
+    const CUtensorMapSwizzle sw = kernel ? CU_TENSOR_MAP_SWIZZLE_NONE
+                                  : c->head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+    const uint32_t box = kernel ? 64u : (uint32_t)c->head_dim;
+    if (!make_tma_map_2d(&mk, CU_TENSOR_MAP_DATA_TYPE_UINT8, c->k, c->head_dim, code_rows, c->head_dim, box, 16, sw) ||
+        !make_tma_map_2d(&mv, CU_TENSOR_MAP_DATA_TYPE_UINT8, c->v, c->head_dim, code_rows, c->head_dim, box, 16, sw))
+      return fail(QGEMM_ERR_CUDA, "kv_attention: cuTensorMapEncodeTiled failed");
     // requests per launch: the prefix sums fit shared memory and the line 31 bits
     const long long per = kernel ? kv_line_most(a, 256, 7) : kv_line_most(a, 8 * nt, 4);
     if (per > INT32_MAX)
       return fail(QGEMM_ERR_UNSUPPORTED_SHAPE, "kv_attention: a request's rows x heads x tokens exceed 2^31 tiles");
     long long most = INT32_MAX / per;
-    if (most > kKvMaxRequests) most = kKvMaxRequests;
+    if (most > (kernel ? kKvPrefillRequests : kDecRequests)) most = kernel ? kKvPrefillRequests : kDecRequests;
     for (int r0 = 0; r0 < all; r0 += (int)most) {
       a.requests = all - r0 < most ? all - r0 : (int)most;
       a.starts = starts + r0;
       a.lens = lens + r0;
       a.table = table + (size_t)r0 * a.width;
-      const cudaError_t e = kernel ? kv_prefill_launch(c->type, c->head_dim, a, sm_count, s)
+      const cudaError_t e = kernel ? kv_prefill_launch(c->type, c->head_dim, mk, mv, a, sm_count, s)
                                    : kv_decode_launch(c->type, c->head_dim, nt, mk, mv, a, sm_count, s);
       if (e != cudaSuccess) return fail(QGEMM_ERR_CUDA, "kv_attention: launch: %s", cudaGetErrorString(e));
     }
