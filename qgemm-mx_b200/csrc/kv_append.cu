@@ -51,6 +51,7 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append(const AppendArgs a
   __shared__ uint32_t s_max[kAppendThreads / 32];
   const int gl = threadIdx.x % GT;  // place in the group
   const unsigned item = blockIdx.x * (kAppendThreads / GT) + threadIdx.x / GT;
+  pdl_begin();
   if (item >= a.items) return;  // whole groups
   const unsigned run = item / (2u * a.heads), rest = item - run * 2u * a.heads;
   const int which = rest >= (unsigned)a.heads, h = (int)rest - (which ? a.heads : 0);
@@ -119,11 +120,11 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append(const AppendArgs a
 }
 
 template <int TYPE, int HD>
-static void launch_append(const AppendArgs& a, bool wide, cudaStream_t s) {
+static cudaError_t launch_append(const AppendArgs& a, bool wide, cudaStream_t s) {
   const unsigned per = wide ? 1 : kAppendThreads / 32;
   const unsigned grid = (a.items + per - 1) / per;
-  if (wide) k_kv_append<TYPE, HD, kAppendThreads><<<grid, kAppendThreads, 0, s>>>(a);
-  else k_kv_append<TYPE, HD, 32><<<grid, kAppendThreads, 0, s>>>(a);
+  return pdl_launch(wide ? k_kv_append<TYPE, HD, kAppendThreads> : k_kv_append<TYPE, HD, 32>, dim3(grid),
+                    dim3(kAppendThreads), 0, s, a);
 }
 
 }  // namespace qg
@@ -157,14 +158,10 @@ qgemm_status_t qgemm_kv_append(const qgemm_kv_cache_t* c, const uint16_t* k, con
   const int rows = (tokens + max_runs - 1) / max_runs;
   const bool wide = (rows < c->block ? rows : c->block) * c->head_dim / 8 > 32 * kAppendHeld;
   cudaStream_t s = as_stream(stream);
-  if (c->type == QGEMM_KV_E4M3) {
-    if (c->head_dim == 64) launch_append<QGEMM_KV_E4M3, 64>(a, wide, s);
-    else launch_append<QGEMM_KV_E4M3, 128>(a, wide, s);
-  } else {
-    if (c->head_dim == 64) launch_append<QGEMM_KV_INT8, 64>(a, wide, s);
-    else launch_append<QGEMM_KV_INT8, 128>(a, wide, s);
-  }
-  QG_LAUNCH_RET();
+  const bool d64 = c->head_dim == 64;
+  QG_CUDA_RET(c->type == QGEMM_KV_E4M3
+                  ? (d64 ? launch_append<QGEMM_KV_E4M3, 64>(a, wide, s) : launch_append<QGEMM_KV_E4M3, 128>(a, wide, s))
+                  : (d64 ? launch_append<QGEMM_KV_INT8, 64>(a, wide, s) : launch_append<QGEMM_KV_INT8, 128>(a, wide, s)));
   return QGEMM_OK;
 }
 

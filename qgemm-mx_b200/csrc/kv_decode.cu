@@ -112,6 +112,7 @@ k_kv_decode(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  pdl_begin();
   int longest;
   const int V = kv_line<RG, 4, W>(a, s_batch, s_scan, longest);
   // Short pairs are not cut: a share takes the pairs that begin in it.  One pair
@@ -553,8 +554,7 @@ static cudaError_t launch_decode(const CUtensorMap& mk, const CUtensorMap& mv, c
     if (e != cudaSuccess) return e;
     if (dev < 64) attr[dev] = true;
   }
-  k_kv_decode<TYPE, HD, NT><<<grid, DecCfg<HD, NT>::kWarps * 32, BYTES, s>>>(mk, mv, a);
-  return cudaGetLastError();
+  return pdl_launch(k_kv_decode<TYPE, HD, NT>, dim3((unsigned)grid), dim3(DecCfg<HD, NT>::kWarps * 32), BYTES, s, mk, mv, a);
 }
 
 // Two row tiles of 8 when a request brings more than 8 rows per KV head.
@@ -571,8 +571,7 @@ static cudaError_t kv_decode_launch(int type, int head_dim, int nt, const CUtens
 
 extern const int kKvPrefillRequests;  // of a launch
 size_t kv_prefill_workspace(int head_dim, int sm_count);
-cudaError_t kv_prefill_launch(int type, int head_dim, const CUtensorMap& mk, const CUtensorMap& mv, const KvAttnArgs& a,
-                              int grid, cudaStream_t s);
+cudaError_t kv_prefill_launch(int type, int head_dim, const KvAttnArgs& a, int grid, cudaStream_t s);
 
 unsigned kv_decode_fault() {
   unsigned f = 0;
@@ -600,26 +599,27 @@ struct KvWorkspace {
 static qgemm_status_t kv_attention_run(const qgemm_kv_cache_t* c, KvAttnArgs a, void* ws, int sm_count, cudaStream_t s) {
   const long long rows = (long long)a.max_new * a.group;
   const KvWorkspace w(c->head_dim, rows, sm_count);
-  // K and V as rows of head_dim codes, copied 16 at a time: whole and swizzled for
-  // the decode kernel, 64 codes of a row for the prefill kernel
+  // K and V as rows of head_dim codes, which the decode kernel copies 16 at a time
   const uint64_t code_rows = (uint64_t)c->blocks * c->heads * c->block;
   if (code_rows > INT32_MAX)
     return fail(QGEMM_ERR_UNSUPPORTED_SHAPE, "kv_attention: blocks x heads x block of the pool exceed 2^31 - 1");
+  CUtensorMap mk, mv;
+  const CUtensorMapSwizzle sw = c->head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+  if (!make_tma_map_2d(&mk, CU_TENSOR_MAP_DATA_TYPE_UINT8, c->k, c->head_dim, code_rows, c->head_dim, c->head_dim, 16, sw) ||
+      !make_tma_map_2d(&mv, CU_TENSOR_MAP_DATA_TYPE_UINT8, c->v, c->head_dim, code_rows, c->head_dim, c->head_dim, 16, sw))
+    return fail(QGEMM_ERR_CUDA, "kv_attention: cuTensorMapEncodeTiled failed");
   const int all = a.requests;
   const int32_t *starts = a.starts, *lens = a.lens, *table = a.table;
-  for (int kernel = rows > kKvPrefillRows ? 1 : 0; kernel >= 0; --kernel) {
-    a.rows_min = kernel ? kKvPrefillRows : 0;
+  // rows enough for max_new of every request: all bring as many, and one kernel
+  // takes whatever they bring
+  const bool even = (long long)a.requests * a.max_new <= a.tokens;
+  const int last = rows > kKvPrefillRows && even ? 1 : 0;
+  for (int kernel = rows > kKvPrefillRows ? 1 : 0; kernel >= last; --kernel) {
+    a.rows_min = kernel && !even ? kKvPrefillRows : 0;
     a.rows_max = kernel ? INT32_MAX : kKvPrefillRows;
     a.tickets = reinterpret_cast<unsigned*>(static_cast<char*>(ws) + 4096 * kernel);
     a.partials = reinterpret_cast<float*>(static_cast<char*>(ws) + (kernel ? w.prefill : w.decode));
     const int nt = dec_nt(rows);
-    CUtensorMap mk, mv;
-    const CUtensorMapSwizzle sw = kernel ? CU_TENSOR_MAP_SWIZZLE_NONE
-                                  : c->head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
-    const uint32_t box = kernel ? 64u : (uint32_t)c->head_dim;
-    if (!make_tma_map_2d(&mk, CU_TENSOR_MAP_DATA_TYPE_UINT8, c->k, c->head_dim, code_rows, c->head_dim, box, 16, sw) ||
-        !make_tma_map_2d(&mv, CU_TENSOR_MAP_DATA_TYPE_UINT8, c->v, c->head_dim, code_rows, c->head_dim, box, 16, sw))
-      return fail(QGEMM_ERR_CUDA, "kv_attention: cuTensorMapEncodeTiled failed");
     // requests per launch: the prefix sums fit shared memory and the line 31 bits
     const long long per = kernel ? kv_line_most(a, 256, 7) : kv_line_most(a, 8 * nt, 4);
     if (per > INT32_MAX)
@@ -631,7 +631,7 @@ static qgemm_status_t kv_attention_run(const qgemm_kv_cache_t* c, KvAttnArgs a, 
       a.starts = starts + r0;
       a.lens = lens + r0;
       a.table = table + (size_t)r0 * a.width;
-      const cudaError_t e = kernel ? kv_prefill_launch(c->type, c->head_dim, mk, mv, a, sm_count, s)
+      const cudaError_t e = kernel ? kv_prefill_launch(c->type, c->head_dim, a, sm_count, s)
                                    : kv_decode_launch(c->type, c->head_dim, nt, mk, mv, a, sm_count, s);
       if (e != cudaSuccess) return fail(QGEMM_ERR_CUDA, "kv_attention: launch: %s", cudaGetErrorString(e));
     }

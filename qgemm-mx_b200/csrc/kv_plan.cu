@@ -60,6 +60,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(const PlanArgs a) {
   __shared__ int s_warp[3][kPlanThreads / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int lg = a.block_log2;
+  pdl_begin();
   const int count = a.free_list ? max(*a.free_count, 0) : 0;
   // this CTA's rows
   const int t0 = (int)((long long)blockIdx.x * a.tokens / gridDim.x);
@@ -225,8 +226,7 @@ qgemm_status_t qgemm_kv_plan(int32_t block, int32_t requests, const int32_t* len
   if (st != QGEMM_OK) return st;
   int grid = (tokens + kPlanThreads - 1) / kPlanThreads;
   grid = grid < 1 ? 1 : grid > dp.sm_count ? dp.sm_count : grid;
-  k_kv_plan<<<grid, kPlanThreads, 0, as_stream(stream)>>>(a);
-  QG_LAUNCH_RET();
+  QG_CUDA_RET(pdl_launch(k_kv_plan, dim3((unsigned)grid), dim3(kPlanThreads), 0, as_stream(stream), a));
   return QGEMM_OK;
 }
 

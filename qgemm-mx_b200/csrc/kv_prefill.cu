@@ -16,12 +16,13 @@
 //
 // Warps (20): 0-3 and 4-7 the softmax of A and B, one row per thread (TMEM
 // lane = row), 64 scores in registers at a time; 8-15 widen q, K and V into the
-// swizzled operand tiles; 16 and 17 issue the MMAs of A and B (a commit holds up
-// the warp that issues it for some 80 cycles: two warps overlap them); 18 fetches
-// the codes by TMA into a ring of 64-token units, ahead of the widening.
-// Widening costs 2 conversions per 4 codes once per 256 rows.  Registers go where
-// the data waits: 136 a softmax thread, 72 a widening one, 48 in the last four
-// warps (together no more than the launch's 640 x 96).
+// swizzled operand tiles, their global loads one tile ahead in registers; 16 and
+// 17 issue the MMAs of A and B (a commit holds up the warp that issues it for some
+// 80 cycles: two warps overlap them).  Widening costs 2 conversions per 4 codes
+// once per 256 rows.  Registers go where the data waits: 128 a softmax thread, 80
+// a widening one, 56 in the MMA warps' group (together no more than the launch's
+// 640 x 96).  (Codes by TMA into a ring of 64-token units, the room that is left
+// beside the operand tiles, 24 KB: its round trip was longer than the ring.)
 //
 // What bounds it: exponentials.  A row and token cost one ex2, 16 a clock and
 // SM, as long as its 2 x 2 x 128 multiply-adds take the tensor core at 128
@@ -55,9 +56,7 @@ template <int HD>
 struct PreCfg {
   static constexpr int kTile = 128 * HD * 2;           // one f16 operand tile: 128 rows
   static constexpr int kQ = 2 * kTile;
-  static constexpr int kUnit = 64 * HD;                // codes of 64 tokens of K or V
-  static constexpr int kUnits = HD == 128 ? 3 : 6;
-  static constexpr int kSmem = kQ + 4 * kTile + kUnits * kUnit + 1024;  // q, two stages of K and V, codes, alignment
+  static constexpr int kSmem = kQ + 4 * kTile + 1024;  // q, two stages of K and V, alignment
   static constexpr int kSlot = kPreRows * (HD + 2);    // floats of a partial: O, m, l
 };
 
@@ -128,11 +127,6 @@ __device__ __forceinline__ void add2(float& a, float& b, float c, float d) {
       "  add.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x; }"
       : "+f"(a), "+f"(b) : "f"(c), "f"(d));
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
 __device__ __forceinline__ void sts16(uint32_t p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(p), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -146,13 +140,13 @@ struct PreMeta {
 
 template <int TYPE, int HD>
 __global__ void __launch_bounds__(kPreWarps * 32, 1)
-k_kv_prefill(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const KvAttnArgs a) {
+k_kv_prefill(const KvAttnArgs a) {
   using Cfg = PreCfg<HD>;
   constexpr int RG = kPreRows, TL = kPreTokLog2, TILE = Cfg::kTile;
   extern __shared__ uint8_t smem_raw[];
   __shared__ KvBatch<kKvPrefillRequests> s_batch;
   __shared__ int s_scan[32];
-  __shared__ __align__(1024) uint64_t s_bars[40];
+  __shared__ __align__(1024) uint64_t s_bars[32];
   __shared__ PreMeta s_meta[4][8];   // by tile, four deep: read after the tile's stage may be refilled
   __shared__ float s_fq[2][RG];      // by stretch: score factor of each row
   __shared__ int s_seg[2];           // by stretch, for the MMA warps: tiles * 2 + B in use; 0: the end
@@ -162,14 +156,14 @@ k_kv_prefill(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
   auto q_addr = [&](int x) { return base + (uint32_t)(x * TILE); };
   auto k_addr = [&](int st) { return base + (uint32_t)((2 + 2 * st) * TILE); };
   auto v_addr = [&](int st) { return base + (uint32_t)((3 + 2 * st) * TILE); };
-  auto raw_addr = [&](int u) { return base + (uint32_t)(6 * TILE + u * Cfg::kUnit); };
   auto bar = [&](int i) { return su32(&s_bars[i]); };
   // barriers: K and V stages full / empty, q full / empty; per row tile x
   // and buffer h, 2 x + h: S full (and so the W.V before it done), W full, and the
   // stretch's last two W.V done
   constexpr int K_FULL = 0, K_EMPTY = 2, V_FULL = 4, V_EMPTY = 6, Q_FULL = 8, Q_EMPTY = 9, S_FULL = 10, P_FULL = 14,
-                O_DONE = 18, U_FULL = 22, U_EMPTY = U_FULL + Cfg::kUnits;
+                O_DONE = 18;
 
+  pdl_begin();
   int longest;
   const int V = kv_line<RG, TL, 16>(a, s_batch, s_scan, longest);
   const int E = max(1, min((int)gridDim.x, V));
@@ -187,7 +181,6 @@ k_kv_prefill(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
       mbar_init(bar(S_FULL + i), 1); mbar_init(bar(P_FULL + i), 4); mbar_init(bar(O_DONE + i), 1);
     }
     mbar_init(bar(Q_FULL), kPreLoaders / 32);
-    for (int i = 0; i < Cfg::kUnits; ++i) { mbar_init(bar(U_FULL + i), 1); mbar_init(bar(U_EMPTY + i), kPreLoaders / 32); }
     mbar_init(bar(Q_EMPTY), 2);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -209,48 +202,72 @@ k_kv_prefill(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
   };
 
   if (warp >= kPreLoad && warp < kPreMma) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     // ---- widening: codes -> f16 operand tiles ------------------------------------
     const int lt = tid - kPreLoad * 32;  // 0 .. 255
-    // 8 neighbouring lanes take two tokens' 64 dims: their loads and stores meet 8
-    // bank groups
-    const int ch = lt & 3, atom = HD == 128 ? (lt >> 3) & 1 : 0;
+    constexpr int CPR = HD / 16;         // 16-code pieces per token
+    constexpr int PC = 128 * CPR / kPreLoaders;  // pieces per thread of K (and of V)
+    constexpr int TSTEP = kPreLoaders / CPR;     // tokens between a thread's pieces: 32, or 64
+    // 8 neighbouring lanes take two tokens' 64 dims: their stores meet 8 bank groups
+    const int ch = (lt & 3) | (HD == 128 ? (lt >> 1) & 4 : 0);
     const int tok0 = (HD == 128 ? (lt >> 4) << 1 : (lt >> 3) << 1) | ((lt >> 2) & 1);
+    const int lg = a.block_log2;
+    const uint32_t block_bytes = (uint32_t)(a.heads << lg) * HD;
     int n_tile = 0, n_seg = 0, r = kv_find(s_batch, a.requests, v0);
-    int u = 0;            // next unit of the ring, and its phase
-    uint32_t u_par = 0;
     for (int v = v0; v < v1 && ok;) {
       KvSeg s;
       kv_seg<RG, TL>(a, s_batch, r, v, v1, s);
       v = min(s.pair_end, v1);
       if (s.tile >= s.tile_end) continue;
-      // one unit into rows 64 h .. of an operand tile; room: tokens it may hold
-      auto widen = [&](uint32_t dst, int h, int room) {
-        ok = pre_wait(bar(U_FULL + u), u_par);
-        if (!ok) return;
-        uint4 w[HD / 64];
+      const int32_t* row_table = a.table + (size_t)s.r * a.width;
+      const uint32_t head_off = (uint32_t)(s.h << lg) * HD + ch * 16;
+      // lane i < 8: block of the i-th 16 tokens of tile x; -1 past the end or
+      // outside the pool
+      auto load_id = [&](int x) {
+        const long long t = (long long)x * kPreTok + lane * 16;
+        int id = -1;
+        if (lane < 8 && x < s.tile_end && t < s.len) id = row_table[t >> lg];
+        return id < a.blocks ? id : -1;
+      };
+      // and its exponents, K's | V's << 8
+      auto load_exp = [&](int id) -> uint32_t {
+        if (id < 0) return 127u | (127u << 8);
+        const size_t cell = (size_t)id * a.heads + s.h;
+        return (uint32_t)__ldg(a.ks + cell) | ((uint32_t)__ldg(a.vs + cell) << 8);
+      };
+      auto load_codes = [&](const uint8_t* src, int x, int id, uint4 (&w)[PC]) {
+        const int room = s.len - x * kPreTok;  // tokens of tile x (and more)
 #pragma unroll
-        for (int i = 0; i < HD / 64; ++i) {
-          const int row = tok0 + 32 * i;
-          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                       : "=r"(w[i].x), "=r"(w[i].y), "=r"(w[i].z), "=r"(w[i].w)
-                       : "r"(raw_addr(u) + (uint32_t)(atom * 4096 + row * 64 + ch * 16)) : "memory");
-          if (row >= room) w[i] = make_uint4(0, 0, 0, 0);  // behind the last token: not the request's
+        for (int i = 0; i < PC; ++i) {
+          const int t = tok0 + i * TSTEP;
+          const int b = __shfl_sync(0xFFFFFFFFu, id, t >> 4);
+          w[i] = make_uint4(0, 0, 0, 0);
+          if (b >= 0 && t < room)
+            w[i] = __ldg(reinterpret_cast<const uint4*>(src + (uint64_t)(uint32_t)b * block_bytes + head_off +
+                                                        (t & ((1 << lg) - 1)) * HD));
         }
+      };
+      auto widen = [&](uint32_t dst, const uint4 (&w)[PC]) {
 #pragma unroll
-        for (int i = 0; i < HD / 64; ++i) {
-          const int row = tok0 + 32 * i + 64 * h;
-          const uint32_t c4[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+        for (int i = 0; i < PC; ++i) {
+          const int row = tok0 + i * TSTEP;
+          const int c = 2 * (ch & 3);
+          const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
           uint32_t o[8];
 #pragma unroll
-          for (int y = 0; y < 4; ++y) codes4_to_f16<TYPE>(c4[y], o[2 * y], o[2 * y + 1]);
-          const uint32_t p = dst + (uint32_t)atom * 16384u;
-          sts16(p + sw128_off(row, 2 * ch), o[0], o[1], o[2], o[3]);
-          sts16(p + sw128_off(row, 2 * ch + 1), o[4], o[5], o[6], o[7]);
+          for (int y = 0; y < 4; ++y) codes4_to_f16<TYPE>(u[y], o[2 * y], o[2 * y + 1]);
+          const uint32_t p = dst + (uint32_t)(ch >> 2) * 16384u;
+          sts16(p + sw128_off(row, c), o[0], o[1], o[2], o[3]);
+          sts16(p + sw128_off(row, c + 1), o[4], o[5], o[6], o[7]);
         }
-        warp_arrive(U_EMPTY + u);
-        if (++u == Cfg::kUnits) { u = 0; u_par ^= 1u; }
       };
+      // codes and exponents are loaded one tile ahead, block ids two
+      uint4 wk[PC], wv[PC];
+      int id = load_id(s.tile);
+      load_codes(a.k, s.tile, id, wk);
+      load_codes(a.v, s.tile, id, wv);
+      uint32_t exps = load_exp(id);
+      id = load_id(s.tile + 1);
       // q: 16 (8 for 64 dims) lanes a row
       if (n_seg > 0) ok = pre_wait(bar(Q_EMPTY), (n_seg - 1) & 1);
       if (!ok) break;
@@ -302,18 +319,24 @@ k_kv_prefill(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
       for (int x = s.tile; x < s.tile_end && ok; ++x, ++n_tile) {
         const int st = n_tile & 1;
         const uint32_t par = (uint32_t)(n_tile >> 1) & 1u;
-        const int room = s.len - x * kPreTok;
-#pragma unroll 1
-        for (int kv = 0; kv < 2 && ok; ++kv) {
-          if (n_tile >= 2) ok = pre_wait(bar((kv ? V_EMPTY : K_EMPTY) + st), par ^ 1u);
-          if (!ok) break;
-          const uint32_t dst = kv ? v_addr(st) : k_addr(st);
-          widen(dst, 0, room);
-          if (ok) widen(dst, 1, room - 64);
-          if (!ok) break;
-          fence_proxy_async();
-          warp_arrive((kv ? V_FULL : K_FULL) + st);
+        if (n_tile >= 2) ok = pre_wait(bar(K_EMPTY + st), par ^ 1u);
+        if (!ok) break;
+        widen(k_addr(st), wk);
+        if (lt < 8) {
+          const int ev = (int)(exps >> 8) - 127;
+          s_meta[n_tile & 3][lt] = PreMeta{u2f((exps & 0xFFu) << 23), (float)ev, pow2f(-ev), 0.0f};
         }
+        fence_proxy_async();
+        warp_arrive(K_FULL + st);
+        load_codes(a.k, x + 1, id, wk);
+        exps = load_exp(id);
+        if (n_tile >= 2) ok = pre_wait(bar(V_EMPTY + st), par ^ 1u);
+        if (!ok) break;
+        widen(v_addr(st), wv);
+        fence_proxy_async();
+        warp_arrive(V_FULL + st);
+        load_codes(a.v, x + 1, id, wv);
+        id = load_id(x + 2);
       }
       ++n_seg;
     }
@@ -324,7 +347,7 @@ k_kv_prefill(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
       warp_arrive(Q_FULL);
     }
   } else if (warp >= kPreMma) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp < kPreMma + 2) {
       constexpr uint32_t id_qk = idesc_f16(128, 64), id_pv = idesc_f16(128, HD) | (1u << 16);
       const uint32_t one = lane == 0, tm = __reduce_or_sync(0xFFFFFFFFu, tmem);  // uniform
@@ -387,62 +410,8 @@ k_kv_prefill(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         }
       }
     }
-    if (warp == kPreMma + 2) {
-      // ---- codes by TMA: each tile's K, then its V, 64 tokens a unit ---------------
-      int n_tile = 0, r = kv_find(s_batch, a.requests, v0), u = 0, n_unit = 0;
-      uint32_t u_par = 1;  // the first round finds the ring empty
-      const int lg = a.block_log2;
-      for (int v = v0; v < v1 && ok;) {
-        KvSeg s;
-        kv_seg<RG, TL>(a, s_batch, r, v, v1, s);
-        v = min(s.pair_end, v1);
-        const int32_t* row_table = a.table + (size_t)s.r * a.width;
-        // lane i < 8: block of the i-th 16 tokens of tile x; -1 past the end or
-        // outside the pool
-        auto load_id = [&](int x) {
-          const long long t = (long long)x * kPreTok + lane * 16;
-          int id = -1;
-          if (lane < 8 && x < s.tile_end && t < s.len) id = row_table[t >> lg];
-          return id < a.blocks ? id : -1;
-        };
-        // and its exponents, K's | V's << 8
-        auto load_exp = [&](int id) -> uint32_t {
-          if (id < 0) return 127u | (127u << 8);
-          const int cell = id * a.heads + s.h;
-          return (uint32_t)__ldg(a.ks + cell) | ((uint32_t)__ldg(a.vs + cell) << 8);
-        };
-        int next = load_id(s.tile);
-        uint32_t next_exps = load_exp(next);
-#pragma unroll 1
-        for (int x = s.tile; x < s.tile_end && ok; ++x, ++n_tile) {
-          const int id = next, cell = id * a.heads + s.h;
-          const uint32_t exps = next_exps;
-          next = load_id(x + 1);
-          // outside the pool: rows in front of it, which TMA fills with zeros
-          const int y = id < 0 ? -16 : (cell << lg) + ((x * kPreTok + lane * 16) & ((1 << lg) - 1));
-#pragma unroll 1
-          for (int q = 0; q < 4 && ok; ++q, ++n_unit) {
-            ok = __all_sync(0xFFFFFFFFu, n_unit < Cfg::kUnits || pre_wait(bar(U_EMPTY + u), u_par));
-            if (!ok) break;
-            if (q == 0 && lane < 8) {  // the tile's factors, ordered before the unit
-              const int ev = (int)(exps >> 8) - 127;
-              s_meta[n_tile & 3][lane] = PreMeta{u2f((exps & 0xFFu) << 23), (float)ev, pow2f(-ev), 0.0f};
-            }
-            __syncwarp();
-            const int row = __shfl_sync(0xFFFFFFFFu, y, (q & 1) * 4 + (lane & 3));
-            if (lane == 0) mbar_expect_tx(bar(U_FULL + u), Cfg::kUnit);
-            __syncwarp();
-            if (lane < HD / 16)
-              tma_load_2d(raw_addr(u) + (uint32_t)((lane >> 2) * 4096 + (lane & 3) * 1024), q < 2 ? &map_k : &map_v,
-                          (lane >> 2) * 64, row, bar(U_FULL + u));
-            if (++u == Cfg::kUnits) { u = 0; u_par ^= 1u; }
-          }
-          next_exps = load_exp(next);
-        }
-      }
-    }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
     // ---- softmax: one row per thread -----------------------------------------------
     const int x = warp >> 2;  // row tile
     const uint32_t quad = (uint32_t)(32 * (warp & 3)) << 16;
@@ -492,7 +461,7 @@ k_kv_prefill(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
               tmem_ld_wait(w[1]);
             }
             // exponents relative to m, and their maximum
-            float mx = -INFINITY;
+            float mxa[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
               const float f = fq * meta[g].ks, b = meta[g].ev - m;
@@ -504,9 +473,10 @@ k_kv_prefill(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                   if (t0 + t < lo || t0 + t >= hi) p[t] = -INFINITY;
                   if (t0 + t + 1 < lo || t0 + t + 1 >= hi) p[t + 1] = -INFINITY;
                 }
-                mx = max3(mx, p[t], p[t + 1]);
+                mxa[g] = fmaxf(mxa[g], fmaxf(p[t], p[t + 1]));
               }
             }
+            const float mx = fmaxf(fmaxf(mxa[0], mxa[1]), fmaxf(mxa[2], mxa[3]));
             // m moves, by a whole number, when a weight would pass 2^15, and at a
             // row's first visible token (fresh: nothing is summed yet)
             const bool move = mx > kKvGrow || (fresh && mx > -INFINITY);
@@ -630,6 +600,7 @@ __global__ void __launch_bounds__(256) k_kv_prefill_join(const KvAttnArgs a, int
   __shared__ KvBatch<kKvPrefillRequests> s_batch;
   __shared__ int s_scan[16];
   const int tid = threadIdx.x;
+  pdl_begin();
   int longest;
   const int V = kv_line<RG, TL, 8>(a, s_batch, s_scan, longest);
   const int E = max(1, min(grid, V)), c_first = blockIdx.x;
@@ -686,8 +657,7 @@ __global__ void __launch_bounds__(256) k_kv_prefill_join(const KvAttnArgs a, int
 }
 
 template <int TYPE, int HD>
-static cudaError_t launch_prefill(const CUtensorMap& mk, const CUtensorMap& mv, const KvAttnArgs& a, int grid,
-                                  cudaStream_t s) {
+static cudaError_t launch_prefill(const KvAttnArgs& a, int grid, cudaStream_t s) {
   constexpr int BYTES = PreCfg<HD>::kSmem;
   static bool attr[64] = {false};
   int dev = 0;
@@ -698,24 +668,21 @@ static cudaError_t launch_prefill(const CUtensorMap& mk, const CUtensorMap& mv, 
     if (e != cudaSuccess) return e;
     if (dev < 64) attr[dev] = true;
   }
-  k_kv_prefill<TYPE, HD><<<grid, kPreWarps * 32, BYTES, s>>>(mk, mv, a);
-  e = cudaGetLastError();
+  e = pdl_launch(k_kv_prefill<TYPE, HD>, dim3((unsigned)grid), dim3(kPreWarps * 32), BYTES, s, a);
   if (e != cudaSuccess) return e;
-  k_kv_prefill_join<HD><<<dim3((unsigned)grid, kPreRows / 32), 256, 0, s>>>(a, grid);
-  return cudaGetLastError();
+  return pdl_launch(k_kv_prefill_join<HD>, dim3((unsigned)grid, kPreRows / 32), dim3(256), 0, s, a, grid);
 }
 
 size_t kv_prefill_workspace(int head_dim, int sm_count) {
   return (size_t)sm_count * 2 * kPreRows * (head_dim + 2) * sizeof(float);
 }
 
-cudaError_t kv_prefill_launch(int type, int head_dim, const CUtensorMap& mk, const CUtensorMap& mv, const KvAttnArgs& a,
-                              int grid, cudaStream_t s) {
+cudaError_t kv_prefill_launch(int type, int head_dim, const KvAttnArgs& a, int grid, cudaStream_t s) {
   if (type == QGEMM_KV_E4M3)
-    return head_dim == 64 ? launch_prefill<QGEMM_KV_E4M3, 64>(mk, mv, a, grid, s)
-                          : launch_prefill<QGEMM_KV_E4M3, 128>(mk, mv, a, grid, s);
-  return head_dim == 64 ? launch_prefill<QGEMM_KV_INT8, 64>(mk, mv, a, grid, s)
-                        : launch_prefill<QGEMM_KV_INT8, 128>(mk, mv, a, grid, s);
+    return head_dim == 64 ? launch_prefill<QGEMM_KV_E4M3, 64>(a, grid, s)
+                          : launch_prefill<QGEMM_KV_E4M3, 128>(a, grid, s);
+  return head_dim == 64 ? launch_prefill<QGEMM_KV_INT8, 64>(a, grid, s)
+                        : launch_prefill<QGEMM_KV_INT8, 128>(a, grid, s);
 }
 
 unsigned kv_prefill_fault() {

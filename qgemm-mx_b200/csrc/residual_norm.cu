@@ -115,6 +115,7 @@ __global__ void __launch_bounds__(512) k_residual_norm(const NormArgs a) {
   const bool live = row_raw < a.tokens;
   const int64_t row = live ? row_raw : a.tokens - 1;  // spare rows recompute the last one and store nothing
   const float inv_width = 1.0f / (float)a.width;
+  pdl_begin();
   float r[V][8], x[V][8];
   uint4 g[V];
 #pragma unroll
@@ -172,9 +173,9 @@ __global__ void __launch_bounds__(512) k_residual_norm(const NormArgs a) {
 }
 
 template <int V, bool LAYER>
-static void launch_norm(const NormArgs& a, bool f32, unsigned grid, unsigned threads, cudaStream_t s) {
-  if (f32) k_residual_norm<V, LAYER, true><<<grid, threads, 0, s>>>(a);
-  else k_residual_norm<V, LAYER, false><<<grid, threads, 0, s>>>(a);
+static cudaError_t launch_norm(const NormArgs& a, bool f32, unsigned grid, unsigned threads, cudaStream_t s) {
+  return pdl_launch(f32 ? k_residual_norm<V, LAYER, true> : k_residual_norm<V, LAYER, false>, dim3(grid), dim3(threads), 0,
+                    s, a);
 }
 
 }  // namespace qg
@@ -220,14 +221,15 @@ qgemm_status_t qgemm_residual_norm(const qgemm_residual_norm_t* p, void* stream)
   const unsigned grid = ((unsigned)p->tokens + rows - 1) / rows;
   cudaStream_t s = as_stream(stream);
   const bool layer = p->kind == QGEMM_NORM_LAYER, f32 = p->residual_f32 != 0;
+  cudaError_t e = cudaSuccess;
 #define QG_NORM(V_)                                                       \
   case V_:                                                                \
-    if (layer) launch_norm<V_, true>(a, f32, grid, rows * row_threads, s); \
-    else launch_norm<V_, false>(a, f32, grid, rows * row_threads, s);      \
+    e = layer ? launch_norm<V_, true>(a, f32, grid, rows * row_threads, s)  \
+              : launch_norm<V_, false>(a, f32, grid, rows * row_threads, s); \
     break;
   switch (V) { QG_NORM(1) QG_NORM(2) QG_NORM(4) }
 #undef QG_NORM
-  QG_LAUNCH_RET();
+  QG_CUDA_RET(e);
   return QGEMM_OK;
 }
 

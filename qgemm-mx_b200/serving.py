@@ -42,9 +42,20 @@ _sig("qgemm_kv_attention", _i32, [C.POINTER(_KVCache), _vp, _i64, _i64, _i32, _i
 _sig("qgemm_residual_norm", _i32, [C.POINTER(_ResidualNorm), _vp])
 
 
-def _want(ok: bool, where: str, what: str) -> None:
-    if not ok:
-        raise ValueError(f"{where}: {what}")
+# The stream pointer of torch's current stream on a device: the calls below are
+# short beside torch.cuda.current_stream().
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_i32t, _i64t, _u8t, _bf16, _f32t = torch.int32, torch.int64, torch.uint8, torch.bfloat16, torch.float32
+_empty = torch.empty
+
+
+def _on(t: torch.Tensor, stream) -> int:
+    return _raw_stream(t.get_device()) if stream is None else stream.cuda_stream
+
+
+def _bad(where: str, what: str):
+    raise ValueError(f"{where}: {what}")
 
 
 @dataclass
@@ -59,15 +70,17 @@ class KVCache:
     v_scales: torch.Tensor
 
     def __post_init__(self):
-        shape = self.k.shape
-        for t in (self.k, self.v):
-            _want(t.dim() == 4 and t.dtype == torch.uint8 and t.is_contiguous() and t.shape == shape, "KVCache",
-                  "k and v must be contiguous uint8 tensors of one shape [blocks, heads, block, head_dim]")
-        for t in (self.k_scales, self.v_scales):
-            _want(t.dtype == torch.uint8 and t.is_contiguous() and t.shape == shape[:2], "KVCache",
-                  "k_scales and v_scales must be contiguous uint8 [blocks, heads]")
-        self._desc = _KVCache(self.type, shape[2], shape[1], shape[3], shape[0], self.k.data_ptr(),
-                              self.v.data_ptr(), self.k_scales.data_ptr(), self.v_scales.data_ptr())
+        k, v, ks, vs = self.k, self.v, self.k_scales, self.v_scales
+        shape = k.shape
+        if not (len(shape) == 4 and v.shape == shape and k.dtype is _u8t and v.dtype is _u8t and k.is_contiguous() and
+                v.is_contiguous()):
+            _bad("KVCache", "k and v must be contiguous uint8 tensors of one shape [blocks, heads, block, head_dim]")
+        if not (ks.shape == shape[:2] and vs.shape == shape[:2] and ks.dtype is _u8t and vs.dtype is _u8t and
+                ks.is_contiguous() and vs.is_contiguous()):
+            _bad("KVCache", "k_scales and v_scales must be contiguous uint8 [blocks, heads]")
+        self._desc = _KVCache(self.type, shape[2], shape[1], shape[3], shape[0], k.data_ptr(), v.data_ptr(),
+                              ks.data_ptr(), vs.data_ptr())
+        self._ref = C.byref(self._desc)
 
     def values(self) -> tuple[torch.Tensor, torch.Tensor]:
         """(K, V) as float32 [blocks, heads, block, head_dim], for inspection."""
@@ -96,9 +109,8 @@ class KVPlan:
     counts: torch.Tensor     # int32 [4]: free blocks left, runs, rows, refused requests
 
 
-def _ints(t: torch.Tensor, where: str, what: str, dims: int = 1) -> None:
-    _want(t.dtype == torch.int32 and t.dim() == dims and t.is_contiguous() and t.is_cuda, where,
-          f"{what} must be a contiguous int32 CUDA tensor with {dims} dimension(s)")
+def _ints(t: torch.Tensor, dims: int = 1) -> bool:
+    return t.dtype is _i32t and t.dim() == dims and t.is_cuda and t.is_contiguous()
 
 
 def kv_plan(lens: torch.Tensor, new: torch.Tensor, table: torch.Tensor, free_list: torch.Tensor,
@@ -106,43 +118,42 @@ def kv_plan(lens: torch.Tensor, new: torch.Tensor, table: torch.Tensor, free_lis
     """Blocks, slots and positions of the `new` tokens of requests that hold
     `lens`; new block ids go into `table` [requests, width].  `tokens` is the
     step's row count (rows no request covers get slot -1).  Nothing is read
-    back: plan.counts[3] tells on the device how many requests were refused."""
-    requests = lens.numel()
-    _ints(lens, "kv_plan", "lens")
-    _ints(new, "kv_plan", "new")
-    _ints(table, "kv_plan", "table", 2)
-    _ints(free_list, "kv_plan", "free_list")
-    _ints(free_count, "kv_plan", "free_count")
-    _want(new.numel() == requests and table.shape[0] == requests and free_count.numel() == 1, "kv_plan",
-          "new, table and free_count must have one entry per request, row per request, and one element")
+    back: plan.counts[3] tells on the device how many requests were refused.
+    With `out` (an earlier plan of the same sizes) nothing is allocated."""
+    if not (_ints(lens) and _ints(new) and _ints(table, 2) and _ints(free_list) and _ints(free_count)):
+        _bad("kv_plan", "lens, new, table [requests, width], free_list and free_count must be contiguous int32 CUDA tensors")
+    requests, width = table.shape
+    if not (lens.numel() == requests and new.numel() == requests and free_count.numel() == 1):
+        _bad("kv_plan", "new, table and free_count must have one entry per request, row per request, and one element")
     most = _lib.qgemm_kv_max_runs(requests, tokens, block)
-    _want(most >= 0, "kv_plan", "block must be 16, 32, 64 or 128 and tokens not negative")
+    if most < 0:
+        _bad("kv_plan", "block must be 16, 32, 64 or 128 and tokens not negative")
     if out is None:
-        # one allocation for the int32 outputs
-        sizes = (requests + 1, requests, tokens, most + 1, 4)
-        starts, lens_out, positions, runs, counts = torch.empty(
-            sum(sizes), dtype=torch.int32, device=lens.device).split(sizes)
-        out = KVPlan(starts, lens_out, torch.empty(tokens, dtype=torch.int64, device=lens.device), positions, runs,
-                     counts)
-    else:
-        _want(out.starts.numel() == requests + 1 and out.lens.numel() == requests and out.slots.numel() == tokens and
-              out.positions.numel() == tokens and out.runs.numel() == most + 1 and out.counts.numel() == 4, "kv_plan",
-              "out was made for other sizes")
-    _check(_lib.qgemm_kv_plan(block, requests, lens.data_ptr(), new.data_ptr(), table.data_ptr(), table.shape[1],
-                              free_list.data_ptr(), free_count.data_ptr(), tokens, out.lens.data_ptr(),
-                              out.starts.data_ptr(), out.slots.data_ptr(), out.positions.data_ptr(),
-                              out.runs.data_ptr(), out.counts.data_ptr(), _stream(stream)), "kv_plan")
+        dev = lens.device
+        out = KVPlan(_empty(requests + 1, dtype=_i32t, device=dev), _empty(requests, dtype=_i32t, device=dev),
+                     _empty(tokens, dtype=_i64t, device=dev), _empty(tokens, dtype=_i32t, device=dev),
+                     _empty(most + 1, dtype=_i32t, device=dev), _empty(4, dtype=_i32t, device=dev))
+    elif not (out.starts.numel() == requests + 1 and out.lens.numel() == requests and out.slots.numel() == tokens and
+              out.positions.numel() == tokens and out.runs.numel() == most + 1 and out.counts.numel() == 4):
+        _bad("kv_plan", "out was made for other sizes")
+    st = _lib.qgemm_kv_plan(block, requests, lens.data_ptr(), new.data_ptr(), table.data_ptr(), width,
+                            free_list.data_ptr(), free_count.data_ptr(), tokens, out.lens.data_ptr(),
+                            out.starts.data_ptr(), out.slots.data_ptr(), out.positions.data_ptr(), out.runs.data_ptr(),
+                            out.counts.data_ptr(), _on(lens, stream))
+    if st:
+        _check(st, "kv_plan")
     return out
 
 
-def _rows(t: torch.Tensor, heads: int | None, head_dim: int, where: str, what: str) -> tuple[int, int]:
+def _rows(t: torch.Tensor, head_dim: int, where: str, what: str) -> tuple[int, int, int]:
     """Checks bf16 [tokens, heads, head_dim] rows (any spacing of tokens and
-    heads); returns the elements between tokens and between heads."""
-    _want(t.dtype == torch.bfloat16 and t.dim() == 3 and t.is_cuda and t.shape[2] == head_dim and
-          (heads is None or t.shape[1] == heads), where, f"{what} must be bf16 [tokens, heads, {head_dim}] on the GPU")
+    heads); returns the heads, and the elements between tokens and heads."""
+    if t.dtype is not _bf16 or t.dim() != 3 or not t.is_cuda or t.shape[2] != head_dim:
+        _bad(where, f"{what} must be bf16 [tokens, heads, {head_dim}] on the GPU")
     a, b, c = t.stride()
-    _want(c == 1 or t.numel() == 0, where, f"the head_dim values of {what} must lie together")
-    return a, b
+    if c != 1 and t.numel():
+        _bad(where, f"the head_dim values of {what} must lie together")
+    return t.shape[1], a, b
 
 
 def kv_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, runs: torch.Tensor,
@@ -150,19 +161,22 @@ def kv_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Ten
     """Quantises the rows k, v (bf16 [tokens, heads, head_dim], rows may be
     slices of a QKV product) into the slots that kv_plan gave them."""
     d = cache._desc
-    ks = _rows(k, d.heads, d.head_dim, "kv_append", "k")
-    vs = _rows(v, d.heads, d.head_dim, "kv_append", "v")
+    kh, ka, kb = _rows(k, d.head_dim, "kv_append", "k")
+    vh, va, vb = _rows(v, d.head_dim, "kv_append", "v")
     tokens = k.shape[0]
-    _want(v.shape[0] == tokens and slots.dtype == torch.int64 and slots.numel() == tokens and slots.is_contiguous(),
-          "kv_append", "k, v and int64 slots must have one row per token")
-    _ints(runs, "kv_append", "runs")
-    _want(runs.numel() >= 1, "kv_append", "runs must hold an end mark")
-    _check(_lib.qgemm_kv_append(C.byref(d), k.data_ptr(), v.data_ptr(), *ks, *vs, tokens, slots.data_ptr(),
-                                runs.data_ptr(), runs.numel() - 1, _stream(stream)), "kv_append")
+    if not (kh == d.heads and vh == kh and v.shape[0] == tokens and slots.dtype is _i64t and slots.numel() == tokens and
+            slots.is_contiguous()):
+        _bad("kv_append", "k, v (the cache's heads) and int64 slots must have one row per token")
+    if not _ints(runs) or runs.numel() < 1:
+        _bad("kv_append", "runs must be a contiguous int32 CUDA tensor with an end mark")
+    st = _lib.qgemm_kv_append(cache._ref, k.data_ptr(), v.data_ptr(), ka, kb, va, vb, tokens, slots.data_ptr(),
+                              runs.data_ptr(), runs.numel() - 1, _on(k, stream))
+    if st:
+        _check(st, "kv_append")
 
 
 def kv_attention_workspace(cache: KVCache, q_heads: int, requests: int, tokens: int, max_new: int) -> int:
-    return _lib.qgemm_kv_attention_workspace(C.byref(cache._desc), q_heads, requests, tokens, max_new)
+    return _lib.qgemm_kv_attention_workspace(cache._ref, q_heads, requests, tokens, max_new)
 
 
 def make_kv_workspace(cache: KVCache, q_heads: int, requests: int, tokens: int, max_new: int,
@@ -182,27 +196,26 @@ def kv_attention(cache: KVCache, q: torch.Tensor, starts: torch.Tensor, lens: to
     of its lens[r] tokens.  scale defaults to head_dim ** -0.5; window > 0
     bounds how far back a row sees.  Returns out (bf16, as q), or (out, lse)."""
     d = cache._desc
-    strides = _rows(q, None, d.head_dim, "kv_attention", "q")
-    tokens, q_heads = q.shape[0], q.shape[1]
-    _ints(starts, "kv_attention", "starts")
-    _ints(lens, "kv_attention", "lens")
-    _ints(table, "kv_attention", "table", 2)
-    requests = lens.numel()
-    _want(starts.numel() == requests + 1 and table.shape[0] == requests, "kv_attention",
-          "starts needs requests + 1 entries and table a row per request")
+    head_dim = d.head_dim
+    q_heads, qa, qb = _rows(q, head_dim, "kv_attention", "q")
+    tokens, requests = q.shape[0], lens.numel()
+    if not (_ints(starts) and _ints(lens) and _ints(table, 2)):
+        _bad("kv_attention", "starts, lens and table [requests, width] must be contiguous int32 CUDA tensors")
+    if not (starts.numel() == requests + 1 and table.shape[0] == requests):
+        _bad("kv_attention", "starts needs requests + 1 entries and table a row per request")
     if out is None:
-        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-    else:
-        _want(out.shape == q.shape and out.dtype == torch.bfloat16 and out.is_contiguous(), "kv_attention",
-              "out must be contiguous bf16 of q's shape")
-    z = torch.empty((tokens, q_heads), dtype=torch.float32, device=q.device) if lse else None
+        out = _empty(q.shape, dtype=_bf16, device=q.device)
+    elif not (out.shape == q.shape and out.dtype is _bf16 and out.is_contiguous()):
+        _bad("kv_attention", "out must be contiguous bf16 of q's shape")
+    z = _empty((tokens, q_heads), dtype=_f32t, device=q.device) if lse else None
     if workspace is None:
         workspace = make_kv_workspace(cache, q_heads, requests, tokens, max_new, stream)
-    _check(_lib.qgemm_kv_attention(C.byref(d), q.data_ptr(), *strides, q_heads, requests, starts.data_ptr(),
-                                   lens.data_ptr(), table.data_ptr(), table.shape[1], tokens, max_new,
-                                   d.head_dim ** -0.5 if scale is None else scale, window, causal, out.data_ptr(),
-                                   0 if z is None else z.data_ptr(), workspace.data_ptr(), workspace.numel(),
-                                   _stream(stream)), "kv_attention")
+    st = _lib.qgemm_kv_attention(cache._ref, q.data_ptr(), qa, qb, q_heads, requests, starts.data_ptr(),
+                                 lens.data_ptr(), table.data_ptr(), table.shape[1], tokens, max_new,
+                                 head_dim ** -0.5 if scale is None else scale, window, causal, out.data_ptr(),
+                                 z.data_ptr() if lse else 0, workspace.data_ptr(), workspace.numel(), _on(q, stream))
+    if st:
+        _check(st, "kv_attention")
     return (out, z) if lse else out
 
 
@@ -217,34 +230,41 @@ def residual_norm(y: torch.Tensor | None, residual: torch.Tensor, post: torch.Te
     post, gate or bias drops its factor; without pre, h is None; without y
     (the first block) residual is only normed.  residual_out may be residual
     and h may be y."""
-    where = "residual_norm"
-    _want(kind in NORM_KINDS, where, "kind must be 'rms' or 'layer'")
-    _want(residual.dim() == 2 and residual.dtype in (torch.bfloat16, torch.float32) and residual.is_contiguous() and
-          residual.is_cuda, where, "residual must be contiguous bf16 or float32 [tokens, width] on the GPU")
-    tokens, width = residual.shape
-    stream_like = residual.dtype
-    for t, what in ((y, "y"), (h, "h")):
-        _want(t is None or (t.shape == residual.shape and t.dtype == torch.bfloat16 and t.is_contiguous()), where,
-              f"{what} must be contiguous bf16 [tokens, width]")
-    for t, what in ((post, "post"), (pre, "pre"), (post_bias, "post_bias"), (pre_bias, "pre_bias")):
-        _want(t is None or (t.shape == (width,) and t.dtype == torch.bfloat16 and t.is_contiguous()), where,
-              f"{what} must be contiguous bf16 [width]")
+    if not (residual.dim() == 2 and residual.dtype in (_bf16, _f32t) and residual.is_cuda and residual.is_contiguous()):
+        _bad("residual_norm", "residual must be contiguous bf16 or float32 [tokens, width] on the GPU")
+    shape = residual.shape
+    tokens, width = shape
+    for t in (y, h):
+        if t is not None and not (t.dtype is _bf16 and t.shape == shape and t.is_contiguous()):
+            _bad("residual_norm", "y and h must be contiguous bf16 [tokens, width]")
+    for t in (post, pre, post_bias, pre_bias):
+        if t is not None and not (t.dtype is _bf16 and t.dim() == 1 and t.numel() == width and t.is_contiguous()):
+            _bad("residual_norm", "post, pre and their biases must be contiguous bf16 [width]")
     gate_stride = 0
     if gate is not None:
-        _want(gate.dtype == torch.bfloat16 and gate.is_cuda and gate.shape in ((width,), (tokens, width)) and
-              (gate.stride(-1) == 1 or width == 1), where, "gate must be bf16 [width] or [tokens, width]")
+        if not (gate.dtype is _bf16 and gate.is_cuda and gate.shape in ((width,), shape) and
+                (gate.stride(-1) == 1 or width == 1)):
+            _bad("residual_norm", "gate must be bf16 [width] or [tokens, width]")
         gate_stride = gate.stride(0) if gate.dim() == 2 else 0
-    if y is not None and residual_out is None:
-        residual_out = torch.empty_like(residual)
-    elif y is None:
+    code = NORM_KINDS.get(kind)
+    if code is None:
+        _bad("residual_norm", "kind must be 'rms' or 'layer'")
+    if y is None:
         residual_out = residual
-    _want(residual_out.shape == residual.shape and residual_out.dtype == stream_like and
-          residual_out.is_contiguous(), where, "residual_out must be like residual")
-    if pre is not None and h is None:
-        h = torch.empty(residual.shape, dtype=torch.bfloat16, device=residual.device)
-    a = _ResidualNorm(NORM_KINDS[kind], tokens, width, stream_like == torch.float32,
-                      *(0 if t is None else t.data_ptr() for t in (y, residual, post, post_bias, gate)), gate_stride,
-                      *(0 if t is None else t.data_ptr() for t in (pre, pre_bias)), alpha, eps,
-                      residual_out.data_ptr(), 0 if pre is None else h.data_ptr())
-    _check(_lib.qgemm_residual_norm(C.byref(a), _stream(stream)), where)
-    return residual_out, h if pre is not None else None
+    elif residual_out is None:
+        residual_out = _empty(shape, dtype=residual.dtype, device=residual.device)
+    elif not (residual_out.shape == shape and residual_out.dtype is residual.dtype and residual_out.is_contiguous()):
+        _bad("residual_norm", "residual_out must be like residual")
+    if pre is None:
+        h = None
+    elif h is None:
+        h = _empty(shape, dtype=_bf16, device=residual.device)
+    a = _ResidualNorm(code, tokens, width, residual.dtype is _f32t, 0 if y is None else y.data_ptr(),
+                      residual.data_ptr(), 0 if post is None else post.data_ptr(),
+                      0 if post_bias is None else post_bias.data_ptr(), 0 if gate is None else gate.data_ptr(),
+                      gate_stride, 0 if pre is None else pre.data_ptr(), 0 if pre_bias is None else pre_bias.data_ptr(),
+                      alpha, eps, residual_out.data_ptr(), 0 if h is None else h.data_ptr())
+    st = _lib.qgemm_residual_norm(C.byref(a), _on(residual, stream))
+    if st:
+        _check(st, "residual_norm")
+    return residual_out, h
