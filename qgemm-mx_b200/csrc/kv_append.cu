@@ -18,8 +18,6 @@
 namespace qg {
 
 constexpr int kAppendThreads = 256;
-constexpr int kAppendHeld = 8;  // 16-byte vectors a thread keeps in registers
-
 struct AppendArgs {
   uint8_t *k, *v, *ks, *vs;
   const uint16_t *xk, *xv;
@@ -31,21 +29,41 @@ struct AppendArgs {
   unsigned items;
 };
 
-// Largest finite |x| of two bf16 values, as bf16 bits.
+// |x| of bf16 pairs as bits: the larger of each half.
 __device__ __forceinline__ uint32_t amax2(uint32_t w, uint32_t m) {
+  uint32_t d;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(w & 0x7FFF7FFFu), "r"(m));
+  return d;
+}
+// Largest finite |x| of two bf16 values, where infinities or NaN occur.
+__device__ __forceinline__ uint32_t amax_finite(uint32_t w, uint32_t m) {
   const uint32_t lo = w & 0x7FFFu, hi = (w >> 16) & 0x7FFFu;
   if (lo < 0x7F80u) m = max(m, lo);
   if (hi < 0x7F80u) m = max(m, hi);
   return m;
 }
-template <int TYPE>
+// Four bf16 values times f to codes.  FINITE: none is infinite or NaN, and the scale
+// keeps them in range, so only rounding is left.
+template <int TYPE, bool FINITE>
 __device__ __forceinline__ uint32_t encode4(uint32_t w0, uint32_t w1, float f) {
   const float x0 = u2f(w0 << 16) * f, x1 = u2f(w0 & 0xFFFF0000u) * f;
   const float x2 = u2f(w1 << 16) * f, x3 = u2f(w1 & 0xFFFF0000u) * f;
-  return kv_encode<TYPE>(x0) | (kv_encode<TYPE>(x1) << 8) | (kv_encode<TYPE>(x2) << 16) | (kv_encode<TYPE>(x3) << 24);
+  if (!FINITE)
+    return kv_encode<TYPE>(x0) | (kv_encode<TYPE>(x1) << 8) | (kv_encode<TYPE>(x2) << 16) | (kv_encode<TYPE>(x3) << 24);
+  if (TYPE == QGEMM_KV_E4M3) {
+    uint16_t lo, hi;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(x1), "f"(x0));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(x3), "f"(x2));
+    return (uint32_t)lo | ((uint32_t)hi << 16);
+  }
+  uint32_t d;  // bytes 0, 1 of the second packing, then 2, 3
+  asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(__float2int_rn(x3)), "r"(__float2int_rn(x2)), "r"(0));
+  asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(__float2int_rn(x1)), "r"(__float2int_rn(x0)), "r"(d));
+  return d;
 }
 
-template <int TYPE, int HD, int GT>
+// HELD: 16-byte vectors a thread keeps in registers.
+template <int TYPE, int HD, int GT, int HELD>
 __global__ void __launch_bounds__(kAppendThreads) k_kv_append(const AppendArgs a) {
   constexpr int VPR = HD / 8;  // 16-byte vectors in a row
   __shared__ uint32_t s_max[kAppendThreads / 32];
@@ -72,26 +90,42 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append(const AppendArgs a
   uint8_t* scale = (which ? a.vs : a.ks) + cell;
   const int e_old = off > 0 ? (int)*scale - 127 : kKvLowestExp;
 
-  uint4 held[kAppendHeld];
-  uint32_t m = 0;
+  uint4 held[HELD];
+  uint32_t m2 = 0;
 #pragma unroll
-  for (int j = 0; j < kAppendHeld; ++j) {
+  for (int j = 0; j < HELD; ++j) {
     const int v = gl + j * GT;
     held[j] = v < nv ? __ldg(src(v)) : make_uint4(0, 0, 0, 0);
   }
 #pragma unroll
-  for (int j = 0; j < kAppendHeld; ++j)
-    m = amax2(held[j].x, amax2(held[j].y, amax2(held[j].z, amax2(held[j].w, m))));
-  for (int v = gl + kAppendHeld * GT; v < nv; v += GT) {  // only a warp's long runs; read again below
+  for (int j = 0; j < HELD; ++j)
+    m2 = amax2(held[j].x, amax2(held[j].y, amax2(held[j].z, amax2(held[j].w, m2))));
+#pragma unroll 1
+  for (int v = gl + HELD * GT; v < nv; v += GT) {  // only a warp's long runs; read again below
     const uint4 w = __ldg(src(v));
-    m = amax2(w.x, amax2(w.y, amax2(w.z, amax2(w.w, m))));
+    m2 = amax2(w.x, amax2(w.y, amax2(w.z, amax2(w.w, m2))));
   }
-  m = __reduce_max_sync(0xFFFFFFFFu, m);
-  if constexpr (GT > 32) {
-    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
-    __syncthreads();
+  auto group_max = [&](uint32_t m) {
+    m = __reduce_max_sync(0xFFFFFFFFu, m);
+    if constexpr (GT > 32) {
+      __syncthreads();
+      if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
+      __syncthreads();
 #pragma unroll
-    for (int w = 0; w < GT / 32; ++w) m = max(m, s_max[w]);
+      for (int w = 0; w < GT / 32; ++w) m = max(m, s_max[w]);
+    }
+    return m;
+  };
+  uint32_t m = group_max(max(m2 & 0xFFFFu, m2 >> 16));
+  const bool finite = m < 0x7F80u;  // of the whole group
+  if (!finite) {
+    m = 0;
+#pragma unroll 1
+    for (int v = gl; v < nv; v += GT) {
+      const uint4 w = __ldg(src(v));
+      m = amax_finite(w.x, amax_finite(w.y, amax_finite(w.z, amax_finite(w.w, m))));
+    }
+    m = group_max(m);
   }
   const int e = max(e_old, kv_exp_for<TYPE>(u2f(m << 16)));
   if (off > 0 && e > e_old) {  // the block's scale grows: rescale the codes it holds
@@ -107,24 +141,38 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append(const AppendArgs a
   }
   const float f = pow2f(-e);
   uint8_t* dst = codes + off * HD;
-  auto put = [&](int v, const uint4& w) {
-    *reinterpret_cast<uint2*>(dst + v * 8) = make_uint2(encode4<TYPE>(w.x, w.y, f), encode4<TYPE>(w.z, w.w, f));
-  };
+  if (finite) {
+    auto put = [&](int v, const uint4& w) {
+      *reinterpret_cast<uint2*>(dst + v * 8) =
+          make_uint2(encode4<TYPE, true>(w.x, w.y, f), encode4<TYPE, true>(w.z, w.w, f));
+    };
 #pragma unroll
-  for (int j = 0; j < kAppendHeld; ++j) {
-    const int v = gl + j * GT;
-    if (v < nv) put(v, held[j]);
+    for (int j = 0; j < HELD; ++j) {
+      const int v = gl + j * GT;
+      if (v < nv) put(v, held[j]);
+    }
+#pragma unroll 1
+    for (int v = gl + HELD * GT; v < nv; v += GT) put(v, __ldg(src(v)));
+  } else {
+#pragma unroll 1
+    for (int v = gl; v < nv; v += GT) {
+      const uint4 w = __ldg(src(v));
+      *reinterpret_cast<uint2*>(dst + v * 8) =
+          make_uint2(encode4<TYPE, false>(w.x, w.y, f), encode4<TYPE, false>(w.z, w.w, f));
+    }
   }
-  for (int v = gl + kAppendHeld * GT; v < nv; v += GT) put(v, __ldg(src(v)));
   if (gl == 0) *scale = (uint8_t)(e + 127);
 }
 
 template <int TYPE, int HD>
-static cudaError_t launch_append(const AppendArgs& a, bool wide, cudaStream_t s) {
+static cudaError_t launch_append(const AppendArgs& a, int vectors, cudaStream_t s) {
+  const bool wide = vectors > 8 * 32;
   const unsigned per = wide ? 1 : kAppendThreads / 32;
   const unsigned grid = (a.items + per - 1) / per;
-  return pdl_launch(wide ? k_kv_append<TYPE, HD, kAppendThreads> : k_kv_append<TYPE, HD, 32>, dim3(grid),
-                    dim3(kAppendThreads), 0, s, a);
+  auto kernel = !wide ? (vectors > 2 * 32 ? k_kv_append<TYPE, HD, 32, 8> : k_kv_append<TYPE, HD, 32, 2>)
+                      : (vectors > 4 * kAppendThreads ? k_kv_append<TYPE, HD, kAppendThreads, 8>
+                                                      : k_kv_append<TYPE, HD, kAppendThreads, 4>);
+  return pdl_launch(kernel, dim3(grid), dim3(kAppendThreads), 0, s, a);
 }
 
 }  // namespace qg
@@ -154,9 +202,10 @@ qgemm_status_t qgemm_kv_append(const qgemm_kv_cache_t* c, const uint16_t* k, con
   a.slots = slots; a.runs = runs; a.blocks = c->blocks; a.heads = c->heads; a.tokens = tokens;
   a.block_log2 = c->block == 16 ? 4 : c->block == 32 ? 5 : c->block == 64 ? 6 : 7;
   a.items = (unsigned)items;
-  // 256 threads an item when the usual run does not fit one warp's registers
+  // 16-byte vectors of the usual run: they choose the threads of an item and what
+  // each keeps in registers, so that a run is read once
   const int rows = (tokens + max_runs - 1) / max_runs;
-  const bool wide = (rows < c->block ? rows : c->block) * c->head_dim / 8 > 32 * kAppendHeld;
+  const int wide = (rows < c->block ? rows : c->block) * c->head_dim / 8;
   cudaStream_t s = as_stream(stream);
   const bool d64 = c->head_dim == 64;
   QG_CUDA_RET(c->type == QGEMM_KV_E4M3
