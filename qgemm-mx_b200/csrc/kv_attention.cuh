@@ -34,6 +34,7 @@ struct KvAttnArgs {
   int window, causal;
   uint16_t* out;
   float* lse;
+  int beside;  // the launch before is this call's other kernel, whose results are not needed
   unsigned* tickets;  // zero between calls
   float* partials;
 };

@@ -112,7 +112,7 @@ k_kv_decode(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  pdl_begin();
+  pdl_begin_after();
   int longest;
   const int V = kv_line<RG, 4, W>(a, s_batch, s_scan, longest);
   // Short pairs are not cut: a share takes the pairs that begin in it.  One pair
@@ -611,15 +611,16 @@ static qgemm_status_t kv_attention_run(const qgemm_kv_cache_t* c, KvAttnArgs a, 
   const int all = a.requests;
   const int32_t *starts = a.starts, *lens = a.lens, *table = a.table;
   // rows enough for max_new of every request: all bring as many, and one kernel
-  // takes whatever they bring
-  const bool even = (long long)a.requests * a.max_new <= a.tokens;
-  const int last = rows > kKvPrefillRows && even ? 1 : 0;
-  for (int kernel = rows > kKvPrefillRows ? 1 : 0; kernel >= last; --kernel) {
+  // takes whatever they bring.  Otherwise the decode kernel goes first and the
+  // prefill kernel's CTAs take the SMs as it leaves them.
+  const bool many = rows > kKvPrefillRows, even = (long long)a.requests * a.max_new <= a.tokens;
+  for (int kernel = many && even ? 1 : 0; kernel <= (many ? 1 : 0); ++kernel) {
     a.rows_min = kernel && !even ? kKvPrefillRows : 0;
     a.rows_max = kernel ? INT32_MAX : kKvPrefillRows;
     a.tickets = reinterpret_cast<unsigned*>(static_cast<char*>(ws) + 4096 * kernel);
     a.partials = reinterpret_cast<float*>(static_cast<char*>(ws) + (kernel ? w.prefill : w.decode));
-    const int nt = dec_nt(rows);
+    // beside prompt chunks the few rows are as a rule one token's
+    const int nt = dec_nt(many ? a.group : rows);
     // requests per launch: the prefix sums fit shared memory and the line 31 bits
     const long long per = kernel ? kv_line_most(a, 256, 7) : kv_line_most(a, 8 * nt, 4);
     if (per > INT32_MAX)
@@ -628,6 +629,7 @@ static qgemm_status_t kv_attention_run(const qgemm_kv_cache_t* c, KvAttnArgs a, 
     if (most > (kernel ? kKvPrefillRequests : kDecRequests)) most = kernel ? kKvPrefillRequests : kDecRequests;
     for (int r0 = 0; r0 < all; r0 += (int)most) {
       a.requests = all - r0 < most ? all - r0 : (int)most;
+      a.beside = kernel && !even && r0 == 0;
       a.starts = starts + r0;
       a.lens = lens + r0;
       a.table = table + (size_t)r0 * a.width;

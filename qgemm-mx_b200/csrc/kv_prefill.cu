@@ -163,12 +163,16 @@ k_kv_prefill(const KvAttnArgs a) {
   constexpr int K_FULL = 0, K_EMPTY = 2, V_FULL = 4, V_EMPTY = 6, Q_FULL = 8, Q_EMPTY = 9, S_FULL = 10, P_FULL = 14,
                 O_DONE = 18;
 
-  pdl_begin();
+  if (a.beside) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the wait is at the end
+  else pdl_begin_after();
   int longest;
   const int V = kv_line<RG, TL, 16>(a, s_batch, s_scan, longest);
   const int E = max(1, min((int)gridDim.x, V));
   const int cta = blockIdx.x;
-  if (V == 0 || cta >= E) return;
+  if (V == 0 || cta >= E) {
+    if (a.beside) pdl_wait();
+    return;
+  }
   const KvCuts cuts(V, E);
   const int v0 = cuts.at(cta), v1 = cuts.at(cta + 1);
 
@@ -584,6 +588,7 @@ k_kv_prefill(const KvAttnArgs a) {
     }
   }
   if (!ok && lane == 0) fault_drain();
+  if (a.beside) pdl_wait();
   tc_fence_before();
   __syncthreads();
   if (warp == kPreMma) {
@@ -600,17 +605,22 @@ __global__ void __launch_bounds__(256) k_kv_prefill_join(const KvAttnArgs a, int
   __shared__ KvBatch<kKvPrefillRequests> s_batch;
   __shared__ int s_scan[16];
   const int tid = threadIdx.x;
-  pdl_begin();
+  // the requests are known; only the partials come from the kernel before
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   int longest;
   const int V = kv_line<RG, TL, 8>(a, s_batch, s_scan, longest);
   const int E = max(1, min(grid, V)), c_first = blockIdx.x;
-  if (c_first + 1 >= E) return;
+  if (c_first + 1 >= E) {
+    pdl_wait();
+    return;
+  }
   const KvCuts cuts(V, E);
   const int v = cuts.at(c_first + 1);
   KvSeg s;
   int r = kv_find(s_batch, a.requests, v);
   kv_seg<RG, TL>(a, s_batch, r, v, INT32_MAX, s);
   const int rows = s.rows - s.row0 - (int)blockIdx.y * 32;  // of this CTA's 32
+  pdl_wait();
   if (s.pair_v == v || s.pair_v < cuts.at(c_first) || rows <= 0) return;
   const int c_last = cuts.share_of(s.pair_end - 1);
   KvJoined<RG, 128> j[N4];  // 4 values each
