@@ -105,14 +105,17 @@ struct KvBatch {
 // ---- the line: all pairs' tiles, one after another ---------------------------
 // A pair is (request, KV head, group of RG rows); its tokens are tiles of
 // T = 2^TL.  The line gives group g of a request S(g + 1) - S(g) places,
-//   S(g) = floor(sum over k < g of (h0 + (k + 1) slope) / T + 1),
+//   S(g) = floor(sum over k < g of (h0 + (k + 1) slope) / T + kStart),
 // where h0 + (g + 1) slope bounds the tokens the group sees: slope is RG / group
 // tokens, rounded up, for causal rows and 0 otherwise.  floor(a + x) - floor(a)
-// >= floor(x), so the places suffice for the group's tiles; the spare one
-// stands for the cost of starting a pair.  A closed form keeps causal prompts
+// >= floor(x), so kStart = 1 suffices for the group's tiles; the places beyond
+// stand for the cost of starting a pair.  A closed form keeps causal prompts
 // balanced (their groups see from few to all tokens) without a list of groups.
 template <int RG, int TL>
 struct KvLine {
+  // Tiles of 16 go by in a quarter of the time that a pair's queries, search and
+  // store take.
+  static constexpr int kStart = TL == 4 ? 4 : 1;
   int h0, slope, groups;
   __device__ __forceinline__ KvLine(const KvAttnArgs& a, const KvRequest& q) {
     h0 = q.len;
@@ -128,7 +131,7 @@ struct KvLine {
     groups = (int)(((unsigned)q.n * (unsigned)a.group + RG - 1u) / RG);
   }
   __device__ __forceinline__ int upto(int g) const {
-    return (int)(((long long)g * h0 + (long long)slope * ((long long)g * (g + 1) / 2)) >> TL) + g;
+    return (int)(((long long)g * h0 + (long long)slope * ((long long)g * (g + 1) / 2)) >> TL) + g * kStart;
   }
 };
 
@@ -176,7 +179,7 @@ inline long long kv_line_most(const KvAttnArgs& a, int rg, int tl) {
   const long long rows = (long long)a.max_new * a.group < a.rows_max ? (long long)a.max_new * a.group : a.rows_max;
   const long long groups = (rows + rg - 1) / rg;
   const long long tokens = ((long long)a.width << a.block_log2) + a.max_new + rg + (2ll << tl);
-  const long long per_head = groups * ((tokens >> tl) + 2);
+  const long long per_head = groups * ((tokens >> tl) + 5);
   return per_head > (1ll << 40) ? per_head : per_head * a.heads;
 }
 
@@ -256,7 +259,7 @@ __device__ __forceinline__ int kv_line(const KvAttnArgs& a, KvBatch<MOST>& b, in
 // One row (of RG) of a pair that crosses CTAs, joined by a warp from the CTAs'
 // partials in CTA order: lane i takes dims 4 i .. 4 i + 3 (HD = 128), or 2 i,
 // 2 i + 1.  Lanes first take a contributor's (m, l) each, so that the chain of
-// L2 trips is short: two, and one for every eight contributors' values.
+// L2 trips is short: one for every 16 contributors' values.
 template <int RG, int HD>
 struct KvJoined {
   float acc[HD / 32], M, L;
@@ -273,12 +276,30 @@ __device__ __forceinline__ KvJoined<RG, HD> kv_join(const float* partials, int s
   for (int i = 0; i < N; ++i) j.acc[i] = 0.0f;
 #pragma unroll 1
   for (int c0 = c_first; c0 <= c_last; c0 += 32) {
+    constexpr int Y = 16;
     const int n = min(c_last - c0 + 1, 32);
     float m = -INFINITY, l = 0.0f;
     if (lane < n) {
-      l = __ldcg(part(c0 + lane) + RG * HD + RG + row);
-      m = l != 0.0f ? __ldcg(part(c0 + lane) + RG * HD + row) : -INFINITY;
+      const float* p = part(c0 + lane) + RG * HD + row;
+      m = __ldcg(p);
+      l = __ldcg(p + RG);
     }
+    float x[Y][N];
+    auto load = [&](int c) {
+#pragma unroll
+      for (int y = 0; y < Y; ++y) {
+        const float* p = part(c0 + min(c + y, n - 1)) + row * HD + lane * N;
+        if (N == 4) {
+          const float4 o = __ldcg(reinterpret_cast<const float4*>(p));
+          x[y][0] = o.x; x[y][1] = o.y; x[y][N - 2] = o.z; x[y][N - 1] = o.w;
+        } else {
+          const float2 o = __ldcg(reinterpret_cast<const float2*>(p));
+          x[y][0] = o.x; x[y][1] = o.y;
+        }
+      }
+    };
+    load(0);
+    if (l == 0.0f) m = -INFINITY;  // a share that saw no token
     float top = m;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
@@ -293,21 +314,10 @@ __device__ __forceinline__ KvJoined<RG, HD> kv_join(const float* partials, int s
 #pragma unroll
     for (int i = 0; i < N; ++i) j.acc[i] *= f0;
 #pragma unroll 1
-    for (int c = 0; c < n; c += 8) {
-      float x[8][N];
+    for (int c = 0; c < n; c += Y) {
+      if (c) load(c);
 #pragma unroll
-      for (int y = 0; y < 8; ++y) {
-        const float* p = part(c0 + min(c + y, n - 1)) + row * HD + lane * N;
-        if (N == 4) {
-          const float4 o = __ldcg(reinterpret_cast<const float4*>(p));
-          x[y][0] = o.x; x[y][1] = o.y; x[y][N - 2] = o.z; x[y][N - 1] = o.w;
-        } else {
-          const float2 o = __ldcg(reinterpret_cast<const float2*>(p));
-          x[y][0] = o.x; x[y][1] = o.y;
-        }
-      }
-#pragma unroll
-      for (int y = 0; y < 8; ++y) {
+      for (int y = 0; y < Y; ++y) {
         const float w = __shfl_sync(0xFFFFFFFFu, f, c + y);  // lanes from n on hold 0
         if (w != 0.0f) {
 #pragma unroll

@@ -40,7 +40,7 @@ __device__ unsigned g_kv_decode_fault = 0;
 
 constexpr int kDecRequests = 1024;  // of a launch: they are kept in shared memory
 constexpr int kDecMinTiles = 2;   // tiles per warp below which the grid shrinks
-constexpr int kDecSnapTiles = 16;  // longest pair for which shares end with whole pairs
+constexpr int kDecSnapTiles = 19;  // longest pair, with its start, for which shares end with whole pairs
 constexpr float kDecLow = -1e30f;  // m before a row has seen a token
 
 template <int HD, int NT>
@@ -98,7 +98,7 @@ k_kv_decode(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
   __shared__ int2 s_part[2 * W];   // the pair each partial belongs to: its range on the line
   __shared__ int4 s_rows[2 * W];   // and its rows: first token row, first row, rows, head
   __shared__ int4 s_cross[2];              // pairs that cross CTAs: begun before this CTA, begun in it
-  __shared__ unsigned s_ticket[2];
+  __shared__ int2 s_joins[2];              // the CTAs of those that this CTA joins
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const uint32_t raw = su32(smem_raw), base = (raw + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - raw);
@@ -519,14 +519,21 @@ k_kv_decode(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
   }
   __syncthreads();
   // ---- pairs that cross CTAs: the last of their CTAs to arrive joins them ----------
-  if (tid < 2 && s_cross[tid].x >= 0) s_ticket[tid] = ticket_acq_rel(a.tickets + cuts.share_of(s_cross[tid].x) / W);
+  if (tid < 2) {
+    const int4 pr = s_cross[tid];
+    int c_first = 0, c_last = -1;
+    if (pr.x >= 0) {
+      const int first = cuts.share_of(pr.x) / W, last = cuts.share_of(pr.y - 1) / W;
+      if (ticket_acq_rel(a.tickets + first) == (unsigned)(last - first)) { c_first = first; c_last = last; }
+    }
+    s_joins[tid] = make_int2(c_first, c_last);
+  }
   __syncthreads();
 #pragma unroll 1
   for (int x = 0; x < 2; ++x) {
+    const int c_first = s_joins[x].x, c_last = s_joins[x].y;
+    if (c_last < 0) continue;
     const int4 pr = s_cross[x];
-    if (pr.x < 0) continue;
-    const int c_first = cuts.share_of(pr.x) / W, c_last = cuts.share_of(pr.y - 1) / W;
-    if (s_ticket[x] != (unsigned)(c_last - c_first)) continue;
     const int4 rw = s_rows[pr.z];
 #pragma unroll 1
     for (int qr = warp; qr < min(RG, rw.z - rw.y); qr += W) {
