@@ -39,8 +39,9 @@ namespace qg {
 __device__ unsigned g_kv_decode_fault = 0;
 
 constexpr int kDecRequests = 1024;  // of a launch: they are kept in shared memory
-constexpr int kDecMinTiles = 2;   // tiles per warp below which the grid shrinks
-constexpr int kDecSnapTiles = 19;  // longest pair, with its start, for which shares end with whole pairs
+// Shares end with whole pairs where those have at most so many places and the
+// fullest share then gets at most so many more than the mean.
+constexpr int kDecSnapLongest = 40, kDecSnapOver = 13;
 constexpr float kDecLow = -1e30f;  // m before a row has seen a token
 
 template <int HD, int NT>
@@ -115,12 +116,16 @@ k_kv_decode(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
   pdl_begin_after();
   int longest;
   const int V = kv_line<RG, 4, W>(a, s_batch, s_scan, longest);
-  // Short pairs are not cut: a share takes the pairs that begin in it.  One pair
-  // more in some shares costs less than joining nearly every pair.
-  const bool snap = longest <= kDecSnapTiles;
-  const int E = max(1, min((int)gridDim.x * W, V / kDecMinTiles));  // shares
+  const int E = max(1, min((int)gridDim.x * W, V));  // shares
   const int k0 = blockIdx.x * W;
   if (V == 0 || k0 >= E) return;
+  // Short pairs are not cut where that keeps the shares even: a share takes the
+  // pairs that begin in it, which costs the fullest one some tiles and saves
+  // joining nearly every pair.  Requests x tokens, 8 KV heads of 128: 200 x 100
+  // 14.7 us instead of 27.3, 200 x 500 41 instead of 52, 64 x 200 18.4 and 18.2;
+  // uneven and so cut: 64 x 300 20.5 instead of 24.2, 64 x 500 24 instead of 31.
+  const int mean = V / E;
+  const bool snap = longest <= kDecSnapLongest && (mean + longest - 1) / longest * longest - mean <= kDecSnapOver;
   const KvCuts cuts(V, E);
 
   const uint32_t ring = base + warp * Cfg::kRing;
@@ -564,8 +569,12 @@ static cudaError_t launch_decode(const CUtensorMap& mk, const CUtensorMap& mv, c
   return pdl_launch(k_kv_decode<TYPE, HD, NT>, dim3((unsigned)grid), dim3(DecCfg<HD, NT>::kWarps * 32), BYTES, s, mk, mv, a);
 }
 
-// Two row tiles of 8 when a request brings more than 8 rows per KV head.
-static int dec_nt(long long rows) { return rows > 8 ? 2 : 1; }
+// Row tiles of 8 that share a pair's codes: two when a request brings more than 8
+// rows per KV head and the pairs are enough to fill the GPU.  Measured with 2
+// tokens x 8 heads x 8 grouped, 128 dims, 4000 tokens: 1, 8 and 16 requests 20.0,
+// 29.9 and 44.7 us with two tiles, 14.4, 29.3 and 46.7 with one, whose second
+// reading of the codes mostly hits L2.
+static int dec_nt(long long rows, long long pairs) { return rows > 8 && pairs * rows > 1024 ? 2 : 1; }
 
 static cudaError_t kv_decode_launch(int type, int head_dim, int nt, const CUtensorMap& mk, const CUtensorMap& mv,
                                     const KvAttnArgs& a, int grid, cudaStream_t s) {
@@ -590,16 +599,19 @@ cudaError_t kv_decode_fault_clear() {
 }
 
 // Requests with more rows per KV head than this run on the tcgen05 kernel.
-constexpr int kKvPrefillRows = 32;
+// Measured there and here: 8 requests x 8 heads of 128 over 4096 tokens, 48 rows
+// 65 and 57 us, 64 rows 65 and 71 us; 64 requests x 8 heads of 64 over 1000 to 3000,
+// 32 rows 147 and 113 us, 40 rows 148 and 158 us.
+static int kv_prefill_rows(int head_dim) { return head_dim == 128 ? 48 : 32; }
 
 // Workspace: 4 KiB of tickets for each kernel, then their partials.
 struct KvWorkspace {
   size_t decode, prefill, total;  // byte offsets of the partials
   KvWorkspace(int head_dim, long long rows, int sm_count) {
-    const size_t slot = (size_t)8 * dec_nt(rows) * (head_dim + 2) * sizeof(float);
+    const size_t slot = (size_t)8 * dec_nt(rows, INT32_MAX) * (head_dim + 2) * sizeof(float);
     decode = 8192;
     prefill = decode + (size_t)sm_count * 2 * slot;
-    total = prefill + (rows > kKvPrefillRows ? kv_prefill_workspace(head_dim, sm_count) : 0);
+    total = prefill + (rows > kv_prefill_rows(head_dim) ? kv_prefill_workspace(head_dim, sm_count) : 0);
   }
 };
 
@@ -620,14 +632,15 @@ static qgemm_status_t kv_attention_run(const qgemm_kv_cache_t* c, KvAttnArgs a, 
   // rows enough for max_new of every request: all bring as many, and one kernel
   // takes whatever they bring.  Otherwise the decode kernel goes first and the
   // prefill kernel's CTAs take the SMs as it leaves them.
-  const bool many = rows > kKvPrefillRows, even = (long long)a.requests * a.max_new <= a.tokens;
+  const int few = kv_prefill_rows(c->head_dim);
+  const bool many = rows > few, even = (long long)a.requests * a.max_new <= a.tokens;
   for (int kernel = many && even ? 1 : 0; kernel <= (many ? 1 : 0); ++kernel) {
-    a.rows_min = kernel && !even ? kKvPrefillRows : 0;
-    a.rows_max = kernel ? INT32_MAX : kKvPrefillRows;
+    a.rows_min = kernel && !even ? few : 0;
+    a.rows_max = kernel ? INT32_MAX : few;
     a.tickets = reinterpret_cast<unsigned*>(static_cast<char*>(ws) + 4096 * kernel);
     a.partials = reinterpret_cast<float*>(static_cast<char*>(ws) + (kernel ? w.prefill : w.decode));
     // beside prompt chunks the few rows are as a rule one token's
-    const int nt = dec_nt(many ? a.group : rows);
+    const int nt = dec_nt(many ? a.group : rows, (long long)all * a.heads);
     // requests per launch: the prefix sums fit shared memory and the line 31 bits
     const long long per = kernel ? kv_line_most(a, 256, 7) : kv_line_most(a, 8 * nt, 4);
     if (per > INT32_MAX)
