@@ -74,6 +74,24 @@ struct Place {
 Tensor make(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
   return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
 }
+// Tensors of one dimension in one allocation, each on a 16-byte boundary: a plan's
+// six, made one by one, took 3 us longer.
+template <size_t N>
+void make_together(Tensor (&out)[N], const int64_t (&sizes)[N], const at::ScalarType (&types)[N], const Tensor& like) {
+  int64_t at[N], bytes = 0;
+  for (size_t i = 0; i < N; ++i) {
+    at[i] = bytes;
+    bytes += (sizes[i] * (int64_t)c10::elementSize(types[i]) + 15) / 16 * 16;
+  }
+  const Tensor whole = make({bytes}, at::kByte, like);
+  for (size_t i = 0; i < N; ++i) {
+    out[i] = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(),
+                                                      c10::scalarTypeToTypeMeta(types[i]));
+    c10::TensorImpl* t = out[i].unsafeGetTensorImpl();
+    t->set_storage_offset(at[i] / (int64_t)c10::elementSize(types[i]));
+    t->set_sizes_contiguous({sizes[i]});
+  }
+}
 // (status, result...): serving.py turns a status other than 0 into its error.
 PyObject* done(int status, std::initializer_list<const Tensor*> out) {
   PyObject* r = PyTuple_New((Py_ssize_t)out.size() + 1);
@@ -165,7 +183,7 @@ PyObject* kv_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
           refuse(W, "out was made for other sizes");
       }
     } else {
-      for (int i = 0; i < 6; ++i) o[i] = make({sizes[i]}, i == 2 ? at::kLong : at::kInt, lens);
+      make_together(o, sizes, {at::kInt, at::kInt, at::kLong, at::kInt, at::kInt, at::kInt}, lens);
     }
     const int st = qgemm_kv_plan(block, requests, ptr(lens), ptr(news), ptr(table), width, ptr(list), ptr(count), tokens,
                                  ptr(o[1]), ptr(o[0]), ptr<int64_t>(o[2]), ptr(o[3]), ptr(o[4]), ptr(o[5]),
