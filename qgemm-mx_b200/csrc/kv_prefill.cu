@@ -225,19 +225,25 @@ k_kv_prefill(const KvAttnArgs a) {
       if (s.tile >= s.tile_end) continue;
       const int32_t* row_table = a.table + (size_t)s.r * a.width;
       const uint32_t head_off = (uint32_t)(s.h << lg) * HD + ch * 16;
-      // lane i < 8: block of the i-th 16 tokens of tile x; -1 past the end or
-      // outside the pool
+      // What is loaded here is looked at a tile later: one look before its use, even
+      // a comparison, would hold the warp up for the load's round trip.
+      // lane i < 8: block of the i-th 16 tokens of tile x; -1 past the end
       auto load_id = [&](int x) {
         const long long t = (long long)x * kPreTok + lane * 16;
         int id = -1;
         if (lane < 8 && x < s.tile_end && t < s.len) id = row_table[t >> lg];
-        return id < a.blocks ? id : -1;
+        return id;
       };
-      // and its exponents, K's | V's << 8
-      auto load_exp = [&](int id) -> uint32_t {
-        if (id < 0) return 127u | (127u << 8);
-        const size_t cell = (size_t)id * a.heads + s.h;
-        return (uint32_t)__ldg(a.ks + cell) | ((uint32_t)__ldg(a.vs + cell) << 8);
+      auto in_pool = [&](int id) { return id < a.blocks ? id : -1; };
+      // and its exponents
+      uint32_t ek, ev;
+      auto load_exp = [&](int id) {
+        ek = ev = 127u;
+        if (id >= 0) {
+          const size_t cell = (size_t)id * a.heads + s.h;
+          ek = __ldg(a.ks + cell);
+          ev = __ldg(a.vs + cell);
+        }
       };
       auto load_codes = [&](const uint8_t* src, int x, int id, uint4 (&w)[PC]) {
         const int room = s.len - x * kPreTok;  // tokens of tile x (and more)
@@ -265,39 +271,34 @@ k_kv_prefill(const KvAttnArgs a) {
           sts16(p + sw128_off(row, c + 1), o[4], o[5], o[6], o[7]);
         }
       };
-      // codes and exponents are loaded one tile ahead, block ids two
+      // codes and exponents are loaded one tile ahead, block ids three
+      int id = load_id(s.tile), id1 = load_id(s.tile + 1), id2 = load_id(s.tile + 2);
       uint4 wk[PC], wv[PC];
-      int id = load_id(s.tile);
-      load_codes(a.k, s.tile, id, wk);
-      load_codes(a.v, s.tile, id, wv);
-      uint32_t exps = load_exp(id);
-      id = load_id(s.tile + 1);
-      // q: 16 (8 for 64 dims) lanes a row
-      if (n_seg > 0) ok = pre_wait(bar(Q_EMPTY), (n_seg - 1) & 1);
-      if (!ok) break;
+      // q: 16 (8 for 64 dims) lanes a row, 8 rows' loads at a time.  The first are
+      // under way while the last stretch's q is still read, the next while the first
+      // are converted: a stretch's start is a pause for all other warps.
       {
         constexpr int LPR = HD / 8;  // lanes per row
-        constexpr int STEP = kPreLoaders / LPR;
-        const int c8 = lt % LPR;
+        constexpr int STEP = kPreLoaders / LPR, BATCHES = RG / (8 * STEP);
+        const int c8 = lt % LPR, r0 = lt / LPR;
         // row0 + x over group, x < 256: exact in float
         const int i0 = s.row0 / a.group, g0 = s.row0 - i0 * a.group;
         const float inv_group = 1.0f / (float)a.group;
         const int rows = min(RG, s.rows - s.row0);
-#pragma unroll 1
-        for (int r0 = lt / LPR; r0 < RG; r0 += 4 * STEP) {
-          uint4 w[4];
+        const uint16_t* const q0 = a.q + (int64_t)(s.start + i0) * a.q_stride + (int64_t)(s.h * a.group) * a.q_head_stride + c8 * 8;
+        auto load_q = [&](int batch, uint4 (&w)[8]) {
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const int rr = r0 + y * STEP;
+          for (int y = 0; y < 8; ++y) {
+            const int rr = r0 + (batch * 8 + y) * STEP;
             const int i = (int)(((float)(g0 + rr) + 0.5f) * inv_group), gh = g0 + rr - i * a.group;
             w[y] = make_uint4(0, 0, 0, 0);
-            if (rr < rows)
-              w[y] = __ldg(reinterpret_cast<const uint4*>(a.q + (int64_t)(s.start + i0 + i) * a.q_stride +
-                                                          (int64_t)(s.h * a.group + gh) * a.q_head_stride + c8 * 8));
+            if (rr < rows) w[y] = __ldg(reinterpret_cast<const uint4*>(q0 + i * a.q_stride + gh * a.q_head_stride));
           }
+        };
+        auto put_q = [&](int batch, const uint4 (&w)[8]) {
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const int rr = r0 + y * STEP;
+          for (int y = 0; y < 8; ++y) {
+            const int rr = r0 + (batch * 8 + y) * STEP;
             const uint32_t u[4] = {w[y].x, w[y].y, w[y].z, w[y].w};
             uint32_t mx = 0;
 #pragma unroll
@@ -313,6 +314,25 @@ k_kv_prefill(const KvAttnArgs a) {
             sts16(q_addr(rr >> 7) + (uint32_t)(c8 >> 3) * 16384u + sw128_off(rr & 127, c8 & 7), o[0], o[1], o[2], o[3]);
             if (c8 == 0) s_fq[n_seg & 1][rr] = fabsf(a.scale_log2) * pow2f(e);
           }
+        };
+        uint4 wq[8];
+        load_q(0, wq);
+        if (n_seg > 0) ok = pre_wait(bar(Q_EMPTY), (n_seg - 1) & 1);
+        if (!ok) break;
+        id = in_pool(id);
+        if (BATCHES > 1) {
+          uint4 wn[8];
+          load_q(1, wn);
+          put_q(0, wq);
+          load_codes(a.k, s.tile, id, wk);
+          load_codes(a.v, s.tile, id, wv);
+          load_exp(id);
+          put_q(1, wn);
+        } else {
+          load_codes(a.k, s.tile, id, wk);
+          load_codes(a.v, s.tile, id, wv);
+          load_exp(id);
+          put_q(0, wq);
         }
         // the MMA warps' view of the stretch: tiles, and whether B has rows
         if (lt == 0) s_seg[n_seg & 1] = (s.tile_end - s.tile) * 2 + (rows > 128 ? 1 : 0);
@@ -327,20 +347,22 @@ k_kv_prefill(const KvAttnArgs a) {
         if (!ok) break;
         widen(k_addr(st), wk);
         if (lt < 8) {
-          const int ev = (int)(exps >> 8) - 127;
-          s_meta[n_tile & 3][lt] = PreMeta{u2f((exps & 0xFFu) << 23), (float)ev, pow2f(-ev), 0.0f};
+          const int e = (int)ev - 127;
+          s_meta[n_tile & 3][lt] = PreMeta{u2f(ek << 23), (float)e, pow2f(-e), 0.0f};
         }
         fence_proxy_async();
         warp_arrive(K_FULL + st);
+        id = in_pool(id1);
+        id1 = id2;
+        id2 = load_id(x + 3);
         load_codes(a.k, x + 1, id, wk);
-        exps = load_exp(id);
+        load_exp(id);
         if (n_tile >= 2) ok = pre_wait(bar(V_EMPTY + st), par ^ 1u);
         if (!ok) break;
         widen(v_addr(st), wv);
         fence_proxy_async();
         warp_arrive(V_FULL + st);
         load_codes(a.v, x + 1, id, wv);
-        id = load_id(x + 2);
       }
       ++n_seg;
     }
