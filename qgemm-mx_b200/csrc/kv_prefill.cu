@@ -583,10 +583,10 @@ k_kv_prefill(const KvAttnArgs a) {
 #pragma unroll
           for (int y = 0; y < 32; ++y) w[y] = 0u;
         }
-        if (!whole) {
+        if (!whole) {  // four dims of all rows after one another: a warp writes 512 bytes together
 #pragma unroll
           for (int y = 0; y < 8; ++y)
-            __stcg(reinterpret_cast<float4*>(slot + rr * HD + 32 * c) + y,
+            __stcg(reinterpret_cast<float4*>(slot) + (8 * c + y) * RG + rr,
                    make_float4(u2f(w[4 * y]), u2f(w[4 * y + 1]), u2f(w[4 * y + 2]), u2f(w[4 * y + 3])));
         } else if (on) {
           uint4* dst = reinterpret_cast<uint4*>(a.out + at * HD + 32 * c);
@@ -660,10 +660,10 @@ __global__ void __launch_bounds__(256) k_kv_prefill_join(const KvAttnArgs a, int
     float4 o[N4];
 #pragma unroll
     for (int i = 0; i < N4; ++i) {
-      const int e4 = i * 256 + tid, qr = blockIdx.y * 32 + e4 * 4 / HD;
+      const int qr = blockIdx.y * 32 + (tid & 31), d4 = i * 8 + (tid >> 5);
       m[i] = __ldcg(p + RG * HD + qr);
       l[i] = __ldcg(p + RG * HD + RG + qr);
-      o[i] = __ldcg(reinterpret_cast<const float4*>(p + blockIdx.y * 32 * HD) + e4);
+      o[i] = __ldcg(reinterpret_cast<const float4*>(p) + d4 * RG + qr);
     }
 #pragma unroll
     for (int i = 0; i < N4; ++i) {
@@ -677,7 +677,7 @@ __global__ void __launch_bounds__(256) k_kv_prefill_join(const KvAttnArgs a, int
   }
 #pragma unroll
   for (int i = 0; i < N4; ++i) {
-    const int e4 = i * 256 + tid, qr = e4 * 4 / HD, d = e4 * 4 % HD;
+    const int qr = tid & 31, d = 4 * (i * 8 + (tid >> 5));
     if (qr >= rows) continue;
     const int row = s.row0 + blockIdx.y * 32 + qr, tk = row / a.group;
     const int64_t at = (int64_t)(s.start + tk) * (a.heads * a.group) + s.h * a.group + row - tk * a.group;
