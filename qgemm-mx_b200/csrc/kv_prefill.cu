@@ -127,6 +127,11 @@ __device__ __forceinline__ void add2(float& a, float& b, float c, float d) {
       "  add.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x; }"
       : "+f"(a), "+f"(b) : "f"(c), "f"(d));
 }
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
 __device__ __forceinline__ void sts16(uint32_t p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(p), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -206,7 +211,7 @@ k_kv_prefill(const KvAttnArgs a) {
   };
 
   if (warp >= kPreLoad && warp < kPreMma) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     // ---- widening: codes -> f16 operand tiles ------------------------------------
     const int lt = tid - kPreLoad * 32;  // 0 .. 255
     constexpr int CPR = HD / 16;         // 16-code pieces per token
@@ -274,65 +279,74 @@ k_kv_prefill(const KvAttnArgs a) {
       // codes and exponents are loaded one tile ahead, block ids three
       int id = load_id(s.tile), id1 = load_id(s.tile + 1), id2 = load_id(s.tile + 2);
       uint4 wk[PC], wv[PC];
-      // q: 16 (8 for 64 dims) lanes a row, 8 rows' loads at a time.  The first are
-      // under way while the last stretch's q is still read, the next while the first
-      // are converted: a stretch's start is a pause for all other warps.
+      // q: 16 (8 for 64 dims) lanes a row.  All of its loads are under way while the
+      // last stretch's q is still read and before that stretch's partials are
+      // written, whose stores would hold them up for some 5000 cycles: a stretch's
+      // start is a pause for all other warps.
       {
         constexpr int LPR = HD / 8;  // lanes per row
-        constexpr int STEP = kPreLoaders / LPR, BATCHES = RG / (8 * STEP);
+        constexpr int STEP = kPreLoaders / LPR, BATCHES = RG / (4 * STEP);
         const int c8 = lt % LPR, r0 = lt / LPR;
         // row0 + x over group, x < 256: exact in float
         const int i0 = s.row0 / a.group, g0 = s.row0 - i0 * a.group;
         const float inv_group = 1.0f / (float)a.group;
         const int rows = min(RG, s.rows - s.row0);
         const uint16_t* const q0 = a.q + (int64_t)(s.start + i0) * a.q_stride + (int64_t)(s.h * a.group) * a.q_head_stride + c8 * 8;
-        auto load_q = [&](int batch, uint4 (&w)[8]) {
+        auto load_q = [&](int batch, uint4 (&w)[4]) {
 #pragma unroll
-          for (int y = 0; y < 8; ++y) {
-            const int rr = r0 + (batch * 8 + y) * STEP;
+          for (int y = 0; y < 4; ++y) {
+            const int rr = r0 + (batch * 4 + y) * STEP;
             const int i = (int)(((float)(g0 + rr) + 0.5f) * inv_group), gh = g0 + rr - i * a.group;
             w[y] = make_uint4(0, 0, 0, 0);
             if (rr < rows) w[y] = __ldg(reinterpret_cast<const uint4*>(q0 + i * a.q_stride + gh * a.q_head_stride));
           }
         };
-        auto put_q = [&](int batch, const uint4 (&w)[8]) {
+        auto put_q = [&](int batch, const uint4 (&w)[4]) {
+          uint32_t mx[4];  // the rows' maxima side by side, one chain of shuffles for all
 #pragma unroll
-          for (int y = 0; y < 8; ++y) {
-            const int rr = r0 + (batch * 8 + y) * STEP;
+          for (int y = 0; y < 4; ++y) {
+            mx[y] = max_u16x2(max_u16x2(w[y].x & 0x7FFF7FFFu, w[y].y & 0x7FFF7FFFu),
+                              max_u16x2(w[y].z & 0x7FFF7FFFu, w[y].w & 0x7FFF7FFFu));
+          }
+#pragma unroll
+          for (int d = 1; d < LPR; d <<= 1)
+#pragma unroll
+            for (int y = 0; y < 4; ++y) mx[y] = max_u16x2(mx[y], __shfl_xor_sync(0xFFFFFFFFu, mx[y], d));
+          uint32_t o[4][4];
+          float fq[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
             const uint32_t u[4] = {w[y].x, w[y].y, w[y].z, w[y].w};
-            uint32_t mx = 0;
-#pragma unroll
-            for (int z = 0; z < 4; ++z) mx = max(mx, max(u[z] & 0x7FFFu, (u[z] >> 16) & 0x7FFFu));
-#pragma unroll
-            for (int d = 1; d < LPR; d <<= 1) mx = max(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, d));
-            const int e = mx >= 0x7F80u || mx < 0x0080u ? 0 : min((int)(mx >> 7) - 127, 126);
+            const uint32_t top = max(mx[y] & 0xFFFFu, mx[y] >> 16);
+            const int e = top >= 0x7F80u || top < 0x0080u ? 0 : min((int)(top >> 7) - 127, 126);
             // the sign of the scale goes into q, so that factors are never negative
             const float down = a.scale_log2 < 0.0f ? -pow2f(-e) : pow2f(-e);
-            uint32_t o[4];
 #pragma unroll
-            for (int z = 0; z < 4; ++z) o[z] = pack_f16(u2f(u[z] << 16) * down, u2f(u[z] & 0xFFFF0000u) * down);
-            sts16(q_addr(rr >> 7) + (uint32_t)(c8 >> 3) * 16384u + sw128_off(rr & 127, c8 & 7), o[0], o[1], o[2], o[3]);
-            if (c8 == 0) s_fq[n_seg & 1][rr] = fabsf(a.scale_log2) * pow2f(e);
+            for (int z = 0; z < 4; ++z) o[y][z] = pack_f16(u2f(u[z] << 16) * down, u2f(u[z] & 0xFFFF0000u) * down);
+            fq[y] = fabsf(a.scale_log2) * pow2f(e);
+          }
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const int rr = r0 + (batch * 4 + y) * STEP;
+            sts16(q_addr(rr >> 7) + (uint32_t)(c8 >> 3) * 16384u + sw128_off(rr & 127, c8 & 7), o[y][0], o[y][1], o[y][2],
+                  o[y][3]);
+            if (c8 == 0) s_fq[n_seg & 1][rr] = fq[y];
           }
         };
-        uint4 wq[8];
-        load_q(0, wq);
+        uint4 wq[BATCHES][4];
+#pragma unroll
+        for (int k = 0; k < BATCHES; ++k) load_q(k, wq[k]);
+        id = in_pool(id);
+        load_exp(id);
         if (n_seg > 0) ok = pre_wait(bar(Q_EMPTY), (n_seg - 1) & 1);
         if (!ok) break;
-        id = in_pool(id);
-        if (BATCHES > 1) {
-          uint4 wn[8];
-          load_q(1, wn);
-          put_q(0, wq);
-          load_codes(a.k, s.tile, id, wk);
-          load_codes(a.v, s.tile, id, wv);
-          load_exp(id);
-          put_q(1, wn);
-        } else {
-          load_codes(a.k, s.tile, id, wk);
-          load_codes(a.v, s.tile, id, wv);
-          load_exp(id);
-          put_q(0, wq);
+#pragma unroll
+        for (int k = 0; k < BATCHES; ++k) {
+          put_q(k, wq[k]);
+          if (k == BATCHES / 2 - 1) {  // into the registers of the queries that are done
+            load_codes(a.k, s.tile, id, wk);
+            load_codes(a.v, s.tile, id, wv);
+          }
         }
         // the MMA warps' view of the stretch: tiles, and whether B has rows
         if (lt == 0) s_seg[n_seg & 1] = (s.tile_end - s.tile) * 2 + (rows > 128 ? 1 : 0);
@@ -373,7 +387,7 @@ k_kv_prefill(const KvAttnArgs a) {
       warp_arrive(Q_FULL);
     }
   } else if (warp >= kPreMma) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp < kPreMma + 2) {
       constexpr uint32_t id_qk = idesc_f16(128, 64), id_pv = idesc_f16(128, HD) | (1u << 16);
       const uint32_t one = lane == 0, tm = __reduce_or_sync(0xFFFFFFFFu, tmem);  // uniform
