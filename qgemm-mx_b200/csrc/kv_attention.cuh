@@ -116,7 +116,9 @@ struct KvLine {
   // Tiles of 16 go by in a quarter of the time that a pair's queries, search and
   // store take: 64 requests of 129 to 8192 tokens 97.5 us, 200 in a window of 128
   // 18.8 us, against 102 and 20.5 with 2, 97.5 and 19.6 with 8, 108 and 29.8 with 1.
-  static constexpr int kStart = TL == 4 ? 4 : 1;
+  // Of the prefill kernel's 128 tokens a start weighs three: 13 decoding requests and 3
+  // prompt chunks of up to 512 tokens 126 us, 138 with 1, 129 with 5.
+  static constexpr int kStart = TL == 4 ? 4 : 3;
   int h0, slope, groups;
   __device__ __forceinline__ KvLine(const KvAttnArgs& a, const KvRequest& q) {
     h0 = q.len;

@@ -19,14 +19,17 @@
 // swizzled operand tiles, their global loads one tile ahead in registers; 16 and
 // 17 issue the MMAs of A and B (a commit holds up the warp that issues it for some
 // 80 cycles: two warps overlap them).  Widening costs 2 conversions per 4 codes
-// once per 256 rows.  Registers go where the data waits: 128 a softmax thread, 80
-// a widening one, 56 in the MMA warps' group (together no more than the launch's
+// once per 256 rows.  Registers go where the data waits: 128 a softmax thread, 88
+// a widening one, 40 in the MMA warps' group (together no more than the launch's
 // 640 x 96).  (Codes by TMA into a ring of 64-token units, the room that is left
 // beside the operand tiles, 24 KB: its round trip was longer than the ring.)
 //
-// What bounds it: exponentials.  A row and token cost one ex2, 16 a clock and
-// SM, as long as its 2 x 2 x 128 multiply-adds take the tensor core at 128
-// dims; at 64 dims the tensor core needs half of that.
+// What bounds it: exponentials and the tensor core alike (a row and token cost one
+// ex2, 16 a clock and SM, as long as its 2 x 2 x 128 multiply-adds take at 128
+// dims), and above that the roles' waiting for one another.  Measured, 2048 rows of
+// 32 heads over 8 KV heads of 128 dims and 8192 tokens: 295 us, 816 TFLOP/s; a tile
+// of 128 tokens takes some 4400 cycles where its MMAs take 3200, a stretch's start
+// 15000.
 //
 // The line of all pairs' tiles is cut into one equal share per CTA
 // (kv_attention.cuh), so all CTAs finish together whatever the pair count; pairs
