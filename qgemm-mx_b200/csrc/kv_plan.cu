@@ -142,7 +142,9 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(const PlanArgs a) {
       for (int step = kPlanChunk / 2; step; step >>= 1)
         if (s_start[b + step] <= t) b += step;
       const int r = r0 + b, len = s_len[b];
-      const int at_t = len + (t - s_start[b]), blk = at_t >> lg, off = at_t & ((1 << lg) - 1);
+      // 64 bits: a request that is refused may hold close to 2^31 tokens
+      const long long at_t = (long long)len + (t - s_start[b]);
+      const int blk = (int)(at_t >> lg), off = (int)at_t & ((1 << lg) - 1);
       const int taken = s_upto[b];
       int64_t slot = -1;
       if (taken >= 0) {
@@ -157,7 +159,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(const PlanArgs a) {
         slot = ((int64_t)id << lg) + off;
       }
       a.slots[t] = slot;
-      a.positions[t] = taken >= 0 ? at_t : -1;
+      a.positions[t] = taken >= 0 ? (int)at_t : -1;
       if (t == s_start[b] || off == 0) {
         const int k = s_run[b] + blk - (len >> lg);
         if (k < a.max_runs) a.runs[k] = t;
