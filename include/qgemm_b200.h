@@ -300,7 +300,8 @@ typedef struct {
 /* Block tables and slot maps from the requests' lengths.  Request r holds
  * lens[r] tokens and brings news[r] (negative: 0); its new tokens are rows
  * starts[r] .. starts[r + 1] - 1 of the step's activations, starts being the
- * exclusive prefix sum.  New blocks come off the end of the free list
+ * exclusive prefix sum (which stops at 2^30, past any row).  New blocks come
+ * off the end of the free list
  * (free_list[*free_count - 1] first) in request order and go into
  * table[r][ceil(lens[r] / block) ..].  A request is refused, and takes no
  * block, if its length is negative, if its tokens exceed its row of the

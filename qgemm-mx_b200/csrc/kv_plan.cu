@@ -38,6 +38,8 @@ struct PlanSize {
   int len, n, have, need, touched;
   bool fits;  // its tokens fit its row of the table
 };
+// Sums that stop at 2^30; the terms are at most that each, so 32 bits unsigned hold them.
+__device__ __forceinline__ int sat_add(int a, int b) { return (int)min((unsigned)a + (unsigned)b, (unsigned)kKvMaxTokens); }
 // Blocks that n tokens after the first len touch.
 __device__ __forceinline__ int runs_of(int len, int n, int lg) {
   return n > 0 ? (int)(((long long)len + n - 1) >> lg) - (len >> lg) + 1 : 0;
@@ -78,7 +80,8 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(const PlanArgs a) {
       z[i] = r < a.requests ? plan_size(a.lens[r], a.news[r], a.width, lg) : PlanSize{0, 0, 0, 0, 0, true};
       tok += z[i].n; need += z[i].need; run += z[i].touched;
     }
-    // Sums saturate at 2^30: rows past `tokens` are never written.
+    // Sums stop at 2^30: rows past `tokens` are never written, and no request is granted
+    // blocks where their count has stopped.
     int sums[3] = {(int)min(tok, (long long)kKvMaxTokens), min(need, kKvMaxTokens), min(run, kKvMaxTokens)};
     int incl[3];
 #pragma unroll
@@ -87,7 +90,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(const PlanArgs a) {
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const int u = __shfl_up_sync(0xFFFFFFFFu, v, d);
-        if (lane >= d) v = min(v + u, kKvMaxTokens);
+        if (lane >= d) v = sat_add(v, u);
       }
       incl[k] = v;
       if (lane == 31) s_warp[k][warp] = v;
@@ -100,19 +103,19 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(const PlanArgs a) {
 #pragma unroll
       for (int w = 0; w < kPlanThreads / 32; ++w) {
         if (w == warp) b = t;
-        t = min(t + s_warp[k][w], kKvMaxTokens);
+        t = sat_add(t, s_warp[k][w]);
       }
       const int up = __shfl_up_sync(0xFFFFFFFFu, incl[k], 1);
-      before[k] = min(b + (lane ? up : 0), kKvMaxTokens);
+      before[k] = sat_add(b, lane ? up : 0);
       total[k] = t;
     }
     long long at = base_tok + before[0];
-    int upto = min(base_need + before[1], kKvMaxTokens), runs = min(base_run + before[2], kKvMaxTokens);
+    int upto = sat_add(base_need, before[1]), runs = sat_add(base_run, before[2]);
 #pragma unroll
     for (int i = 0; i < kPlanItems; ++i) {
       const int j = tid * kPlanItems + i, r = r0 + j;
-      upto = min(upto + z[i].need, kKvMaxTokens);
-      const bool granted = z[i].fits && at + z[i].n <= a.tokens && (z[i].need == 0 || upto <= count);
+      upto = sat_add(upto, z[i].need);
+      const bool granted = z[i].fits && at + z[i].n <= a.tokens && (z[i].need == 0 || (upto <= count && upto < kKvMaxTokens));
       s_start[j] = (int)min(at, (long long)kKvMaxTokens);
       s_upto[j] = granted ? upto - z[i].need : -1;
       s_run[j] = runs;
@@ -127,12 +130,12 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(const PlanArgs a) {
         }
       }
       at = min(at + z[i].n, (long long)kKvMaxTokens);
-      runs = min(runs + z[i].touched, kKvMaxTokens);
+      runs = sat_add(runs, z[i].touched);
     }
     base_tok = min(base_tok + total[0], (long long)kKvMaxTokens);
     if (tid == kPlanThreads - 1) s_start[kPlanChunk] = (int)base_tok;
-    base_need = min(base_need + total[1], kKvMaxTokens);
-    base_run = min(base_run + total[2], kKvMaxTokens);
+    base_need = sat_add(base_need, total[1]);
+    base_run = sat_add(base_run, total[2]);
     __syncthreads();
     // tokens of this chunk in this CTA's range
     const int lo = max(t0, s_start[0]), hi = min(t1, s_start[kPlanChunk]);

@@ -1,8 +1,9 @@
 """The serving operators at the edges of what their entry points promise: lengths
 and counts near 2^31, block ids outside the pool, calls on other streams."""
 import pytest
+import serving_ref as R
 import torch
-from test_gpu_kv_cache import check_plan, make_step
+from test_gpu_kv_cache import check_plan, i32, make_step
 
 pytestmark = pytest.mark.gpu
 
@@ -20,3 +21,23 @@ def test_plan_refuses_lengths_that_pass_31_bits(qg, cuda, block):
     lens, new, table, free = make_step(21, 1500, 40, 3, block)
     lens[3], lens[1100], lens[1499] = TOP, TOP - 1, TOP - 5
     check_plan(qg, lens, new, table, free, block, sum(new))
+
+
+@pytest.mark.parametrize("new", [
+    [2 ** 30, 2 ** 30, 1], [TOP, TOP, 2, 1], [3, TOP, TOP, TOP, TOP, 1], [2 ** 30 - 1, 1, 1], [2, 2 ** 30, 2 ** 30 - 1, 4],
+    [1] * 40 + [2 ** 30] * 6 + [1] * 40, [1] * 600 + [TOP] * 900 + [1],
+])
+def test_plan_refuses_counts_that_pass_30_bits(qg, cuda, new):
+    """Row and block counts whose sums pass 2^30 and 2^31: starts stop at 2^30 and no
+    request behind them is granted rows."""
+    block, tokens = 16, 700
+    lens = [(5 * i) % 16 for i in range(len(new))]
+    table = [[3] * 2 for _ in new]
+    free = list(range(10, 700))
+    want = R.plan(lens, new, table, free, len(free), block, tokens)
+    tab = torch.tensor(table, dtype=torch.int32, device="cuda")
+    p = qg.kv_plan(i32(lens), i32(new), tab, i32(free), i32([len(free)]), block, tokens)
+    assert tab.tolist() == want[0] and p.lens.tolist() == want[1]
+    assert p.starts.tolist() == [min(s, 2 ** 30) for s in want[2]]
+    assert p.slots.tolist() == want[3] and p.positions.tolist() == want[4]
+    assert p.runs.tolist() == want[5] and p.counts.tolist() == want[6]
