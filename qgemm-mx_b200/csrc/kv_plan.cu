@@ -214,6 +214,8 @@ qgemm_status_t qgemm_kv_plan(int32_t block, int32_t requests, const int32_t* len
   if (requests < 0 || tokens < 0 || table_width < 0)
     return fail(QGEMM_ERR_INVALID_ARG, "kv_plan: negative size");
   if (tokens >= kKvMaxTokens) return fail(QGEMM_ERR_INVALID_ARG, "kv_plan: at most 2^30 - 1 rows");
+  if ((long long)table_width * block > INT32_MAX)  // lengths and positions have 32 bits
+    return fail(QGEMM_ERR_UNSUPPORTED_SHAPE, "kv_plan: table rows of more than 2^31 - 1 tokens");
   if (!free_count || !starts || !runs || !counts || (requests && (!lens || !news || !lens_out)) ||
       (requests && table_width && !table) || (tokens && (!slots || !positions)))
     return fail(QGEMM_ERR_INVALID_ARG, "kv_plan: null pointer");
