@@ -315,8 +315,10 @@ typedef struct {
  * count as end marks, and counts [4]: free blocks left, runs, rows, refused
  * requests.  free_list and *free_count are not changed: the caller keeps
  * counts[0] as the next call's free_count and pushes a finished request's
- * blocks back behind it.  A null free_list is an empty one.  lens_out must not
- * be lens.  table_width * block is at most 2^31 - 1.                         */
+ * blocks back behind it.  A null free_list is an empty one.  No output
+ * may overlap an input (a plan's counts[0] is not free_count of a call that
+ * writes the same counts) or another output.  table_width * block is at most
+ * 2^31 - 1.                                                                  */
 int32_t qgemm_kv_max_runs(int32_t requests, int32_t tokens, int32_t block);
 qgemm_status_t qgemm_kv_plan(int32_t block, int32_t requests, const int32_t* lens,
                              const int32_t* news, int32_t* table, int32_t table_width,

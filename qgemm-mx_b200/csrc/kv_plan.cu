@@ -194,6 +194,33 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(const PlanArgs a) {
   }
 }
 
+// Two of the call's buffers that share a byte, one of them an output: CTAs read the inputs
+// while others write the outputs.
+struct PlanSpan {
+  const char* name;
+  const void* at;
+  long long bytes;
+};
+static bool plan_overlap(const PlanArgs& a, const char** x, const char** y) {
+  const long long R = a.requests, T = a.tokens;
+  const PlanSpan spans[] = {
+      {"lens_out", a.lens_out, 4 * R}, {"starts", a.starts, 4 * R + 4}, {"slots", a.slots, 8 * T},
+      {"positions", a.positions, 4 * T}, {"runs", a.runs, 4 * (a.max_runs + 1ll)}, {"counts", a.counts, 16},
+      {"lens", a.lens, 4 * R}, {"news", a.news, 4 * R}, {"table", a.table, 4 * R * a.width},
+      {"free_list", a.free_list, a.free_list ? 4 : 0}, {"free_count", a.free_count, 4}};
+  constexpr int outputs = 6, all = sizeof(spans) / sizeof(spans[0]);
+  for (int i = 0; i < outputs; ++i)
+    for (int j = i + 1; j < all; ++j) {
+      const uintptr_t p = reinterpret_cast<uintptr_t>(spans[i].at), q = reinterpret_cast<uintptr_t>(spans[j].at);
+      if (spans[i].bytes > 0 && spans[j].bytes > 0 && p < q + spans[j].bytes && q < p + spans[i].bytes) {
+        *x = spans[i].name;
+        *y = spans[j].name;
+        return true;
+      }
+    }
+  return false;
+}
+
 }  // namespace qg
 
 using namespace qg;
@@ -219,8 +246,6 @@ qgemm_status_t qgemm_kv_plan(int32_t block, int32_t requests, const int32_t* len
   if (!free_count || !starts || !runs || !counts || (requests && (!lens || !news || !lens_out)) ||
       (requests && table_width && !table) || (tokens && (!slots || !positions)))
     return fail(QGEMM_ERR_INVALID_ARG, "kv_plan: null pointer");
-  if (lens_out && lens_out == lens)
-    return fail(QGEMM_ERR_INVALID_ARG, "kv_plan: lens_out must not be lens: CTAs read lens while others write");
   PlanArgs a;
   a.lens = lens; a.news = news; a.table = table; a.free_list = free_list; a.free_count = free_count;
   a.requests = requests; a.width = table_width; a.tokens = tokens;
@@ -228,6 +253,9 @@ qgemm_status_t qgemm_kv_plan(int32_t block, int32_t requests, const int32_t* len
   a.max_runs = qgemm_kv_max_runs(requests, tokens, block);
   a.lens_out = lens_out; a.starts = starts; a.slots = slots; a.positions = positions; a.runs = runs;
   a.counts = counts;
+  const char *x = nullptr, *y = nullptr;
+  if (plan_overlap(a, &x, &y))
+    return fail(QGEMM_ERR_INVALID_ARG, "kv_plan: %s and %s overlap: CTAs read inputs while others write outputs", x, y);
   DevProps dp;
   qgemm_status_t st = device_props(&dp);
   if (st != QGEMM_OK) return st;

@@ -84,7 +84,8 @@ def kv_plan(lens: torch.Tensor, new: torch.Tensor, table: torch.Tensor, free_lis
     `lens`; new block ids go into `table` [requests, width].  `tokens` is the
     step's row count (rows no request covers get slot -1).  Nothing is read
     back: plan.counts[3] tells on the device how many requests were refused.
-    With `out` (an earlier plan of the same sizes) nothing is allocated."""
+    With `out` (an earlier plan of the same sizes) nothing is allocated; lens,
+    new and free_count must then not be that plan's own tensors."""
     kept = None if out is None else (out.starts, out.lens, out.slots, out.positions, out.runs, out.counts)
     st, *got = _b.kv_plan(lens, new, table, free_list, free_count, block, tokens, kept, _handle(stream))
     if st:

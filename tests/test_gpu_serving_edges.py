@@ -41,3 +41,20 @@ def test_plan_refuses_counts_that_pass_30_bits(qg, cuda, new):
     assert p.starts.tolist() == [min(s, 2 ** 30) for s in want[2]]
     assert p.slots.tolist() == want[3] and p.positions.tolist() == want[4]
     assert p.runs.tolist() == want[5] and p.counts.tolist() == want[6]
+
+
+def test_plan_refuses_its_own_outputs_as_inputs(qg, cuda):
+    lens, new, table, free = make_step(31, 9, 90, 12, 32)
+    tab = torch.tensor(table, dtype=torch.int32, device="cuda")
+    tokens = sum(new)
+
+    def call(a, b, count, out):
+        return qg.kv_plan(a, b, tab, i32(free), count, 32, tokens, out=out)
+
+    p = call(i32(lens), i32(new), i32([len(free)]), None)
+    for args in ((p.lens, i32(new), i32([3])), (i32(lens), p.lens, i32([3])), (i32(lens), i32(new), p.counts[:1]),
+                 (i32(lens), i32(new), p.counts[3:]), (i32(lens), p.starts[1:], i32([3]))):
+        with pytest.raises(ValueError, match="overlap"):
+            call(*args, p)
+    other = call(i32(lens), i32(new), i32([len(free)]), None)
+    call(p.lens, i32(new), p.counts[:1], other)  # another plan's are inputs like any

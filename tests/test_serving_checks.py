@@ -17,3 +17,23 @@ def test_plan_refuses_table_rows_past_31_bits(qg, block):
     """A granted request's length and positions are 32-bit numbers."""
     assert plan(qg, block=block, width=2 ** 31 // block) == qg.ERR_UNSUPPORTED_SHAPE
     assert plan(qg, block=block, width=2 ** 31 - 1) == qg.ERR_UNSUPPORTED_SHAPE
+
+
+INPUTS = {"lens": 8, "news": 8, "table": 32, "count": 4}  # bytes that 2 requests, 4 table columns and 5 rows take
+OUTPUTS = {"lens_out": 8, "starts": 12, "slots": 40, "positions": 20, "runs": 20, "counts": 16}
+
+
+@pytest.mark.parametrize("out", list(OUTPUTS))
+def test_plan_refuses_outputs_on_inputs_and_on_each_other(qg, out):
+    """Blocks of the launch read the inputs while others write the outputs, so no output
+    may share a byte with an input (counts[0] is the next call's free_count: not in the
+    same call) nor with another output."""
+    at = {"lens": M, "news": 2 * M, "table": 3 * M, "count": 5 * M, "lens_out": 6 * M, "starts": 7 * M, "slots": 8 * M,
+          "positions": 9 * M, "runs": 10 * M, "counts": 11 * M}
+    for other, size in {**INPUTS, **OUTPUTS}.items():
+        if other == out:
+            continue
+        for shift in (0, size - 4, 4 - OUTPUTS[out]):  # equal, and one word shared at either end
+            assert plan(qg, **{out: at[other] + shift}) == qg.ERR_INVALID_ARG, (other, shift)
+            assert b"overlap" in qg.lib().qgemm_last_error_message(), (other, shift)
+    assert plan(qg, **{out: 4 * M}) == qg.ERR_INVALID_ARG  # the free list, whose first entry may be read
