@@ -326,6 +326,15 @@ qgemm_status_t qgemm_kv_plan(int32_t block, int32_t requests, const int32_t* len
                              int32_t tokens, int32_t* lens_out, int32_t* starts,
                              int64_t* slots, int32_t* positions, int32_t* runs,
                              int32_t* counts, void* stream);
+/* The same with the free list's length: a *free_count past it counts as
+ * free_len (qgemm_kv_plan trusts *free_count).                               */
+qgemm_status_t qgemm_kv_plan_bounded(int32_t block, int32_t requests, const int32_t* lens,
+                                     const int32_t* news, int32_t* table, int32_t table_width,
+                                     const int32_t* free_list, int32_t free_len,
+                                     const int32_t* free_count, int32_t tokens,
+                                     int32_t* lens_out, int32_t* starts, int64_t* slots,
+                                     int32_t* positions, int32_t* runs, int32_t* counts,
+                                     void* stream);
 
 /* Quantises the step's K and V rows (bf16 bits, [tokens][heads][head_dim],
  * tokens *_stride and heads *_head_stride elements apart, head_dim values

@@ -185,9 +185,9 @@ PyObject* kv_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
     } else {
       make_together(o, sizes, {at::kInt, at::kInt, at::kLong, at::kInt, at::kInt, at::kInt}, lens);
     }
-    const int st = qgemm_kv_plan(block, requests, ptr(lens), ptr(news), ptr(table), width, ptr(list), ptr(count), tokens,
-                                 ptr(o[1]), ptr(o[0]), ptr<int64_t>(o[2]), ptr(o[3]), ptr(o[4]), ptr(o[5]),
-                                 place.stream);
+    const int st = qgemm_kv_plan_bounded(block, requests, ptr(lens), ptr(news), ptr(table), width, ptr(list),
+                                         fits(list.numel(), W), ptr(count), tokens, ptr(o[1]), ptr(o[0]),
+                                         ptr<int64_t>(o[2]), ptr(o[3]), ptr(o[4]), ptr(o[5]), place.stream);
     return done(st, {&o[0], &o[1], &o[2], &o[3], &o[4], &o[5]});
   });
 }

@@ -27,6 +27,7 @@ struct PlanArgs {
   const int32_t *lens, *news;
   int32_t* table;
   const int32_t *free_list, *free_count;
+  int32_t free_len;  // entries of the free list
   int32_t requests, width, block_log2, tokens, max_runs;
   int32_t *lens_out, *starts;
   int64_t* slots;
@@ -63,7 +64,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(const PlanArgs a) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int lg = a.block_log2;
   pdl_begin();
-  const int count = a.free_list ? max(*a.free_count, 0) : 0;
+  const int count = a.free_list ? min(max(*a.free_count, 0), a.free_len) : 0;
   // this CTA's rows
   const int t0 = (int)((long long)blockIdx.x * a.tokens / gridDim.x);
   const int t1 = (int)((long long)(blockIdx.x + 1) * a.tokens / gridDim.x);
@@ -207,7 +208,7 @@ static bool plan_overlap(const PlanArgs& a, const char** x, const char** y) {
       {"lens_out", a.lens_out, 4 * R}, {"starts", a.starts, 4 * R + 4}, {"slots", a.slots, 8 * T},
       {"positions", a.positions, 4 * T}, {"runs", a.runs, 4 * (a.max_runs + 1ll)}, {"counts", a.counts, 16},
       {"lens", a.lens, 4 * R}, {"news", a.news, 4 * R}, {"table", a.table, 4 * R * a.width},
-      {"free_list", a.free_list, a.free_list ? 4 : 0}, {"free_count", a.free_count, 4}};
+      {"free_list", a.free_list, !a.free_list ? 0 : a.free_len == INT32_MAX ? 4 : 4ll * a.free_len}, {"free_count", a.free_count, 4}};
   constexpr int outputs = 6, all = sizeof(spans) / sizeof(spans[0]);
   for (int i = 0; i < outputs; ++i)
     for (int j = i + 1; j < all; ++j) {
@@ -233,12 +234,13 @@ int32_t qgemm_kv_max_runs(int32_t requests, int32_t tokens, int32_t block) {
   return (int32_t)(b < tokens ? b : tokens);
 }
 
-qgemm_status_t qgemm_kv_plan(int32_t block, int32_t requests, const int32_t* lens, const int32_t* news,
-                             int32_t* table, int32_t table_width, const int32_t* free_list,
-                             const int32_t* free_count, int32_t tokens, int32_t* lens_out, int32_t* starts,
-                             int64_t* slots, int32_t* positions, int32_t* runs, int32_t* counts, void* stream) {
+qgemm_status_t qgemm_kv_plan_bounded(int32_t block, int32_t requests, const int32_t* lens, const int32_t* news,
+                                     int32_t* table, int32_t table_width, const int32_t* free_list, int32_t free_len,
+                                     const int32_t* free_count, int32_t tokens, int32_t* lens_out, int32_t* starts,
+                                     int64_t* slots, int32_t* positions, int32_t* runs, int32_t* counts,
+                                     void* stream) {
   if (!kv_block_ok(block)) return fail(QGEMM_ERR_INVALID_ARG, "kv_plan: block must be 16, 32, 64 or 128 tokens");
-  if (requests < 0 || tokens < 0 || table_width < 0)
+  if (requests < 0 || tokens < 0 || table_width < 0 || free_len < 0)
     return fail(QGEMM_ERR_INVALID_ARG, "kv_plan: negative size");
   if (tokens >= kKvMaxTokens) return fail(QGEMM_ERR_INVALID_ARG, "kv_plan: at most 2^30 - 1 rows");
   if ((long long)table_width * block > INT32_MAX)  // lengths and positions have 32 bits
@@ -248,6 +250,7 @@ qgemm_status_t qgemm_kv_plan(int32_t block, int32_t requests, const int32_t* len
     return fail(QGEMM_ERR_INVALID_ARG, "kv_plan: null pointer");
   PlanArgs a;
   a.lens = lens; a.news = news; a.table = table; a.free_list = free_list; a.free_count = free_count;
+  a.free_len = free_len;
   a.requests = requests; a.width = table_width; a.tokens = tokens;
   a.block_log2 = block == 16 ? 4 : block == 32 ? 5 : block == 64 ? 6 : 7;
   a.max_runs = qgemm_kv_max_runs(requests, tokens, block);
@@ -263,6 +266,14 @@ qgemm_status_t qgemm_kv_plan(int32_t block, int32_t requests, const int32_t* len
   grid = grid < 1 ? 1 : grid > dp.sm_count ? dp.sm_count : grid;
   QG_CUDA_RET(pdl_launch(k_kv_plan, dim3((unsigned)grid), dim3(kPlanThreads), 0, as_stream(stream), a));
   return QGEMM_OK;
+}
+
+qgemm_status_t qgemm_kv_plan(int32_t block, int32_t requests, const int32_t* lens, const int32_t* news,
+                             int32_t* table, int32_t table_width, const int32_t* free_list,
+                             const int32_t* free_count, int32_t tokens, int32_t* lens_out, int32_t* starts,
+                             int64_t* slots, int32_t* positions, int32_t* runs, int32_t* counts, void* stream) {
+  return qgemm_kv_plan_bounded(block, requests, lens, news, table, table_width, free_list, INT32_MAX, free_count, tokens,
+                               lens_out, starts, slots, positions, runs, counts, stream);
 }
 
 }  // extern "C"

@@ -25,6 +25,8 @@ NORM_KINDS = {"rms": 0, "layer": 1}
 
 _sig("qgemm_kv_max_runs", _i32, [_i32, _i32, _i32])
 _sig("qgemm_kv_plan", _i32, [_i32, _i32] + [C.c_void_p] * 3 + [_i32] + [C.c_void_p] * 2 + [_i32] + [C.c_void_p] * 7)
+_sig("qgemm_kv_plan_bounded", _i32, [_i32, _i32] + [C.c_void_p] * 3 + [_i32, C.c_void_p, _i32, C.c_void_p, _i32] +
+     [C.c_void_p] * 7)
 _sig("qgemm_kv_append", _i32, [C.c_void_p] * 3 + [C.c_int64] * 4 + [_i32, C.c_void_p, C.c_void_p, _i32, C.c_void_p])
 _sig("qgemm_kv_attention_workspace", _sz, [C.c_void_p, _i32, _i32, _i32, _i32])
 _sig("qgemm_kv_attention", _i32, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, _i32, _i32] + [C.c_void_p] * 3 +
@@ -82,7 +84,8 @@ def kv_plan(lens: torch.Tensor, new: torch.Tensor, table: torch.Tensor, free_lis
             free_count: torch.Tensor, block: int, tokens: int, out: KVPlan | None = None, stream=None) -> KVPlan:
     """Blocks, slots and positions of the `new` tokens of requests that hold
     `lens`; new block ids go into `table` [requests, width].  `tokens` is the
-    step's row count (rows no request covers get slot -1).  Nothing is read
+    step's row count (rows no request covers get slot -1).  A free_count past
+    free_list's end counts as its length.  Nothing is read
     back: plan.counts[3] tells on the device how many requests were refused.
     With `out` (an earlier plan of the same sizes) nothing is allocated; lens,
     new and free_count must then not be that plan's own tensors."""

@@ -58,3 +58,14 @@ def test_plan_refuses_its_own_outputs_as_inputs(qg, cuda):
             call(*args, p)
     other = call(i32(lens), i32(new), i32([len(free)]), None)
     call(p.lens, i32(new), p.counts[:1], other)  # another plan's are inputs like any
+
+
+@pytest.mark.parametrize("listed", [0, 1, 5, 60])
+def test_plan_takes_no_block_past_the_free_list(qg, cuda, listed):
+    """A free_count above the list's length counts as that length."""
+    lens, new, table, free = make_step(41, 40, 70, 50, 16, spare=listed)
+    want = R.plan(lens, new, table, free, listed, 16, sum(new))
+    for count in (listed + 1, listed + 1000, TOP):
+        tab = torch.tensor(table, dtype=torch.int32, device="cuda")
+        p = qg.kv_plan(i32(lens), i32(new), tab, i32(free), i32([count]), 16, sum(new))
+        assert tab.tolist() == want[0] and p.slots.tolist() == want[3] and p.counts.tolist() == want[6]

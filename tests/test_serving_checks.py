@@ -37,3 +37,11 @@ def test_plan_refuses_outputs_on_inputs_and_on_each_other(qg, out):
             assert plan(qg, **{out: at[other] + shift}) == qg.ERR_INVALID_ARG, (other, shift)
             assert b"overlap" in qg.lib().qgemm_last_error_message(), (other, shift)
     assert plan(qg, **{out: 4 * M}) == qg.ERR_INVALID_ARG  # the free list, whose first entry may be read
+
+
+def test_plan_bounded_refuses_a_negative_length(qg):
+    args = [64, 2, M, 2 * M, 3 * M, 4, 4 * M, -1, 5 * M, 5, 6 * M, 7 * M, 8 * M, 9 * M, 10 * M, 11 * M, None]
+    assert qg.lib().qgemm_kv_plan_bounded(*args) == qg.ERR_INVALID_ARG
+    args[7], args[10] = 8, 4 * M + 28  # lens_out on the list's last entry
+    assert qg.lib().qgemm_kv_plan_bounded(*args) == qg.ERR_INVALID_ARG
+    assert b"overlap" in qg.lib().qgemm_last_error_message()
