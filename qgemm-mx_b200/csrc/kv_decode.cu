@@ -162,7 +162,7 @@ k_kv_decode(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
         win_end = page + 32;
         const int p = page + lane;
         win_id = ((long long)p << lg) < ps.len ? a.table[(size_t)ps.r * a.width + p] : -1;
-        if (win_id >= a.blocks) win_id = -1;
+        if (win_id < 0 || win_id >= a.blocks) win_id = -1;  // before it is multiplied
       }
       const int id = __shfl_sync(0xFFFFFFFFu, win_id, page - win);
       if (lane == 0) {

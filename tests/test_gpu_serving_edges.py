@@ -3,6 +3,7 @@ and counts near 2^31, block ids outside the pool, calls on other streams."""
 import pytest
 import serving_ref as R
 import torch
+from test_gpu_kv_attention import make
 from test_gpu_kv_cache import check_plan, i32, make_step
 
 pytestmark = pytest.mark.gpu
@@ -69,3 +70,44 @@ def test_plan_takes_no_block_past_the_free_list(qg, cuda, listed):
         tab = torch.tensor(table, dtype=torch.int32, device="cuda")
         p = qg.kv_plan(i32(lens), i32(new), tab, i32(free), i32([count]), 16, sum(new))
         assert tab.tolist() == want[0] and p.slots.tolist() == want[3] and p.counts.tolist() == want[6]
+
+
+# ---- attention ----------------------------------------------------------------------
+
+def check_outside(qg, kv, lens, new, block, heads, group, d, seed, ids, fill=127):
+    """kv_attention with some table entries outside the pool against a cache in which they
+    name a block of zeros, with the bounds of test_gpu_kv_attention.py.  `fill`: the scale
+    bytes of the pool's first block, which no request then uses."""
+    c, q, starts, n, table = make(qg, kv, lens, [new] * len(lens), block, heads, group, d, seed)
+    blocks = c.k.shape[0]
+    c.k_scales[0] = c.v_scales[0] = fill
+    table = torch.where(table == 0, 1, table)
+    shadow = [torch.cat([x, torch.full_like(x[:1], y)]) for x, y in ((c.k, 0), (c.v, 0), (c.k_scales, 127), (c.v_scales, 127))]
+    mapped, place = table.clone(), 0
+    for r, length in enumerate(lens):
+        for p in range(-(-length // block)):
+            if (p + r) % 3 == 0:
+                table[r, p] = ids[place % len(ids)] if ids[place % len(ids)] != "blocks" else blocks
+                mapped[r, p] = blocks
+                place += 1
+    assert place >= len(ids)
+    ws = qg.make_kv_workspace(c, q.shape[1], len(lens), q.shape[0], new)
+    out, lse = qg.kv_attention(c, q, starts, n, table, new, lse=True, workspace=ws)
+    want, wlse, mass, logit, floor = R.attention(kv, *shadow, q, starts, n, mapped, d ** -0.5)
+    most = max(lens)
+    tol = want.abs() * 2.0 ** -8 + mass * (2.0 ** -11 + 2.0 ** -20 + (2 * d * logit[..., None] + most) * 2.0 ** -23) + \
+        floor * 2.0 ** -35
+    assert ((out.double() - want).abs() <= tol).all()
+    assert ((lse.double() - wlse).abs() <= (d * logit + most + 64) * 2.0 ** -23 + wlse.abs() * 2.0 ** -22).all()
+
+
+OUTSIDE = [-1, -5, "blocks", TOP, -2 ** 31, -2 ** 30 - 1, -2 ** 30, -715827883, 2 ** 30]
+WIDTHS = [(128, 1), (128, 2), (128, 150), (64, 1), (64, 2), (64, 150)]  # head_dim, rows a request brings
+
+
+@pytest.mark.parametrize("kv", [0, 1])
+@pytest.mark.parametrize("heads", [2, 3])
+@pytest.mark.parametrize("d,new", WIDTHS)
+def test_block_ids_far_outside_the_pool_read_as_zeros(qg, cuda, kv, heads, d, new):
+    """Ids whose product with the heads wraps 32 bits to a place far behind the pool."""
+    check_outside(qg, kv, [600, 170, 333], new, 16, heads, 4, d, 101, OUTSIDE)
