@@ -148,6 +148,7 @@ k_kv_decode(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
     KvSeg ps = s;
     ps.tile = 0; ps.tile_end = 0;
     int win = 0, win_end = 0, win_id = -1;  // 32 block ids from `win` on, one per lane
+    uint32_t outside = 0;  // stages whose block is outside the pool, one bit each
     const int lg = a.block_log2;
     auto issue = [&](int stage) {
       while (ps.tile >= ps.tile_end) {
@@ -165,6 +166,7 @@ k_kv_decode(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
         if (win_id < 0 || win_id >= a.blocks) win_id = -1;  // before it is multiplied
       }
       const int id = __shfl_sync(0xFFFFFFFFu, win_id, page - win);
+      outside = (outside & ~(1u << stage)) | ((uint32_t)(id < 0) << stage);
       if (lane == 0) {
         const uint32_t bar = su32(&s_bars[warp * ST + stage]), dst = ring + stage * Cfg::kStage;
         const int cell = id * a.heads + ps.h;
@@ -282,7 +284,7 @@ k_kv_decode(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
         ok = __all_sync(0xFFFFFFFFu, mbar_wait_flag(su32(&s_bars[warp * ST + stage]), parity, &g_kv_decode_fault));
         if (!ok) break;
         const uint32_t sb = ring + stage * Cfg::kStage;
-        const uint32_t mt = mt_next;
+        const uint32_t mt = outside >> stage & 1u ? 0x7F7Fu : mt_next;  // 2^0 beside the zeros outside the pool
         float sc[NT][2][4];
 #pragma unroll
         for (int j = 0; j < KJ; ++j) {

@@ -111,3 +111,11 @@ WIDTHS = [(128, 1), (128, 2), (128, 150), (64, 1), (64, 2), (64, 150)]  # head_d
 def test_block_ids_far_outside_the_pool_read_as_zeros(qg, cuda, kv, heads, d, new):
     """Ids whose product with the heads wraps 32 bits to a place far behind the pool."""
     check_outside(qg, kv, [600, 170, 333], new, 16, heads, 4, d, 101, OUTSIDE)
+
+
+@pytest.mark.parametrize("kv", [0, 1])
+@pytest.mark.parametrize("fill", [0, 1, 60, 200, 254, 255])
+@pytest.mark.parametrize("d,new", WIDTHS)
+def test_block_ids_outside_the_pool_take_no_blocks_scale(qg, cuda, kv, fill, d, new):
+    """Zeros whatever the scale bytes of the pool's first block are."""
+    check_outside(qg, kv, [600, 170, 333], new, 32, 2, 4, d, 102, [-1, "blocks", -5, TOP], fill)
