@@ -111,10 +111,13 @@ def kv_attention_workspace(cache: KVCache, q_heads: int, requests: int, tokens: 
 
 def make_kv_workspace(cache: KVCache, q_heads: int, requests: int, tokens: int, max_new: int,
                       stream=None) -> torch.Tensor:
-    """Zeroed workspace for kv_attention calls of up to these sizes."""
-    n = max(kv_attention_workspace(cache, q_heads, requests, tokens, max_new), 256)
-    ws = torch.empty(n, dtype=torch.uint8, device=cache.k.device)
-    _check(_lib.qgemm_workspace_init(_ptr(ws), n, _stream(stream)), "workspace_init")
+    """Zeroed workspace for kv_attention calls of up to these sizes on `stream`
+    (the current one), whose memory it is: allocated, cleared and, once dropped,
+    given out again in that stream's order."""
+    with torch.cuda.device(cache.k.device) if stream is None else torch.cuda.stream(stream):
+        n = max(kv_attention_workspace(cache, q_heads, requests, tokens, max_new), 256)
+        ws = torch.empty(n, dtype=torch.uint8, device=cache.k.device)
+        _check(_lib.qgemm_workspace_init(_ptr(ws), n, _stream()), "workspace_init")
     return ws
 
 

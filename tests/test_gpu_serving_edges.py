@@ -119,3 +119,26 @@ def test_block_ids_far_outside_the_pool_read_as_zeros(qg, cuda, kv, heads, d, ne
 def test_block_ids_outside_the_pool_take_no_blocks_scale(qg, cuda, kv, fill, d, new):
     """Zeros whatever the scale bytes of the pool's first block are."""
     check_outside(qg, kv, [600, 170, 333], new, 32, 2, 4, d, 102, [-1, "blocks", -5, TOP], fill)
+
+
+@pytest.mark.parametrize("new", [1, 100])
+def test_a_workspace_belongs_to_the_calls_stream(qg, cuda, new):
+    """What a call on another stream takes for itself is that stream's memory: the
+    current stream does not get it when the call has returned."""
+    c, q, starts, lens, table = make(qg, 0, [300, 1100, 64 + new], [new] * 3, 64, 2, 8, 128, 111)
+    want = qg.kv_attention(c, q, starts, lens, table, new)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    ws = qg.make_kv_workspace(c, q.shape[1], 3, q.shape[0], new, stream=s)
+    at, size = ws.data_ptr(), ws.numel()
+    del ws
+    again = torch.empty(size, dtype=torch.uint8, device="cuda")
+    assert again.data_ptr() != at
+    with torch.cuda.stream(s):
+        assert torch.empty(size, dtype=torch.uint8, device="cuda").data_ptr() == at
+    for _ in range(20):
+        out = qg.kv_attention(c, q, starts, lens, table, new, stream=s)
+        taken = [torch.full((size,), 255, dtype=torch.uint8, device="cuda") for _ in range(3)]
+        s.synchronize()
+        assert torch.equal(out, want)
+        del taken
