@@ -16,6 +16,8 @@ The directory name contains a hyphen, so import it with
 from __future__ import annotations
 
 import ctypes as C
+import functools
+import inspect
 import os
 from dataclasses import dataclass
 
@@ -127,6 +129,24 @@ def _stream(stream=None):
     return C.c_void_p(s.cuda_stream)
 
 
+def _on_stream(f):
+    """For functions whose last parameter is `stream`: with one given, what the
+    function allocates or copies for itself is ordered with its kernels (torch's
+    allocator and copies go by the current stream)."""
+    place = len(inspect.signature(f).parameters) - 1
+
+    @functools.wraps(f)
+    def call(*args, **kw):
+        stream = args[place] if len(args) > place else kw.get("stream")
+        if stream is None:
+            return f(*args, **kw)
+        if not isinstance(stream, torch.cuda.Stream):
+            stream = torch.cuda.ExternalStream(stream.cuda_stream)
+        with torch.cuda.stream(stream):
+            return f(*args, **kw)
+    return call
+
+
 def _ptr(t: torch.Tensor | None):
     return C.c_void_p(0 if t is None else t.data_ptr())
 
@@ -202,6 +222,7 @@ def _as_f32_2d(W: torch.Tensor) -> torch.Tensor:
     return W.contiguous()
 
 
+@_on_stream
 def pack_mxfp4(W: torch.Tensor, stream=None) -> Packed:
     """pack.hpp:465-497 on the device (bit-exact)."""
     W = _as_f32_2d(W)
@@ -213,6 +234,7 @@ def pack_mxfp4(W: torch.Tensor, stream=None) -> Packed:
     return Packed(MXFP4, N, K, data, scales)
 
 
+@_on_stream
 def nvfp4_tensor_scale(W: torch.Tensor, stream=None) -> float:
     """max|W| / (448*6) computed on the device; returns the host float."""
     W = _as_f32_2d(W) if W.dim() == 2 else W.contiguous()
@@ -221,6 +243,7 @@ def nvfp4_tensor_scale(W: torch.Tensor, stream=None) -> float:
     return float(out.item())
 
 
+@_on_stream
 def pack_nvfp4(W: torch.Tensor, tensor_scale: float | None = None, stream=None) -> Packed:
     """pack.hpp:502-542 on the device (bit-exact).  tensor_scale defaults to
     max|W|/(448*6)."""
@@ -236,6 +259,7 @@ def pack_nvfp4(W: torch.Tensor, tensor_scale: float | None = None, stream=None) 
     return Packed(NVFP4, N, K, data, scales, float(tensor_scale))
 
 
+@_on_stream
 def pack_int4(W: torch.Tensor, group: int = 128, stream=None) -> Packed:
     """pack.hpp:424-462 on the device (bit-exact)."""
     W = _as_f32_2d(W)
@@ -250,6 +274,7 @@ def pack_int4(W: torch.Tensor, group: int = 128, stream=None) -> Packed:
     return Packed(fmt, N, K, data, scales)
 
 
+@_on_stream
 def pack(fmt: int, W: torch.Tensor, stream=None) -> Packed:
     if fmt == MXFP4:
         return pack_mxfp4(W, stream)
@@ -273,6 +298,7 @@ def from_host(fmt: int, N: int, K: int, data, scales, tensor_scale: float = 1.0,
     return Packed(fmt, N, K, d, s, float(tensor_scale))
 
 
+@_on_stream
 def dequant(p: Packed, stream=None) -> torch.Tensor:
     """pack.hpp:548-585 on the device (bit-exact FP32 [N, K])."""
     out = torch.empty((p.N, p.K), dtype=torch.float32, device=p.data.device)
@@ -284,6 +310,7 @@ def dequant(p: Packed, stream=None) -> torch.Tensor:
 dequant_mxfp4 = dequant_nvfp4 = dequant_int4 = dequant
 
 
+@_on_stream
 def pack_codes(fmt: int, codes: torch.Tensor, scales: torch.Tensor, N: int, K: int,
                tensor_scale: float = 1.0, stream=None) -> Packed:
     """Already-quantised codes to the canonical layout (pack.hpp:611-665):
@@ -300,6 +327,7 @@ def pack_codes(fmt: int, codes: torch.Tensor, scales: torch.Tensor, N: int, K: i
     return Packed(fmt, N, K, data, sc, tensor_scale if fmt == NVFP4 else 1.0)
 
 
+@_on_stream
 def unpack_codes(p: Packed, stream=None) -> torch.Tensor:
     """The packed codes back (pack.hpp:667-682): uint8 E2M1 codes, or int32
     INT4 values, [N*K]."""
@@ -332,6 +360,7 @@ def repack(p: Packed, layout: int = SCALE_CHECKED, stream=None) -> Packed:
     return Packed(p.format, p.N, p.K, p.data, p.scales, p.tensor_scale, layout)
 
 
+@_on_stream
 def unpack(p: Packed, stream=None) -> Packed:
     """The canonical bytes of p (any layout), in new buffers."""
     data, sc = _alloc_packed(p.format, p.N, p.K, p.data.device)
@@ -340,6 +369,7 @@ def unpack(p: Packed, stream=None) -> Packed:
     return Packed(p.format, p.N, p.K, data, sc, p.tensor_scale, CANONICAL)
 
 
+@_on_stream
 def codec_encode(kind: str, x: torch.Tensor, stream=None) -> torch.Tensor:
     """Device scalar encoders (pack.hpp): 'e2m1' | 'e8m0' | 'e4m3' | 'fp16'."""
     k = {"e2m1": 0, "e8m0": 1, "e4m3": 2, "fp16": 3}[kind]
@@ -369,6 +399,7 @@ def launch_count(p: Packed, M: int) -> tuple[int, str]:
     return n, KERNEL_NAMES[k.value]
 
 
+@_on_stream
 def make_workspace(p: Packed, M: int, stream=None) -> torch.Tensor:
     n = max(workspace_size(p, M), 256)
     ws = torch.empty(n, dtype=torch.uint8, device=p.data.device)
@@ -376,6 +407,7 @@ def make_workspace(p: Packed, M: int, stream=None) -> torch.Tensor:
     return ws
 
 
+@_on_stream
 def gemm_w4a16(p: Packed, X: torch.Tensor, out: torch.Tensor | None = None,
                workspace: torch.Tensor | None = None, out_f32: bool = False, stream=None) -> torch.Tensor:
     """Y[M,N] = X[M,K] . W[N,K]^T with X bf16; Y bf16 (or fp32 if out_f32)."""
@@ -407,6 +439,7 @@ def grouped_workspace_size(experts: list[Packed], max_m: int) -> int:
     return _lib.qgemm_grouped_workspace_size(_expert_descs(experts), len(experts), max_m)
 
 
+@_on_stream
 def make_grouped_workspace(experts: list[Packed], max_m: int, stream=None) -> torch.Tensor:
     n = max(grouped_workspace_size(experts, max_m), 256)
     ws = torch.empty(n, dtype=torch.uint8, device=experts[0].data.device)
@@ -414,6 +447,7 @@ def make_grouped_workspace(experts: list[Packed], max_m: int, stream=None) -> to
     return ws
 
 
+@_on_stream
 def grouped_gemm_w4a16(experts: list[Packed], X: torch.Tensor, counts, offsets=None,
                        out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
                        stream=None) -> torch.Tensor:
@@ -450,6 +484,7 @@ def grouped_gemm_w4a16(experts: list[Packed], X: torch.Tensor, counts, offsets=N
     return out
 
 
+@_on_stream
 def cublas_bf16_gemm(W: torch.Tensor, X: torch.Tensor, out: torch.Tensor | None = None, stream=None):
     """Dense cuBLAS BF16 baseline of the same shape (bench_cublas.cu:144-151)."""
     N, K = W.shape
@@ -460,6 +495,7 @@ def cublas_bf16_gemm(W: torch.Tensor, X: torch.Tensor, out: torch.Tensor | None 
     return out
 
 
+@_on_stream
 def cublaslt_fp8_gemm(W8: torch.Tensor, X8: torch.Tensor, scale_w: torch.Tensor, scale_x: torch.Tensor,
                       out: torch.Tensor | None = None, workspace: torch.Tensor | None = None, stream=None):
     """cuBLASLt FP8 dense baseline: Y[M,N] bf16 = (X8.scale_x) . (W8.scale_w)^T.
@@ -505,6 +541,7 @@ def tp_sync_bytes(world: int) -> int:
     return _lib.qgemm_tp_sync_bytes(world)
 
 
+@_on_stream
 def make_tp_workspace(p: Packed, M: int, stream=None) -> torch.Tensor:
     """Zeroed workspace for tp_gemm of this rank's shard p."""
     d = p.desc()
