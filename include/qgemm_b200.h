@@ -364,7 +364,7 @@ qgemm_status_t qgemm_kv_append(const qgemm_kv_cache_t* cache, const uint16_t* k,
  * table_width * block are cut to it; tokens of a block id outside the pool
  * read as zeros.  Rows beyond starts[requests] are left as they are.  head_dim
  * values of q lie together, q is 16-byte aligned, its strides multiples of 8.
- * workspace: qgemm_kv_attention_workspace() bytes, zeroed once
+ * workspace: qgemm_kv_attention_workspace() bytes, 16-byte aligned, zeroed once
  * (qgemm_workspace_init); every call returns its tickets to zero.            */
 size_t qgemm_kv_attention_workspace(const qgemm_kv_cache_t* cache, int32_t q_heads,
                                     int32_t requests, int32_t tokens, int32_t max_new);

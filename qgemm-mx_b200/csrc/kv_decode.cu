@@ -698,6 +698,8 @@ qgemm_status_t qgemm_kv_attention(const qgemm_kv_cache_t* c, const uint16_t* q, 
     return fail(QGEMM_ERR_INVALID_ARG, "kv_attention: q and out must be 16-byte aligned");
   if (q_stride % 8 || q_head_stride % 8)
     return fail(QGEMM_ERR_INVALID_ARG, "kv_attention: q's strides must be multiples of 8");
+  if (reinterpret_cast<uintptr_t>(workspace) & 15u)
+    return fail(QGEMM_ERR_WORKSPACE, "kv_attention: workspace must be 16-byte aligned");
   DevProps dp;
   qgemm_status_t st = device_props(&dp);
   if (st != QGEMM_OK) return st;

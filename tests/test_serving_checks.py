@@ -1,7 +1,10 @@
 """Refusals of the serving operators that are decided on the host (no GPU needed), beside
 those of test_serving_abi.py."""
 
+import ctypes as C
+
 import pytest
+from test_serving_abi import cache
 
 M = 1 << 20  # plausible, aligned addresses that are never read, M apart
 
@@ -45,3 +48,11 @@ def test_plan_bounded_refuses_a_negative_length(qg):
     args[7], args[10] = 8, 4 * M + 28  # lens_out on the list's last entry
     assert qg.lib().qgemm_kv_plan_bounded(*args) == qg.ERR_INVALID_ARG
     assert b"overlap" in qg.lib().qgemm_last_error_message()
+
+
+@pytest.mark.parametrize("off", [1, 4, 8, 15])
+def test_attention_refuses_a_workspace_off_16_bytes(qg, off):
+    """Tickets and vectors of four floats lie in it."""
+    st = qg.lib().qgemm_kv_attention(C.byref(cache()), M, 8192, 128, 64, 2, 2 * M, 3 * M, 4 * M, 4, 3, 2, 0.1, 0, 1, 5 * M,
+                                     None, 6 * M + off, 1 << 30, None)
+    assert st == qg.ERR_WORKSPACE and b"16-byte" in qg.lib().qgemm_last_error_message()
