@@ -47,8 +47,10 @@ int32_t fits(int64_t v, const char* where) {
   if (v > INT32_MAX) refuse(where, "a size exceeds 2^31 - 1");
   return (int32_t)v;
 }
-bool ints(const Tensor& t, int64_t dims = 1) {
-  return t.scalar_type() == at::kInt && t.dim() == dims && t.is_cuda() && t.is_contiguous();
+// On the GPU that the call goes by.
+bool on(const Tensor& t, c10::DeviceIndex device) { return t.is_cuda() && t.get_device() == device; }
+bool ints(const Tensor& t, c10::DeviceIndex device, int64_t dims = 1) {
+  return t.scalar_type() == at::kInt && t.dim() == dims && on(t, device) && t.is_contiguous();
 }
 template <typename P = int32_t>
 P* ptr(const Tensor& t) { return static_cast<P*>(t.data_ptr()); }
@@ -123,12 +125,19 @@ bool count_is(Py_ssize_t n, Py_ssize_t want, const char* where) {
   PyErr_Format(PyExc_TypeError, "%s: %zd arguments expected", where, want);
   return false;
 }
-const qgemm_kv_cache_t* cache_of(PyObject* o, const char* where) {
-  if (!PyBytes_Check(o) || PyBytes_GET_SIZE(o) != (Py_ssize_t)sizeof(qgemm_kv_cache_t)) refuse(where, "not a KVCache");
-  return reinterpret_cast<const qgemm_kv_cache_t*>(PyBytes_AS_STRING(o));
+// A KVCache's description: the C-ABI's, and the GPU it lies on (-1: none).
+struct Cache {
+  qgemm_kv_cache_t c;
+  int64_t device;
+};
+const Cache* cache_of(PyObject* o, const char* where) {
+  if (!PyBytes_Check(o) || PyBytes_GET_SIZE(o) != (Py_ssize_t)sizeof(Cache)) refuse(where, "not a KVCache");
+  const Cache* c = reinterpret_cast<const Cache*>(PyBytes_AS_STRING(o));
+  if (c->device < 0) refuse(where, "the cache must be on a GPU");
+  return c;
 }
 
-// kv_cache(type, k, v, k_scales, v_scales) -> bytes of a qgemm_kv_cache_t
+// kv_cache(type, k, v, k_scales, v_scales) -> bytes of a Cache
 PyObject* kv_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!count_is(n, 5, "KVCache")) return nullptr;
   return guarded([&]() -> PyObject* {
@@ -144,13 +153,15 @@ PyObject* kv_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (t->dim() != 2 || t->scalar_type() != at::kByte || !t->is_contiguous() || t->size(0) != k.size(0) ||
           t->size(1) != k.size(1) || t->device() != k.device())
         refuse("KVCache", scales);
-    qgemm_kv_cache_t c;
-    std::memset(&c, 0, sizeof(c));
+    Cache whole;
+    std::memset(&whole, 0, sizeof(whole));
+    whole.device = k.is_cuda() ? k.get_device() : -1;
+    qgemm_kv_cache_t& c = whole.c;
     c.type = small(a[0], "KVCache");
     c.block = fits(k.size(2), "KVCache"); c.heads = fits(k.size(1), "KVCache"); c.head_dim = fits(k.size(3), "KVCache");
     c.blocks = k.size(0);
     c.k = ptr<uint8_t>(k); c.v = ptr<uint8_t>(v); c.k_scales = ptr<uint8_t>(ks); c.v_scales = ptr<uint8_t>(vs);
-    return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(&c), sizeof(c));
+    return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(&whole), sizeof(whole));
   });
 }
 
@@ -161,10 +172,12 @@ PyObject* kv_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!count_is(n, 9, W)) return nullptr;
   return guarded([&]() -> PyObject* {
     const char* what =
-        "lens, new, table [requests, width], free_list and free_count must be contiguous int32 CUDA tensors";
+        "lens, new, table [requests, width], free_list and free_count must be contiguous int32 CUDA tensors on one GPU";
     const Tensor &lens = tensor(a[0], W, what), &news = tensor(a[1], W, what), &table = tensor(a[2], W, what);
     const Tensor &list = tensor(a[3], W, what), &count = tensor(a[4], W, what);
-    if (!ints(lens) || !ints(news) || !ints(table, 2) || !ints(list) || !ints(count)) refuse(W, what);
+    const auto gpu = lens.is_cuda() ? lens.get_device() : -1;
+    if (!ints(lens, gpu) || !ints(news, gpu) || !ints(table, gpu, 2) || !ints(list, gpu) || !ints(count, gpu))
+      refuse(W, what);
     const int32_t requests = fits(table.size(0), W), width = fits(table.size(1), W);
     if (lens.numel() != requests || news.numel() != requests || count.numel() != 1)
       refuse(W, "new, table and free_count must have one entry per request, row per request, and one element");
@@ -178,9 +191,9 @@ PyObject* kv_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (!PyTuple_Check(a[7]) || PyTuple_GET_SIZE(a[7]) != 6) refuse(W, "out must be a KVPlan");
       for (int i = 0; i < 6; ++i) {
         o[i] = tensor(PyTuple_GET_ITEM(a[7], i), W, "out must hold tensors");
-        if (o[i].numel() != sizes[i] || o[i].scalar_type() != (i == 2 ? at::kLong : at::kInt) || !o[i].is_cuda() ||
+        if (o[i].numel() != sizes[i] || o[i].scalar_type() != (i == 2 ? at::kLong : at::kInt) || !on(o[i], gpu) ||
             !o[i].is_contiguous())
-          refuse(W, "out was made for other sizes");
+          refuse(W, "out was made for other sizes or another GPU");
       }
     } else {
       make_together(o, sizes, {at::kInt, at::kInt, at::kLong, at::kInt, at::kInt, at::kInt}, lens);
@@ -193,8 +206,9 @@ PyObject* kv_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // bf16 [tokens, heads, head_dim] rows with any spacing of tokens and heads.
-void check_rows(const Tensor& t, int64_t head_dim, const char* where, const char* what) {
-  if (t.scalar_type() != at::kBFloat16 || t.dim() != 3 || !t.is_cuda() || t.size(2) != head_dim) refuse(where, what);
+void check_rows(const Tensor& t, const Cache* c, const char* where, const char* what) {
+  if (t.scalar_type() != at::kBFloat16 || t.dim() != 3 || !on(t, c->device) || t.size(2) != c->c.head_dim)
+    refuse(where, what);
   if (t.stride(2) != 1 && t.numel()) refuse(where, "the head_dim values of a row must lie together");
 }
 
@@ -203,16 +217,18 @@ PyObject* kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   constexpr const char* W = "kv_append";
   if (!count_is(n, 6, W)) return nullptr;
   return guarded([&]() -> PyObject* {
-    const qgemm_kv_cache_t* c = cache_of(a[0], W);
-    const char* what = "k and v must be bf16 [tokens, heads, head_dim] of the cache on the GPU";
-    const char* index = "slots (int64) and runs (int32, with an end mark) must be contiguous CUDA tensors, one slot a token";
+    const Cache* cache = cache_of(a[0], W);
+    const qgemm_kv_cache_t* c = &cache->c;
+    const char* what = "k and v must be bf16 [tokens, heads, head_dim] of the cache, on its GPU";
+    const char* index =
+        "slots (int64) and runs (int32, with an end mark) must be contiguous on the cache's GPU, one slot a token";
     const Tensor &k = tensor(a[1], W, what), &v = tensor(a[2], W, what);
     const Tensor &slots = tensor(a[3], W, index), &runs = tensor(a[4], W, index);
-    check_rows(k, c->head_dim, W, what);
-    check_rows(v, c->head_dim, W, what);
+    check_rows(k, cache, W, what);
+    check_rows(v, cache, W, what);
     if (k.size(1) != c->heads || v.size(1) != c->heads || v.size(0) != k.size(0)) refuse(W, what);
-    if (slots.scalar_type() != at::kLong || !slots.is_cuda() || slots.numel() != k.size(0) || !slots.is_contiguous() ||
-        !ints(runs) || runs.numel() < 1)
+    if (slots.scalar_type() != at::kLong || !on(slots, cache->device) || slots.numel() != k.size(0) ||
+        !slots.is_contiguous() || !ints(runs, cache->device) || runs.numel() < 1)
       refuse(W, index);
     const Place place(a[5], k);
     const int st = qgemm_kv_append(c, ptr<uint16_t>(k), ptr<uint16_t>(v), k.stride(0), k.stride(1), v.stride(0),
@@ -228,13 +244,15 @@ PyObject* kv_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   constexpr const char* W = "kv_attention";
   if (!count_is(n, 13, W)) return nullptr;
   return guarded([&]() -> PyObject* {
-    const qgemm_kv_cache_t* c = cache_of(a[0], W);
-    const char* rows = "q must be bf16 [tokens, heads, head_dim] with the cache's head_dim on the GPU";
-    const char* index = "starts, lens and table [requests, width] must be contiguous int32 CUDA tensors";
+    const Cache* cache = cache_of(a[0], W);
+    const qgemm_kv_cache_t* c = &cache->c;
+    const auto gpu = cache->device;
+    const char* rows = "q must be bf16 [tokens, heads, head_dim] with the cache's head_dim, on its GPU";
+    const char* index = "starts, lens and table [requests, width] must be contiguous int32 on the cache's GPU";
     const Tensor& q = tensor(a[1], W, rows);
     const Tensor &starts = tensor(a[2], W, index), &lens = tensor(a[3], W, index), &table = tensor(a[4], W, index);
-    check_rows(q, c->head_dim, W, rows);
-    if (!ints(starts) || !ints(lens) || !ints(table, 2)) refuse(W, index);
+    check_rows(q, cache, W, rows);
+    if (!ints(starts, gpu) || !ints(lens, gpu) || !ints(table, gpu, 2)) refuse(W, index);
     if (starts.numel() != lens.numel() + 1 || table.size(0) != lens.numel())
       refuse(W, "starts needs requests + 1 entries and table a row per request");
     const double scale = PyFloat_AsDouble(a[6]);
@@ -245,14 +263,14 @@ PyObject* kv_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Tensor out, z;
     if (given(a[10])) {
       out = tensor(a[10], W, "out must be a tensor");
-      if (out.sizes() != q.sizes() || out.scalar_type() != at::kBFloat16 || !out.is_cuda() || !out.is_contiguous())
-        refuse(W, "out must be contiguous bf16 of q's shape");
+      if (out.sizes() != q.sizes() || out.scalar_type() != at::kBFloat16 || !on(out, gpu) || !out.is_contiguous())
+        refuse(W, "out must be contiguous bf16 of q's shape on its GPU");
     } else {
       out = make(q.sizes(), at::kBFloat16, q);
     }
     if (lse) z = make({q.size(0), q.size(1)}, at::kFloat, q);
     const Tensor& ws = tensor(a[11], W, "workspace must be a tensor");
-    if (!ws.is_cuda() || !ws.is_contiguous()) refuse(W, "workspace must be a contiguous CUDA tensor");
+    if (!on(ws, gpu) || !ws.is_contiguous()) refuse(W, "workspace must be contiguous on the cache's GPU");
     const int st = qgemm_kv_attention(
         c, ptr<uint16_t>(q), q.stride(0), q.stride(1), fits(q.size(1), W), fits(lens.numel(), W), ptr(starts), ptr(lens),
         ptr(table), fits(table.size(1), W), fits(q.size(0), W), small(a[5], W), (float)scale, small(a[7], W), causal,
@@ -268,14 +286,15 @@ PyObject* residual_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!count_is(n, 13, W)) return nullptr;
   return guarded([&]() -> PyObject* {
     const char* stream_rows = "residual must be contiguous bf16 or float32 [tokens, width] on the GPU";
-    const char* rows = "y and h must be contiguous bf16 [tokens, width]";
-    const char* weights = "post, pre and their biases must be contiguous bf16 [width]";
-    const char* gates = "gate must be bf16 [width] or [tokens, width]";
+    const char* rows = "y and h must be contiguous bf16 [tokens, width] on residual's GPU";
+    const char* weights = "post, pre and their biases must be contiguous bf16 [width] on residual's GPU";
+    const char* gates = "gate must be bf16 [width] or [tokens, width] on residual's GPU";
     const Tensor& r = tensor(a[1], W, stream_rows);
     const auto type = r.scalar_type();
     if (r.dim() != 2 || (type != at::kBFloat16 && type != at::kFloat) || !r.is_cuda() || !r.is_contiguous())
       refuse(W, stream_rows);
     const int64_t width = r.size(1);
+    const auto gpu = r.get_device();
     qgemm_residual_norm_t p;
     std::memset(&p, 0, sizeof(p));
     p.kind = small(a[8], W);
@@ -285,13 +304,13 @@ PyObject* residual_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     auto row = [&](PyObject* o) -> uint16_t* {
       if (!given(o)) return nullptr;
       const Tensor& t = tensor(o, W, rows);
-      if (t.scalar_type() != at::kBFloat16 || t.sizes() != r.sizes() || !t.is_cuda() || !t.is_contiguous()) refuse(W, rows);
+      if (t.scalar_type() != at::kBFloat16 || t.sizes() != r.sizes() || !on(t, gpu) || !t.is_contiguous()) refuse(W, rows);
       return ptr<uint16_t>(t);
     };
     auto weight = [&](PyObject* o) -> const uint16_t* {
       if (!given(o)) return nullptr;
       const Tensor& t = tensor(o, W, weights);
-      if (t.scalar_type() != at::kBFloat16 || t.dim() != 1 || t.numel() != width || !t.is_cuda() || !t.is_contiguous())
+      if (t.scalar_type() != at::kBFloat16 || t.dim() != 1 || t.numel() != width || !on(t, gpu) || !t.is_contiguous())
         refuse(W, weights);
       return ptr<uint16_t>(t);
     };
@@ -301,7 +320,7 @@ PyObject* residual_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (given(a[6])) {
       const Tensor& g = tensor(a[6], W, gates);
       const bool each = g.dim() == 2;
-      if (g.scalar_type() != at::kBFloat16 || !g.is_cuda() || (each ? g.sizes() != r.sizes() : g.dim() != 1 || g.numel() != width) ||
+      if (g.scalar_type() != at::kBFloat16 || !on(g, gpu) || (each ? g.sizes() != r.sizes() : g.dim() != 1 || g.numel() != width) ||
           (g.stride(-1) != 1 && width > 1))
         refuse(W, gates);
       p.gate = ptr<uint16_t>(g);
@@ -315,9 +334,9 @@ PyObject* residual_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!has_y) {
       out = r;
     } else if (given(a[10])) {
-      out = tensor(a[10], W, "residual_out must be like residual");
-      if (out.sizes() != r.sizes() || out.scalar_type() != type || !out.is_cuda() || !out.is_contiguous())
-        refuse(W, "residual_out must be like residual");
+      out = tensor(a[10], W, "residual_out must be like residual, on its GPU");
+      if (out.sizes() != r.sizes() || out.scalar_type() != type || !on(out, gpu) || !out.is_contiguous())
+        refuse(W, "residual_out must be like residual, on its GPU");
     } else {
       out = make(r.sizes(), type, r);
     }

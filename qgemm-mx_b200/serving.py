@@ -46,7 +46,7 @@ class KVCache:
     __slots__ = ("type", "k", "v", "k_scales", "v_scales", "_desc")
 
     def __init__(self, type: int, k: torch.Tensor, v: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor):
-        self._desc = _b.kv_cache(type, k, v, k_scales, v_scales)  # a qgemm_kv_cache_t
+        self._desc = _b.kv_cache(type, k, v, k_scales, v_scales)  # a qgemm_kv_cache_t, then its GPU
         self.type, self.k, self.v, self.k_scales, self.v_scales = type, k, v, k_scales, v_scales
 
     def values(self) -> tuple[torch.Tensor, torch.Tensor]:
@@ -114,6 +114,8 @@ def make_kv_workspace(cache: KVCache, q_heads: int, requests: int, tokens: int, 
     """Zeroed workspace for kv_attention calls of up to these sizes on `stream`
     (the current one), whose memory it is: allocated, cleared and, once dropped,
     given out again in that stream's order."""
+    if not cache.k.is_cuda:
+        raise ValueError("make_kv_workspace: the cache must be on a GPU")
     with torch.cuda.device(cache.k.device) if stream is None else torch.cuda.stream(stream):
         n = max(kv_attention_workspace(cache, q_heads, requests, tokens, max_new), 256)
         ws = torch.empty(n, dtype=torch.uint8, device=cache.k.device)

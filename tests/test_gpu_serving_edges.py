@@ -142,3 +142,48 @@ def test_a_workspace_belongs_to_the_calls_stream(qg, cuda, new):
         s.synchronize()
         assert torch.equal(out, want)
         del taken
+
+
+# ---- where tensors lie ---------------------------------------------------------------
+
+def each_on_the_host(args, kw):
+    """The call's arguments with one tensor at a time on the host."""
+    for i, t in enumerate(args):
+        if isinstance(t, torch.Tensor):
+            yield [*args[:i], t.cpu(), *args[i + 1:]], kw
+    for n, t in kw.items():
+        if isinstance(t, torch.Tensor):
+            yield args, {**kw, n: t.cpu()}
+
+
+def test_every_tensor_must_be_on_the_calls_gpu(qg, cuda):
+    c, q, starts, lens, table = make(qg, 0, [40, 20], [1, 1], 16, 2, 4, 64, 121)
+    ws = qg.make_kv_workspace(c, 8, 2, 2, 1)
+    k = torch.zeros((2, 2, 64), dtype=torch.bfloat16, device="cuda")
+    slots, runs = torch.tensor([0, 16], device="cuda"), i32([0, 1, 2])
+    y, w = torch.zeros((2, 64), dtype=torch.bfloat16, device="cuda"), torch.ones(64, dtype=torch.bfloat16, device="cuda")
+    calls = [
+        (qg.kv_plan, [lens, i32([1, 1]), table, i32([7, 8]), i32([2]), 16, 2], {}),
+        (qg.kv_append, [c, k, k.clone(), slots, runs], {}),
+        (qg.kv_attention, [c, q, starts, lens, table, 1], {"out": torch.empty_like(q, memory_format=torch.contiguous_format),
+                                                           "workspace": ws}),
+        (qg.residual_norm, [y, y.clone()], {"post": w, "pre": w, "post_bias": w, "pre_bias": w, "gate": w, "kind": "layer",
+                                            "residual_out": y.clone(), "h": y.clone()}),
+    ]
+    for f, args, kw in calls:
+        f(*args, **kw)
+        n = 0
+        for a, b in each_on_the_host(args, kw):
+            with pytest.raises(ValueError, match="GPU"):
+                f(*a, **b)
+            n += 1
+        assert n >= 4
+    plan = qg.kv_plan(*calls[0][1])
+    plan.positions = plan.positions.cpu()
+    with pytest.raises(ValueError, match="GPU"):
+        qg.kv_plan(*calls[0][1], out=plan)
+    host = qg.KVCache(qg.KV_E4M3, *(t.cpu() for t in (c.k, c.v, c.k_scales, c.v_scales)))
+    with pytest.raises(ValueError, match="the cache must be on a GPU"):
+        qg.kv_append(host, k, k, slots, runs)
+    with pytest.raises(ValueError, match="the cache must be on a GPU"):
+        qg.kv_attention(host, q, starts, lens, table, 1, workspace=ws)

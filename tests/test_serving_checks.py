@@ -4,6 +4,7 @@ those of test_serving_abi.py."""
 import ctypes as C
 
 import pytest
+import torch
 from test_serving_abi import cache
 
 M = 1 << 20  # plausible, aligned addresses that are never read, M apart
@@ -56,3 +57,17 @@ def test_attention_refuses_a_workspace_off_16_bytes(qg, off):
     st = qg.lib().qgemm_kv_attention(C.byref(cache()), M, 8192, 128, 64, 2, 2 * M, 3 * M, 4 * M, 4, 3, 2, 0.1, 0, 1, 5 * M,
                                      None, 6 * M + off, 1 << 30, None)
     assert st == qg.ERR_WORKSPACE and b"16-byte" in qg.lib().qgemm_last_error_message()
+
+
+def test_calls_refuse_a_host_cache(qg):
+    """A KVCache of host tensors is a description; no call takes it."""
+    k, s = torch.zeros((2, 1, 16, 64), dtype=torch.uint8), torch.zeros((2, 1), dtype=torch.uint8)
+    c = qg.KVCache(qg.KV_E4M3, k, k.clone(), s, s.clone())
+    x = torch.zeros((1, 1, 64), dtype=torch.bfloat16)
+    i = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="the cache must be on a GPU"):
+        qg.kv_append(c, x, x, torch.zeros(1, dtype=torch.int64), i)
+    with pytest.raises(ValueError, match="the cache must be on a GPU"):
+        qg.kv_attention(c, x, i, i[:1], i[None], 1)
+    with pytest.raises(ValueError, match="the cache must be on a GPU"):
+        qg.kv_attention(c, x, i, i[:1], i[None], 1, workspace=torch.zeros(4096, dtype=torch.uint8))
