@@ -42,12 +42,19 @@ class KVCache:
     """A pool of blocks on the device.  ``k`` and ``v`` hold 8-bit codes
     (uint8 storage) [blocks, heads, block, head_dim], ``k_scales`` and
     ``v_scales`` one E8M0 byte per (block, head), 2^(byte - 127).  ``type`` is
-    KV_E4M3 or KV_INT8."""
-    __slots__ = ("type", "k", "v", "k_scales", "v_scales", "_desc")
+    KV_E4M3 or KV_INT8.  The attributes cannot be set: the calls go by the
+    pointers taken here."""
+    __slots__ = ("_type", "_k", "_v", "_k_scales", "_v_scales", "_desc")
 
     def __init__(self, type: int, k: torch.Tensor, v: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor):
         self._desc = _b.kv_cache(type, k, v, k_scales, v_scales)  # a qgemm_kv_cache_t, then its GPU
-        self.type, self.k, self.v, self.k_scales, self.v_scales = type, k, v, k_scales, v_scales
+        self._type, self._k, self._v, self._k_scales, self._v_scales = type, k, v, k_scales, v_scales
+
+    type = property(lambda self: self._type)
+    k = property(lambda self: self._k)
+    v = property(lambda self: self._v)
+    k_scales = property(lambda self: self._k_scales)
+    v_scales = property(lambda self: self._v_scales)
 
     def values(self) -> tuple[torch.Tensor, torch.Tensor]:
         """(K, V) as float32 [blocks, heads, block, head_dim], for inspection."""
@@ -133,7 +140,7 @@ def kv_attention(cache: KVCache, q: torch.Tensor, starts: torch.Tensor, lens: to
     if workspace is None:
         workspace = make_kv_workspace(cache, q.shape[1], lens.numel(), q.shape[0], max_new, stream)
     st, out, z = _b.kv_attention(cache._desc, q, starts, lens, table, max_new,
-                                 cache.k.shape[3] ** -0.5 if scale is None else scale, window, causal, lse, out,
+                                 cache._k.shape[3] ** -0.5 if scale is None else scale, window, causal, lse, out,
                                  workspace, _handle(stream))
     if st:
         _check(st, "kv_attention")

@@ -71,3 +71,18 @@ def test_calls_refuse_a_host_cache(qg):
         qg.kv_attention(c, x, i, i[:1], i[None], 1)
     with pytest.raises(ValueError, match="the cache must be on a GPU"):
         qg.kv_attention(c, x, i, i[:1], i[None], 1, workspace=torch.zeros(4096, dtype=torch.uint8))
+
+
+def test_a_caches_tensors_cannot_be_exchanged(qg):
+    """The calls go by the pointers that the KVCache was made with, and its tensors keep
+    that memory alive."""
+    k, s = torch.zeros((2, 1, 16, 64), dtype=torch.uint8), torch.zeros((2, 1), dtype=torch.uint8)
+    c = qg.KVCache(qg.KV_E4M3, k, k.clone(), s, s.clone())
+    for name, value in (("k", k.clone()), ("v", k), ("k_scales", s), ("v_scales", s), ("type", qg.KV_INT8)):
+        with pytest.raises(AttributeError):
+            setattr(c, name, value)
+        with pytest.raises(AttributeError):
+            delattr(c, name)
+    assert c.k is k and c.k_scales is s and c.type == qg.KV_E4M3
+    c.k[0] = 5  # their contents can be changed
+    assert c.values()[0].shape == (2, 1, 16, 64)
