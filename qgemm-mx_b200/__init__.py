@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import importlib
 import inspect
 import os
 from dataclasses import dataclass
@@ -40,7 +41,7 @@ MXFP4, NVFP4, INT4_G128, INT4_G64, BF16, FP16, FP8_E4M3 = range(7)
 FORMAT_NAMES = {MXFP4: "mxfp4", NVFP4: "nvfp4", INT4_G128: "int4_g128", INT4_G64: "int4_g64",
                 BF16: "bf16", FP16: "fp16", FP8_E4M3: "fp8_e4m3"}
 
-_vp, _sz, _i32, _f32, _u16p = C.c_void_p, C.c_size_t, C.c_int32, C.c_float, C.c_void_p
+_vp, _sz, _i32, _i64, _f32, _u16p = C.c_void_p, C.c_size_t, C.c_int32, C.c_int64, C.c_float, C.c_void_p
 
 
 class _Weights(C.Structure):
@@ -98,6 +99,17 @@ _sig("qgemm_tp_status", _i32, [C.POINTER(_i32)])
 _sig("qgemm_ipc_handle", _i32, [C.c_void_p, C.POINTER(C.c_uint8), C.POINTER(_sz)])
 _sig("qgemm_ipc_open", _i32, [C.POINTER(C.c_uint8), C.POINTER(C.c_void_p)])
 _sig("qgemm_ipc_close", _i32, [C.c_void_p])
+_sig("qgemm_kv_max_runs", _i32, [_i32, _i32, _i32])
+_sig("qgemm_kv_plan", _i32, [_i32, _i32] + [_vp] * 3 + [_i32] + [_vp] * 2 + [_i32] + [_vp] * 7)
+_sig("qgemm_kv_plan_bounded", _i32, [_i32, _i32] + [_vp] * 3 + [_i32, _vp, _i32, _vp, _i32] +
+     [_vp] * 7)
+_sig("qgemm_kv_append", _i32, [_vp] * 3 + [_i64] * 4 + [_i32, _vp, _vp, _i32, _vp])
+_sig("qgemm_kv_attention_workspace", _sz, [_vp, _i32, _i32, _i32, _i32])
+_sig("qgemm_kv_attention", _i32, [_vp, _vp, _i64, _i64, _i32, _i32] + [_vp] * 3 +
+     [_i32, _i32, _i32, _f32, _i32, _i32, _vp, _vp, _vp, _sz, _vp])
+_sig("qgemm_residual_norm", _i32, [_vp, _vp])
+
+EXPORTED = [n for n in dir(_lib) if n.startswith("qgemm_")]
 
 
 class QGemmError(RuntimeError):
@@ -599,7 +611,22 @@ def device_info() -> tuple[int, int]:
 
 # ---- serving operators (serving.py) ---------------------------------------------
 
-from .serving import (KV_E4M3, KV_INT8, KVCache, KVPlan, kv_append, kv_attention,  # noqa: E402
-                      kv_attention_workspace, kv_plan, make_kv_cache, make_kv_workspace, residual_norm)
+# Imported on first use: they need _binding.so, which is built against one torch,
+# and the products do not.
+_SERVING = frozenset((
+    "KV_E4M3", "KV_INT8", "KVCache", "KVPlan", "kv_append", "kv_attention", "kv_attention_workspace", "kv_plan",
+    "make_kv_cache", "make_kv_workspace", "residual_norm"))
 
-EXPORTED = [n for n in dir(_lib) if n.startswith("qgemm_")]
+
+def __getattr__(name: str):
+    if name != "serving" and name not in _SERVING:
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    module = importlib.import_module(".serving", __name__)
+    if name == "serving":
+        return module
+    globals().update({n: getattr(module, n) for n in _SERVING})
+    return globals()[name]
+
+
+def __dir__():
+    return sorted({*globals(), *_SERVING, "serving"})

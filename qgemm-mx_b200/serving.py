@@ -3,35 +3,25 @@
 its gate and residual scale.  Thin layer over the C-ABI in
 ``include/qgemm_b200.h``, which states each operator's formula; everything
 runs on the caller's stream and can be captured into a CUDA graph when the
-workspace is passed in.
+workspace is passed in.  Imported when one of its names is first used; it needs
+``_binding.so`` (`make -C qgemm-mx_b200/csrc binding`) beside the library.
 """
 from __future__ import annotations
 
-import ctypes as C
 import os
 
 import torch
 
-from . import HERE, _check, _i32, _lib, _ptr, _sig, _stream, _sz
+from . import HERE, _check, _lib, _ptr, _stream
 
 if not os.path.exists(os.path.join(HERE, "_binding.so")):
-    raise ImportError(f"{HERE}/_binding.so is missing: build it with `make -C qgemm-mx_b200/csrc`")
+    raise ImportError(f"{HERE}/_binding.so is missing: build it with `make -C qgemm-mx_b200/csrc binding`")
 from . import _binding as _b  # noqa: E402  csrc/binding.cpp
 
 # cache types (qgemm_kv_type_t)
 KV_E4M3, KV_INT8 = 0, 1
 # norm kinds (qgemm_norm_kind_t)
 NORM_KINDS = {"rms": 0, "layer": 1}
-
-_sig("qgemm_kv_max_runs", _i32, [_i32, _i32, _i32])
-_sig("qgemm_kv_plan", _i32, [_i32, _i32] + [C.c_void_p] * 3 + [_i32] + [C.c_void_p] * 2 + [_i32] + [C.c_void_p] * 7)
-_sig("qgemm_kv_plan_bounded", _i32, [_i32, _i32] + [C.c_void_p] * 3 + [_i32, C.c_void_p, _i32, C.c_void_p, _i32] +
-     [C.c_void_p] * 7)
-_sig("qgemm_kv_append", _i32, [C.c_void_p] * 3 + [C.c_int64] * 4 + [_i32, C.c_void_p, C.c_void_p, _i32, C.c_void_p])
-_sig("qgemm_kv_attention_workspace", _sz, [C.c_void_p, _i32, _i32, _i32, _i32])
-_sig("qgemm_kv_attention", _i32, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, _i32, _i32] + [C.c_void_p] * 3 +
-     [_i32, _i32, _i32, C.c_float, _i32, _i32, C.c_void_p, C.c_void_p, C.c_void_p, _sz, C.c_void_p])
-_sig("qgemm_residual_norm", _i32, [C.c_void_p, C.c_void_p])
 
 
 def _handle(stream):
