@@ -120,7 +120,7 @@ struct KvLine {
   // prompt chunks of up to 512 tokens 126 us, 138 with 1, 129 with 5.
   static constexpr int kStart = TL == 4 ? 4 : 3;
   int h0, slope, groups;
-  __device__ __forceinline__ KvLine(const KvAttnArgs& a, const KvRequest& q) {
+  __host__ __device__ __forceinline__ KvLine(const KvAttnArgs& a, const KvRequest& q) {
     h0 = q.len;
     slope = 0;
     const int per = (RG + a.group - 1) / a.group;
@@ -177,11 +177,12 @@ __device__ __forceinline__ void kv_seg(const KvAttnArgs& a, const KvBatch<MOST>&
   s.tile_end = min(hi, lo + min(s.pair_end, v_end) - s.pair_v);
 }
 
-// Most places one request can take on the line (host).
+// Most places one request can take on the line (host): no group is given more tokens
+// than its request holds and one more, and the slope of all groups.
 inline long long kv_line_most(const KvAttnArgs& a, int rg, int tl) {
   const long long rows = (long long)a.max_new * a.group < a.rows_max ? (long long)a.max_new * a.group : a.rows_max;
   const long long groups = (rows + rg - 1) / rg;
-  const long long tokens = ((long long)a.width << a.block_log2) + a.max_new + rg + (2ll << tl);
+  const long long tokens = ((long long)a.width << a.block_log2) + 1 + groups * ((rg + a.group - 1) / a.group);
   const long long per_head = groups * ((tokens >> tl) + 5);
   return per_head > (1ll << 40) ? per_head : per_head * a.heads;
 }
