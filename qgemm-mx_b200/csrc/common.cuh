@@ -74,6 +74,12 @@ __device__ __forceinline__ void pdl_begin_after() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
+// Loads of what an earlier kernel of the stream may have written.  Not __ldg: a kernel
+// launched this way is set up while that kernel still runs, so its inputs are not
+// read-only for its lifetime, and the compiler may move a read-only load in front of
+// pdl_wait().
+__device__ __forceinline__ uint4 ld16(const void* p) { return *static_cast<const uint4*>(p); }
+
 inline cudaStream_t as_stream(void* s) { return static_cast<cudaStream_t>(s); }
 
 struct DevProps {

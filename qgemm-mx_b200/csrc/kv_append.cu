@@ -95,14 +95,14 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append(const AppendArgs a
 #pragma unroll
   for (int j = 0; j < HELD; ++j) {
     const int v = gl + j * GT;
-    held[j] = v < nv ? __ldg(src(v)) : make_uint4(0, 0, 0, 0);
+    held[j] = v < nv ? ld16(src(v)) : make_uint4(0, 0, 0, 0);
   }
 #pragma unroll
   for (int j = 0; j < HELD; ++j)
     m2 = amax2(held[j].x, amax2(held[j].y, amax2(held[j].z, amax2(held[j].w, m2))));
 #pragma unroll 1
   for (int v = gl + HELD * GT; v < nv; v += GT) {  // only a warp's long runs; read again below
-    const uint4 w = __ldg(src(v));
+    const uint4 w = ld16(src(v));
     m2 = amax2(w.x, amax2(w.y, amax2(w.z, amax2(w.w, m2))));
   }
   auto group_max = [&](uint32_t m) {
@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append(const AppendArgs a
     m = 0;
 #pragma unroll 1
     for (int v = gl; v < nv; v += GT) {
-      const uint4 w = __ldg(src(v));
+      const uint4 w = ld16(src(v));
       m = amax_finite(w.x, amax_finite(w.y, amax_finite(w.z, amax_finite(w.w, m))));
     }
     m = group_max(m);
@@ -152,11 +152,11 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append(const AppendArgs a
       if (v < nv) put(v, held[j]);
     }
 #pragma unroll 1
-    for (int v = gl + HELD * GT; v < nv; v += GT) put(v, __ldg(src(v)));
+    for (int v = gl + HELD * GT; v < nv; v += GT) put(v, ld16(src(v)));
   } else {
 #pragma unroll 1
     for (int v = gl; v < nv; v += GT) {
-      const uint4 w = __ldg(src(v));
+      const uint4 w = ld16(src(v));
       *reinterpret_cast<uint2*>(dst + v * 8) =
           make_uint2(encode4<TYPE, false>(w.x, w.y, f), encode4<TYPE, false>(w.z, w.w, f));
     }

@@ -189,7 +189,7 @@ k_kv_decode(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
         for (int j = 0; j < KJ; ++j)
 #pragma unroll
           for (int x = 0; x < 2; ++x)
-            w[nt][j][x] = row < s.rows ? __ldg(reinterpret_cast<const uint4*>(qp + (t + 4 * j) * 16) + x)
+            w[nt][j][x] = row < s.rows ? ld16(reinterpret_cast<const uint4*>(qp + (t + 4 * j) * 16) + x)
                                        : make_uint4(0, 0, 0, 0);
       }
     };
@@ -217,7 +217,7 @@ k_kv_decode(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
     // exponents of a stage's blocks, K's | V's << 8: loaded a tile ahead
     auto load_exp = [&](int stage) {
       const int cell = s_cell[warp * ST + stage];
-      return (uint32_t)__ldg(a.ks + cell) | ((uint32_t)__ldg(a.vs + cell) << 8);
+      return (uint32_t)a.ks[cell] | ((uint32_t)a.vs[cell] << 8);
     };
     __syncwarp();
     uint32_t mt_next = load_exp(0);

@@ -249,8 +249,8 @@ k_kv_prefill(const KvAttnArgs a) {
         ek = ev = 127u;
         if (id >= 0) {
           const size_t cell = (size_t)id * a.heads + s.h;
-          ek = __ldg(a.ks + cell);
-          ev = __ldg(a.vs + cell);
+          ek = a.ks[cell];
+          ev = a.vs[cell];
         }
       };
       auto load_codes = [&](const uint8_t* src, int x, int id, uint4 (&w)[PC]) {
@@ -261,7 +261,7 @@ k_kv_prefill(const KvAttnArgs a) {
           const int b = __shfl_sync(0xFFFFFFFFu, id, t >> 4);
           w[i] = make_uint4(0, 0, 0, 0);
           if (b >= 0 && t < room)
-            w[i] = __ldg(reinterpret_cast<const uint4*>(src + (uint64_t)(uint32_t)b * block_bytes + head_off +
+            w[i] = ld16(reinterpret_cast<const uint4*>(src + (uint64_t)(uint32_t)b * block_bytes + head_off +
                                                         (t & ((1 << lg) - 1)) * HD));
         }
       };
@@ -301,7 +301,7 @@ k_kv_prefill(const KvAttnArgs a) {
             const int rr = r0 + (batch * 4 + y) * STEP;
             const int i = (int)(((float)(g0 + rr) + 0.5f) * inv_group), gh = g0 + rr - i * a.group;
             w[y] = make_uint4(0, 0, 0, 0);
-            if (rr < rows) w[y] = __ldg(reinterpret_cast<const uint4*>(q0 + i * a.q_stride + gh * a.q_head_stride));
+            if (rr < rows) w[y] = ld16(reinterpret_cast<const uint4*>(q0 + i * a.q_stride + gh * a.q_head_stride));
           }
         };
         auto put_q = [&](int batch, const uint4 (&w)[4]) {

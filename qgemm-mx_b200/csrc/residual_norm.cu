@@ -80,7 +80,7 @@ __device__ __forceinline__ uint4 pack8(const Pair (&f)[4]) {
   }
   return make_uint4(u[0], u[1], u[2], u[3]);
 }
-__device__ __forceinline__ uint4 vec_at(const uint16_t* p, int v) { return __ldg(reinterpret_cast<const uint4*>(p) + v); }
+__device__ __forceinline__ uint4 vec_at(const uint16_t* p, int v) { return ld16(reinterpret_cast<const uint4*>(p) + v); }
 
 __device__ __forceinline__ float warp_sum(float x) {
 #pragma unroll

@@ -187,3 +187,63 @@ def test_every_tensor_must_be_on_the_calls_gpu(qg, cuda):
         qg.kv_append(host, k, k, slots, runs)
     with pytest.raises(ValueError, match="the cache must be on a GPU"):
         qg.kv_attention(host, q, starts, lens, table, 1, workspace=ws)
+
+
+# ---- calls behind one another ----------------------------------------------------------
+
+@pytest.mark.parametrize("tokens,width", [(1, 8192), (700, 2880), (64, 16384)])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+def test_norms_read_what_the_call_before_wrote(qg, cuda, tokens, width, kind):
+    """A call is set up while the one before still runs; whatever it reads (stream, block,
+    gate, weights) is what that call left."""
+    g = torch.Generator(device="cuda").manual_seed(width)
+    y, r = (torch.randn((tokens, width), generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    w = (torch.randn(width, generator=g, device="cuda") * 0.1 + 1).to(torch.bfloat16)
+
+    def chain(wait):
+        a, h = qg.residual_norm(y, r, post=w, pre=w, kind=kind)
+        for _ in range(6):
+            wait()
+            b, h2 = qg.residual_norm(h, a, post=w, pre=w, gate=h, alpha=0.5, kind=kind)      # block and gate
+            wait()
+            a, h = qg.residual_norm(h2, b, post=h2[-1], pre=b[0], gate=h2[0], kind=kind)     # weights
+        return a, h
+
+    want = chain(torch.cuda.synchronize)
+    for _ in range(10):
+        got = chain(lambda: None)
+        for x, z in zip(got, want):
+            assert torch.equal(x.view(torch.int16), z.view(torch.int16))
+
+
+@pytest.mark.parametrize("new", [1, 6, 150])
+def test_attention_reads_what_append_just_wrote(qg, cuda, new):
+    """Steps without a wait between their calls give what the same calls give one by one."""
+    block, heads, group, d, requests = 16, 2, 4, 128, 9
+    g = torch.Generator(device="cuda").manual_seed(new)
+    steps = 4
+    x = torch.randn((steps, requests * new, (group + 2) * heads, d), generator=g, device="cuda").to(torch.bfloat16)
+    width = -(-steps * new // block)
+    blocks = requests * width + 2
+
+    def run(wait):
+        c = qg.make_kv_cache(qg.KV_E4M3, blocks, block, heads, d)
+        lens, table = i32([0] * requests), torch.zeros((requests, width), dtype=torch.int32, device="cuda")
+        free, count = torch.arange(blocks, dtype=torch.int32, device="cuda"), i32([blocks])
+        ws = qg.make_kv_workspace(c, heads * group, requests, requests * new, new)
+        outs = []
+        for s in range(steps):
+            q, k, v = x[s].split([group * heads, heads, heads], 1)
+            p = qg.kv_plan(lens, i32([new] * requests), table, free, count, block, requests * new)
+            wait()
+            qg.kv_append(c, k, v, p.slots, p.runs)
+            wait()
+            outs.append(qg.kv_attention(c, q, p.starts, p.lens, table, new, workspace=ws))
+            wait()
+            lens, count = p.lens, p.counts[:1]
+        return outs
+
+    want = run(torch.cuda.synchronize)
+    for _ in range(5):
+        for a, b in zip(run(lambda: None), want):
+            assert torch.equal(a.view(torch.int16), b.view(torch.int16))
