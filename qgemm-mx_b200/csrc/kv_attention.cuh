@@ -19,7 +19,6 @@
 
 namespace qg {
 
-
 struct KvAttnArgs {
   const uint8_t *k, *v, *ks, *vs;
   const uint16_t* q;
@@ -35,7 +34,7 @@ struct KvAttnArgs {
   uint16_t* out;
   float* lse;
   int beside;  // the launch before is this call's other kernel, whose results are not needed
-  unsigned* tickets;  // zero between calls
+  unsigned* tickets;  // the decode kernel's: zero between calls
   float* partials;
 };
 
@@ -210,11 +209,11 @@ __device__ __forceinline__ int kv_find(const KvBatch<MOST>& b, int requests, int
   return lo;
 }
 
-// Fills the batch and returns the line's length; longest: the most places a
-// pair has, at most 2^15.  The first WARPS warps do the
-// work; all threads must call it.
-template <int RG, int TL, int WARPS, int MOST>
-__device__ __forceinline__ int kv_line(const KvAttnArgs& a, KvBatch<MOST>& b, int* scan, int& longest) {
+// Fills the batch and returns the line's length; LONGEST: and the most places a pair
+// has, at most 2^15, in `longest`.  The first WARPS warps do the work; all threads must
+// call it.  scan: WARPS words, 2 WARPS with LONGEST.
+template <int RG, int TL, int WARPS, bool LONGEST, int MOST>
+__device__ __forceinline__ int kv_line_any(const KvAttnArgs& a, KvBatch<MOST>& b, int* scan, int& longest) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int base = 0;
   longest = 0;
@@ -232,7 +231,8 @@ __device__ __forceinline__ int kv_line(const KvAttnArgs& a, KvBatch<MOST>& b, in
       if (q.n > 0) {
         const KvLine<RG, TL> line(a, q);
         c = a.heads * line.upto(line.groups);
-        most = min(line.upto(line.groups) - line.upto(line.groups - 1), 1 << 15);  // the last group's is the largest
+        // the last group's is the largest
+        if (LONGEST) most = min(line.upto(line.groups) - line.upto(line.groups - 1), 1 << 15);
       }
     }
     int v = c;
@@ -241,15 +241,18 @@ __device__ __forceinline__ int kv_line(const KvAttnArgs& a, KvBatch<MOST>& b, in
       const int u = __shfl_up_sync(0xFFFFFFFFu, v, d);
       if (lane >= d) v += u;
     }
-    most = __reduce_max_sync(0xFFFFFFFFu, most);
-    if (lane == 31 && warp < WARPS) { scan[warp] = v; scan[WARPS + warp] = most; }
+    if (LONGEST) most = __reduce_max_sync(0xFFFFFFFFu, most);
+    if (lane == 31 && warp < WARPS) {
+      scan[warp] = v;
+      if (LONGEST) scan[WARPS + warp] = most;
+    }
     __syncthreads();
     int before = base, total = base;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
       if (w == warp) before = total;
       total += scan[w];
-      longest = max(longest, scan[WARPS + w]);
+      if (LONGEST) longest = max(longest, scan[WARPS + w]);
     }
     if (on) b.prefix[r] = before + v - c;
     base = total;
@@ -258,6 +261,15 @@ __device__ __forceinline__ int kv_line(const KvAttnArgs& a, KvBatch<MOST>& b, in
   if (tid == 0) b.prefix[a.requests] = base;
   __syncthreads();
   return base;
+}
+template <int RG, int TL, int WARPS, int MOST>
+__device__ __forceinline__ int kv_line(const KvAttnArgs& a, KvBatch<MOST>& b, int* scan) {
+  int longest;
+  return kv_line_any<RG, TL, WARPS, false>(a, b, scan, longest);
+}
+template <int RG, int TL, int WARPS, int MOST>
+__device__ __forceinline__ int kv_line(const KvAttnArgs& a, KvBatch<MOST>& b, int* scan, int& longest) {
+  return kv_line_any<RG, TL, WARPS, true>(a, b, scan, longest);
 }
 
 // One row (of RG) of a pair that crosses CTAs, joined by a warp from the CTAs'

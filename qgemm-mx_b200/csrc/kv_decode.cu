@@ -606,12 +606,12 @@ cudaError_t kv_decode_fault_clear() {
 // 32 rows 147 and 113 us, 40 rows 148 and 158 us.
 static int kv_prefill_rows(int head_dim) { return head_dim == 128 ? 48 : 32; }
 
-// Workspace: 4 KiB of tickets for each kernel, then their partials.
+// Workspace: 4 KiB of the decode kernel's tickets, then both kernels' partials.
 struct KvWorkspace {
   size_t decode, prefill, total;  // byte offsets of the partials
   KvWorkspace(int head_dim, long long rows, int sm_count) {
     const size_t slot = (size_t)8 * dec_nt(rows, INT32_MAX) * (head_dim + 2) * sizeof(float);
-    decode = 8192;
+    decode = 4096;
     prefill = decode + (size_t)sm_count * 2 * slot;
     total = prefill + (rows > kv_prefill_rows(head_dim) ? kv_prefill_workspace(head_dim, sm_count) : 0);
   }
@@ -639,7 +639,7 @@ static qgemm_status_t kv_attention_run(const qgemm_kv_cache_t* c, KvAttnArgs a, 
   for (int kernel = many && even ? 1 : 0; kernel <= (many ? 1 : 0); ++kernel) {
     a.rows_min = kernel && !even ? few : 0;
     a.rows_max = kernel ? INT32_MAX : few;
-    a.tickets = reinterpret_cast<unsigned*>(static_cast<char*>(ws) + 4096 * kernel);
+    a.tickets = static_cast<unsigned*>(ws);
     a.partials = reinterpret_cast<float*>(static_cast<char*>(ws) + (kernel ? w.prefill : w.decode));
     // beside prompt chunks the few rows are as a rule one token's
     const int nt = dec_nt(many ? a.group : rows, (long long)all * a.heads);

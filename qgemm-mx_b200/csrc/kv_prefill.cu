@@ -153,7 +153,7 @@ k_kv_prefill(const KvAttnArgs a) {
   constexpr int RG = kPreRows, TL = kPreTokLog2, TILE = Cfg::kTile;
   extern __shared__ uint8_t smem_raw[];
   __shared__ KvBatch<kKvPrefillRequests> s_batch;
-  __shared__ int s_scan[32];
+  __shared__ int s_scan[16];
   __shared__ __align__(1024) uint64_t s_bars[32];
   __shared__ PreMeta s_meta[4][8];   // by tile, four deep: read after the tile's stage may be refilled
   __shared__ float s_fq[2][RG];      // by stretch: score factor of each row
@@ -173,8 +173,7 @@ k_kv_prefill(const KvAttnArgs a) {
 
   if (a.beside) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the wait is at the end
   else pdl_begin_after();
-  int longest;
-  const int V = kv_line<RG, TL, 16>(a, s_batch, s_scan, longest);
+  const int V = kv_line<RG, TL, 16>(a, s_batch, s_scan);
   const int E = max(1, min((int)gridDim.x, V));
   const int cta = blockIdx.x;
   if (V == 0 || cta >= E) {
@@ -578,8 +577,8 @@ k_kv_prefill(const KvAttnArgs a) {
         o_par ^= 1u;
         tc_fence_after();
       }
-      // after a timeout the stretches that are left still go through the join, so
-      // that the barrier below is met and the tickets return to zero
+      // after a timeout the stretches that are left still write their partials, which the
+      // join kernel reads, and the barrier below is met
       const bool whole = seg_v0 == s.pair_v && v == s.pair_end;
       const int c_first = cuts.share_of(s.pair_v);
       float* slot = a.partials + (size_t)(cta * 2 + (cta == c_first ? 1 : 0)) * Cfg::kSlot;
@@ -642,12 +641,11 @@ template <int HD>
 __global__ void __launch_bounds__(256) k_kv_prefill_join(const KvAttnArgs a, int grid) {
   constexpr int RG = kPreRows, TL = kPreTokLog2, N4 = 32 * HD / 4 / 256;  // float4 per thread
   __shared__ KvBatch<kKvPrefillRequests> s_batch;
-  __shared__ int s_scan[16];
+  __shared__ int s_scan[8];
   const int tid = threadIdx.x;
   // the requests are known; only the partials come from the kernel before
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  int longest;
-  const int V = kv_line<RG, TL, 8>(a, s_batch, s_scan, longest);
+  const int V = kv_line<RG, TL, 8>(a, s_batch, s_scan);
   const int E = max(1, min(grid, V)), c_first = blockIdx.x;
   if (c_first + 1 >= E) {
     pdl_wait();
