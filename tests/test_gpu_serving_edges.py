@@ -74,6 +74,15 @@ def test_plan_takes_no_block_past_the_free_list(qg, cuda, listed):
 
 # ---- attention ----------------------------------------------------------------------
 
+def within(out, lse, want, wlse, mass, logit, floor, d, most):
+    """The bounds of test_gpu_kv_attention.py."""
+    tol = want.abs() * 2.0 ** -8 + mass * (2.0 ** -11 + 2.0 ** -20 + (2 * d * logit[..., None] + most) * 2.0 ** -23) + \
+        floor * 2.0 ** -35
+    assert ((out.double() - want).abs() <= tol).all()
+    if lse is not None:
+        assert ((lse.double() - wlse).abs() <= (d * logit + most + 64) * 2.0 ** -23 + wlse.abs() * 2.0 ** -22).all()
+
+
 def check_outside(qg, kv, lens, new, block, heads, group, d, seed, ids, fill=127):
     """kv_attention with some table entries outside the pool against a cache in which they
     name a block of zeros, with the bounds of test_gpu_kv_attention.py.  `fill`: the scale
@@ -93,12 +102,7 @@ def check_outside(qg, kv, lens, new, block, heads, group, d, seed, ids, fill=127
     assert place >= len(ids)
     ws = qg.make_kv_workspace(c, q.shape[1], len(lens), q.shape[0], new)
     out, lse = qg.kv_attention(c, q, starts, n, table, new, lse=True, workspace=ws)
-    want, wlse, mass, logit, floor = R.attention(kv, *shadow, q, starts, n, mapped, d ** -0.5)
-    most = max(lens)
-    tol = want.abs() * 2.0 ** -8 + mass * (2.0 ** -11 + 2.0 ** -20 + (2 * d * logit[..., None] + most) * 2.0 ** -23) + \
-        floor * 2.0 ** -35
-    assert ((out.double() - want).abs() <= tol).all()
-    assert ((lse.double() - wlse).abs() <= (d * logit + most + 64) * 2.0 ** -23 + wlse.abs() * 2.0 ** -22).all()
+    within(out, lse, *R.attention(kv, *shadow, q, starts, n, mapped, d ** -0.5), d, max(lens))
 
 
 OUTSIDE = [-1, -5, "blocks", TOP, -2 ** 31, -2 ** 30 - 1, -2 ** 30, -715827883, 2 ** 30]
@@ -142,6 +146,64 @@ def test_a_workspace_belongs_to_the_calls_stream(qg, cuda, new):
         s.synchronize()
         assert torch.equal(out, want)
         del taken
+
+
+@pytest.mark.parametrize("kv", [0, 1])
+@pytest.mark.parametrize("d", [64, 128])
+def test_rows_past_max_new_are_left_alone(qg, cuda, kv, d):
+    """max_new bounds the rows that are computed, from each request's first on; those that
+    are computed are at their own positions."""
+    c, q, starts, lens, table = make(qg, kv, [300, 200, 7], [140, 3, 9], 32, 2, 4, d, 131)
+    want, wlse, mass, logit, floor = R.attention(kv, c.k, c.v, c.k_scales, c.v_scales, q, starts, lens, table, d ** -0.5)
+    first = torch.cat([torch.arange(n) for n in (140, 3, 9)]).to("cuda")
+    empty = torch.isinf(wlse)
+    for most in (1, 4, 12, 20, 139):
+        out = torch.full_like(q, 5.0, memory_format=torch.contiguous_format)
+        _, lse = qg.kv_attention(c, q, starts, lens, table, most, out=out, lse=True)
+        some = first < most
+        assert (out[~some] == 5.0).all()
+        assert torch.equal(torch.isinf(lse[some]), empty[some]) and (out[some][empty[some]] == 0).all()
+        see = some[:, None] & ~empty
+        within(out[see], lse[see], want[see], wlse[see], mass[see], logit[see], floor[see], d, 300)
+
+
+@pytest.mark.parametrize("kv", [0, 1])
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_mixed_call_on_another_stream_and_in_a_graph(qg, cuda, kv, d):
+    """Decoding requests beside prompt chunks, whose two kernels and join overlap, behind and
+    in front of other calls: the same bits every time, within the bounds."""
+    new = [1, 130, 1, 20, 300, 1, 2]
+    c, q, starts, lens, table = make(qg, kv, [700, 500, 90, 64, 300, 1, 1500], new, 64, 2, 4, d, 141)
+    tokens = sum(new)
+    ws = qg.make_kv_workspace(c, 8, 7, tokens, 300)
+    w = torch.ones(8 * d, dtype=torch.bfloat16, device="cuda")
+
+    def call(out, stream=None):
+        qg.kv_attention(c, q, starts, lens, table, 300, out=out, workspace=ws, stream=stream)
+        return qg.residual_norm(None, out.flatten(1), pre=w, stream=stream)[1]
+
+    want = torch.zeros((tokens, 8, d), dtype=torch.bfloat16, device="cuda")
+    h = call(want)
+    within(want, None, *R.attention(kv, c.k, c.v, c.k_scales, c.v_scales, q, starts, lens, table, d ** -0.5), d, 1500)
+    out = torch.zeros_like(want)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    for _ in range(5):
+        got = [call(out, s) for _ in range(3)]
+        s.synchronize()
+        assert torch.equal(out, want) and all(torch.equal(x, h) for x in got)
+        out.zero_()
+        torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(3):
+            got = call(out)
+    for _ in range(5):
+        out.zero_()
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(got, h)
 
 
 # ---- where tensors lie ---------------------------------------------------------------
