@@ -283,7 +283,9 @@ qgemm_status_t qgemm_clear_faults(void);
  * The cache is a pool of blocks.  A block holds `block` consecutive tokens of
  * one request for every KV head; codes lie [blocks][heads][block][head_dim],
  * one E8M0 scale byte (2^(byte - 127)) per (block, head) beside them, for K
- * and for V.  A request's row of the block table names its blocks in order.  */
+ * and for V.  A request's row of the block table names its blocks in order.
+ * Scale bytes are 63 .. 249 (2^-64 .. 2^122), as qgemm_kv_append writes them;
+ * attention over a cache that other code filled with others is not defined.  */
 typedef enum { QGEMM_KV_E4M3 = 0, QGEMM_KV_INT8 = 1 } qgemm_kv_type_t;
 typedef struct {
   int32_t type;       /* qgemm_kv_type_t                                     */
@@ -364,6 +366,12 @@ qgemm_status_t qgemm_kv_append(const qgemm_kv_cache_t* cache, const uint16_t* k,
  * table_width * block are cut to it; tokens of a block id outside the pool
  * read as zeros.  Rows beyond starts[requests] are left as they are.  head_dim
  * values of q lie together, q is 16-byte aligned, its strides multiples of 8.
+ * Arithmetic: q as f16 relative to the power of two below its row's largest
+ * value (exact down to 2^-24 of it), scores and every sum in 32 bits, softmax
+ * weights rounded once to f16 for the product with V's codes (the sum below it
+ * takes them unrounded), approximate exp2, log2 and reciprocal; out is off by
+ * its rounding to bf16 and 2^-11 sum(p |v|) at most, beside the scores' own
+ * error of head_dim 2^-24 scale sum|q K|.
  * workspace: qgemm_kv_attention_workspace() bytes, 16-byte aligned, zeroed once
  * (qgemm_workspace_init); every call returns its tickets to zero.            */
 size_t qgemm_kv_attention_workspace(const qgemm_kv_cache_t* cache, int32_t q_heads,
@@ -389,6 +397,7 @@ qgemm_status_t qgemm_kv_attention(const qgemm_kv_cache_t* cache, const uint16_t*
  * row for all with gate_stride 0.  With y null, h is the norm of residual and
  * residual_out is not written (post, gate must be null).  With pre null, h is
  * not written.  residual_out may be residual, and h may be y.
+ * Sums in 32 bits, r' rounded once; the norms' factors are within 2^-17.
  * width: a multiple of 8, at most 16384; rows 16-byte aligned.               */
 typedef enum { QGEMM_NORM_RMS = 0, QGEMM_NORM_LAYER = 1 } qgemm_norm_kind_t;
 typedef struct {

@@ -5,9 +5,11 @@
 //   w   = 2^(s + ev - m)                             weight with V's scale folded in
 //   out = sum(w vc) / sum(w 2^-ev)
 // V's scale rides in the exponent, so P.V needs no factor per block: w is
-// rounded once to f16 beside the exact f16 widening of vc, and the denominator
-// takes the unrounded w times 2^-ev in 32 bits.  Scales are at least 2^-64, so
-// that denominator stays below 2^80 times the token count.
+// rounded once to f16 beside the exact f16 widening of vc (off by 2^-11 of a weight at
+// most, where the result's own rounding to bf16 may be off by 2^-8; the tensor cores
+// take f16 beside f16 only), and the denominator takes the unrounded w times 2^-ev in 32 bits.  Scales
+// are 2^-64 .. 2^122, as the append writes them (the cache's description requires
+// it), so that denominator stays below 2^80 times the token count.
 // m is a running reference, not the maximum: it moves to max(s + ev) - 10 only
 // when a value passes m + 15.  Rescaling is then rare, w stays below 2^15, and
 // f16 keeps its 11 bits for weights down to 2^-24 of the largest.
@@ -41,6 +43,8 @@ struct KvAttnArgs {
 constexpr float kKvTop = 10.0f;   // log2 of the largest weight after m moves
 constexpr float kKvGrow = 15.0f;  // and the one that makes it move
 
+// The approximate exp2 and reciprocal are off by some 2^-22 of the value, the roundings
+// of the weights and of the result by up to 2^-11 and 2^-8.
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -113,10 +117,11 @@ struct KvBatch {
 template <int RG, int TL>
 struct KvLine {
   // Tiles of 16 go by in a quarter of the time that a pair's queries, search and
-  // store take: 64 requests of 129 to 8192 tokens 97.5 us, 200 in a window of 128
-  // 18.8 us, against 102 and 20.5 with 2, 97.5 and 19.6 with 8, 108 and 29.8 with 1.
+  // store take: 64 requests of 129 to 8192 tokens 97 us, 200 in a window of 128
+  // 18.5 us, against 101 and 19.9 with 2, 97 and 19.2 with 8, 104 and 29.4 with 1.
   // Of the prefill kernel's 128 tokens a start weighs three: 13 decoding requests and 3
-  // prompt chunks of up to 512 tokens 126 us, 138 with 1, 129 with 5.
+  // prompt chunks of up to 512 tokens 120 us, 132 with 1, 122 with 5.  (All of them
+  // calls behind one another in a CUDA graph.)
   static constexpr int kStart = TL == 4 ? 4 : 3;
   int h0, slope, groups;
   __host__ __device__ __forceinline__ KvLine(const KvAttnArgs& a, const KvRequest& q) {

@@ -210,15 +210,21 @@ static bool plan_overlap(const PlanArgs& a, const char** x, const char** y) {
       {"lens", a.lens, 4 * R}, {"news", a.news, 4 * R}, {"table", a.table, 4 * R * a.width},
       {"free_list", a.free_list, !a.free_list ? 0 : a.free_len == INT32_MAX ? 4 : 4ll * a.free_len}, {"free_count", a.free_count, 4}};
   constexpr int outputs = 6, all = sizeof(spans) / sizeof(spans[0]);
+  auto meet = [&](int i, int j) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(spans[i].at), q = reinterpret_cast<uintptr_t>(spans[j].at);
+    const uintptr_t n = (uintptr_t)spans[i].bytes, m = (uintptr_t)spans[j].bytes;
+    return (n > 0) & (m > 0) & (p < q + m) & (q < p + n);
+  };
+  int any = 0;  // no branches while there is nothing to report
   for (int i = 0; i < outputs; ++i)
-    for (int j = i + 1; j < all; ++j) {
-      const uintptr_t p = reinterpret_cast<uintptr_t>(spans[i].at), q = reinterpret_cast<uintptr_t>(spans[j].at);
-      if (spans[i].bytes > 0 && spans[j].bytes > 0 && p < q + spans[j].bytes && q < p + spans[i].bytes) {
+    for (int j = i + 1; j < all; ++j) any |= meet(i, j);
+  for (int i = 0; any && i < outputs; ++i)
+    for (int j = i + 1; j < all; ++j)
+      if (meet(i, j)) {
         *x = spans[i].name;
         *y = spans[j].name;
         return true;
       }
-    }
   return false;
 }
 

@@ -27,9 +27,10 @@
 // What bounds it: exponentials and the tensor core alike (a row and token cost one
 // ex2, 16 a clock and SM, as long as its 2 x 2 x 128 multiply-adds take at 128
 // dims), and above that the roles' waiting for one another.  Measured, 2048 rows of
-// 32 heads over 8 KV heads of 128 dims and 8192 tokens: 295 us, 816 TFLOP/s; a tile
-// of 128 tokens takes some 4400 cycles where its MMAs take 3200, a stretch's start
-// 15000.
+// 32 heads over 8 KV heads of 128 dims and 8192 tokens: 296 us, 813 TFLOP/s; by clock
+// stamps a tile of 128 tokens takes 4400 to 4750 cycles where its MMAs and commits alone
+// take 3200, and 9500 to 16600 pass between a stretch's last scores and the next one's
+// first (8900 to 11200 at 64 dims).
 //
 // The line of all pairs' tiles is cut into one equal share per CTA
 // (kv_attention.cuh), so all CTAs finish together whatever the pair count; pairs
@@ -283,7 +284,7 @@ k_kv_prefill(const KvAttnArgs a) {
       uint4 wk[PC], wv[PC];
       // q: 16 (8 for 64 dims) lanes a row.  All of its loads are under way while the
       // last stretch's q is still read and before that stretch's partials are
-      // written, whose stores would hold them up for some 5000 cycles: a stretch's
+      // written, whose stores would hold them up for 3000 to 7000 cycles: a stretch's
       // start is a pause for all other warps.
       {
         constexpr int LPR = HD / 8;  // lanes per row

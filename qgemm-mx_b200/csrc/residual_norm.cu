@@ -12,9 +12,9 @@
 // With many rows the instructions count as well as the bytes (some 45 for each
 // value's 14 bytes): values are worked on in pairs, and the warps' sums are
 // joined by as many lanes as the row has warps.  Measured: 6000 rows of 2880,
-// LayerNorm, gate, FP32 residual (242 MB): 49.2 us, 4.9 TB/s, 54.1 us with
+// LayerNorm, gate, FP32 residual (242 MB): 49.5 us, 4.9 TB/s, 54.1 us with
 // single values and the warps' sums added up one by one; one row of 8192,
-// RMS: 4.2 us in a stream of such calls (6.2 before).
+// RMS: 2.9 us in a CUDA graph of such calls (host time sets 4.7 outside of one).
 #include <cuda_bf16.h>
 
 #include "common.cuh"
@@ -104,7 +104,8 @@ __device__ __forceinline__ float lanes_sum(float x, int half) {
 // x <- N(x) in place.  V vectors of 8 values per thread; those past the row are
 // zero.  LayerNorm centres each warp's values on the warp's own mean m_w and
 // joins the warps by M2 = sum_w (M2_w + n_w (m_w - mean)^2): as sound as a
-// second pass over the centred row, at one barrier instead of two.  `buf`: one
+// second pass over the centred row, at one barrier instead of two.  (The warp's mean may
+// be off by the approximate division's 2^-22 of it, as by its sum's own rounding.)  `buf`: one
 // entry per warp of the CTA, another one for each norm of a row.
 template <int V, bool LAYER>
 __device__ __forceinline__ void normalise(Pair (&x)[V][4], const uint16_t* weight, const uint16_t* bias, const Place& t,

@@ -31,8 +31,8 @@ def _handle(stream):
 class KVCache:
     """A pool of blocks on the device.  ``k`` and ``v`` hold 8-bit codes
     (uint8 storage) [blocks, heads, block, head_dim], ``k_scales`` and
-    ``v_scales`` one E8M0 byte per (block, head), 2^(byte - 127).  ``type`` is
-    KV_E4M3 or KV_INT8.  The attributes cannot be set: the calls go by the
+    ``v_scales`` one E8M0 byte per (block, head), 2^(byte - 127) with bytes of
+    63 .. 249.  ``type`` is KV_E4M3 or KV_INT8.  The attributes cannot be set: the calls go by the
     pointers taken here."""
     __slots__ = ("_type", "_k", "_v", "_k_scales", "_v_scales", "_desc")
 
@@ -126,7 +126,8 @@ def kv_attention(cache: KVCache, q: torch.Tensor, starts: torch.Tensor, lens: to
     """softmax(scale * q.K) . V over the cache: q bf16 [tokens, q_heads,
     head_dim], request r's rows starts[r] .. starts[r + 1] - 1 being the last
     of its lens[r] tokens.  scale defaults to head_dim ** -0.5; window > 0
-    bounds how far back a row sees.  Returns out (bf16, as q), or (out, lse)."""
+    bounds how far back a row sees.  Returns out (bf16, as q), or (out, lse).
+    Rows that no request brings, or past max_new of theirs, are not written."""
     if workspace is None:
         workspace = make_kv_workspace(cache, q.shape[1], lens.numel(), q.shape[0], max_new, stream)
     st, out, z = _b.kv_attention(cache._desc, q, starts, lens, table, max_new,
