@@ -63,15 +63,10 @@ inline cudaError_t pdl_launch(void (*kernel)(Params...), dim3 grid, dim3 block, 
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_begin() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  pdl_launch_dependents();
   pdl_wait();
-}
-// The same in the other order: a dependent that starts knows that what came before
-// this kernel is done.
-__device__ __forceinline__ void pdl_begin_after() {
-  pdl_wait();
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
 // Loads of what an earlier kernel of the stream may have written.  Not __ldg: a kernel

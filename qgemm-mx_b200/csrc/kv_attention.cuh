@@ -36,6 +36,7 @@ struct KvAttnArgs {
   uint16_t* out;
   float* lse;
   int beside;  // the launch before is this call's other kernel, whose results are not needed
+  unsigned* ready;  // set once what came before the call is done, cleared by the join kernel; or null
   unsigned* tickets;  // the decode kernel's: zero between calls
   float* partials;
 };
@@ -68,6 +69,21 @@ __device__ __forceinline__ float kv_inv(float l) {
 }
 __device__ __forceinline__ float kv_lse(float m, float l) {
   return l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
+}
+
+// A kernel that starts beside the one before it reads the call's inputs, which earlier
+// kernels wrote, without a griddepcontrol.wait of its own.  What orders those reads: a
+// kernel that has waited says so (release) before its dependents may start, and they
+// look (acquire).  A block that does not see it waits for the whole kernel instead.
+// All threads must call kv_look.
+__device__ __forceinline__ void kv_tell(const KvAttnArgs& a) {
+  if (a.ready && blockIdx.x == 0 && threadIdx.x == 0)
+    asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(a.ready), "r"(1u) : "memory");
+}
+__device__ __forceinline__ void kv_look(const KvAttnArgs& a) {
+  unsigned seen = 0;
+  if (threadIdx.x == 0) asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(a.ready) : "memory");
+  if (!__syncthreads_or((int)seen)) pdl_wait();
 }
 
 // Tokens row i of n sees: [lo, hi).

@@ -113,7 +113,9 @@ k_kv_decode(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  pdl_begin_after();
+  pdl_wait();
+  kv_tell(a);
+  pdl_launch_dependents();
   int longest;
   const int V = kv_line<RG, 4, W>(a, s_batch, s_scan, longest);
   const int E = max(1, min((int)gridDim.x * W, V));  // shares
@@ -606,7 +608,8 @@ cudaError_t kv_decode_fault_clear() {
 // 32 rows 147 and 113 us, 40 rows 148 and 158 us.
 static int kv_prefill_rows(int head_dim) { return head_dim == 128 ? 48 : 32; }
 
-// Workspace: 4 KiB of the decode kernel's tickets, then both kernels' partials.
+// Workspace: 4 KiB of the decode kernel's tickets and, as their last word, the call's
+// `ready`; then both kernels' partials.
 struct KvWorkspace {
   size_t decode, prefill, total;  // byte offsets of the partials
   KvWorkspace(int head_dim, long long rows, int sm_count) {
@@ -640,6 +643,7 @@ static qgemm_status_t kv_attention_run(const qgemm_kv_cache_t* c, KvAttnArgs a, 
     a.rows_min = kernel && !even ? few : 0;
     a.rows_max = kernel ? INT32_MAX : few;
     a.tickets = static_cast<unsigned*>(ws);
+    a.ready = many ? a.tickets + 1023 : nullptr;
     a.partials = reinterpret_cast<float*>(static_cast<char*>(ws) + (kernel ? w.prefill : w.decode));
     // beside prompt chunks the few rows are as a rule one token's
     const int nt = dec_nt(many ? a.group : rows, (long long)all * a.heads);

@@ -172,8 +172,14 @@ k_kv_prefill(const KvAttnArgs a) {
   constexpr int K_FULL = 0, K_EMPTY = 2, V_FULL = 4, V_EMPTY = 6, Q_FULL = 8, Q_EMPTY = 9, S_FULL = 10, P_FULL = 14,
                 O_DONE = 18;
 
-  if (a.beside) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the wait is at the end
-  else pdl_begin_after();
+  if (a.beside) {  // the wait is at the end
+    pdl_launch_dependents();
+    kv_look(a);
+  } else {
+    pdl_wait();
+    kv_tell(a);
+    pdl_launch_dependents();
+  }
   const int V = kv_line<RG, TL, 16>(a, s_batch, s_scan);
   const int E = max(1, min((int)gridDim.x, V));
   const int cta = blockIdx.x;
@@ -645,11 +651,17 @@ __global__ void __launch_bounds__(256) k_kv_prefill_join(const KvAttnArgs a, int
   __shared__ int s_scan[8];
   const int tid = threadIdx.x;
   // the requests are known; only the partials come from the kernel before
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  pdl_launch_dependents();
+  kv_look(a);
   const int V = kv_line<RG, TL, 8>(a, s_batch, s_scan);
   const int E = max(1, min(grid, V)), c_first = blockIdx.x;
+  auto clear = [&] {  // after the wait; a block of this kernel that looks later waits instead
+    if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0)
+      asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(a.ready), "r"(0u) : "memory");
+  };
   if (c_first + 1 >= E) {
     pdl_wait();
+    clear();
     return;
   }
   const KvCuts cuts(V, E);
@@ -659,6 +671,7 @@ __global__ void __launch_bounds__(256) k_kv_prefill_join(const KvAttnArgs a, int
   kv_seg<RG, TL>(a, s_batch, r, v, INT32_MAX, s);
   const int rows = s.rows - s.row0 - (int)blockIdx.y * 32;  // of this CTA's 32
   pdl_wait();
+  clear();
   if (s.pair_v == v || s.pair_v < cuts.at(c_first) || rows <= 0) return;
   const int c_last = cuts.share_of(s.pair_end - 1);
   KvJoined<RG, 128> j[N4];  // 4 values each

@@ -278,25 +278,28 @@ def test_norms_read_what_the_call_before_wrote(qg, cuda, tokens, width, kind):
             assert torch.equal(x.view(torch.int16), z.view(torch.int16))
 
 
-@pytest.mark.parametrize("new", [1, 6, 150])
-def test_attention_reads_what_append_just_wrote(qg, cuda, new):
-    """Steps without a wait between their calls give what the same calls give one by one."""
-    block, heads, group, d, requests = 16, 2, 4, 128, 9
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("news", [[1] * 9, [6] * 9, [150] * 9, [1, 150, 1, 1, 300, 1, 70, 1, 2], [1] * 300 + [90] * 4],
+                         ids=["steps", "few", "prompts", "mixed", "many"])
+def test_attention_reads_what_append_just_wrote(qg, cuda, news, d):
+    """Steps without a wait between their calls give what the same calls give one by one;
+    in a mixed step the two kernels of attention start beside one another."""
+    block, heads, group, requests, tokens, new = 16, 2, 4, len(news), sum(news), max(news)
     g = torch.Generator(device="cuda").manual_seed(new)
     steps = 4
-    x = torch.randn((steps, requests * new, (group + 2) * heads, d), generator=g, device="cuda").to(torch.bfloat16)
+    x = torch.randn((steps, tokens, (group + 2) * heads, d), generator=g, device="cuda").to(torch.bfloat16)
     width = -(-steps * new // block)
-    blocks = requests * width + 2
+    blocks = sum(-(-steps * n // block) for n in news) + 2
 
     def run(wait):
         c = qg.make_kv_cache(qg.KV_E4M3, blocks, block, heads, d)
         lens, table = i32([0] * requests), torch.zeros((requests, width), dtype=torch.int32, device="cuda")
         free, count = torch.arange(blocks, dtype=torch.int32, device="cuda"), i32([blocks])
-        ws = qg.make_kv_workspace(c, heads * group, requests, requests * new, new)
+        ws = qg.make_kv_workspace(c, heads * group, requests, tokens, new)
         outs = []
         for s in range(steps):
             q, k, v = x[s].split([group * heads, heads, heads], 1)
-            p = qg.kv_plan(lens, i32([new] * requests), table, free, count, block, requests * new)
+            p = qg.kv_plan(lens, i32(news), table, free, count, block, tokens)
             wait()
             qg.kv_append(c, k, v, p.slots, p.runs)
             wait()
