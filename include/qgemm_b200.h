@@ -396,7 +396,8 @@ qgemm_status_t qgemm_kv_attention(const qgemm_kv_cache_t* cache, const uint16_t*
  * 0; gate is [tokens][width] with gate_stride elements between rows, or one
  * row for all with gate_stride 0.  With y null, h is the norm of residual and
  * residual_out is not written (post, gate must be null).  With pre null, h is
- * not written.  residual_out may be residual, and h may be y.
+ * not written.  residual_out may be residual, and h may be y
+ * (an output may be any input of its layout and type, and overlap nothing else).
  * Sums in 32 bits, r' rounded once; the norms' factors are within 2^-17.
  * width: a multiple of 8, at most 16384; rows 16-byte aligned.               */
 typedef enum { QGEMM_NORM_RMS = 0, QGEMM_NORM_LAYER = 1 } qgemm_norm_kind_t;

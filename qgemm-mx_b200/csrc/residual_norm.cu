@@ -254,6 +254,36 @@ static cudaError_t launch_norm(const NormArgs& a, bool f32, unsigned grid, unsig
                     s, a);
 }
 
+// Whether an output shares a byte with the other output, or with an input whose elements
+// there are not the same ones: a thread reads its own elements of a row before it writes
+// them, but neither another thread's nor another row's.
+static bool norm_overlap(const qgemm_residual_norm_t* p) {
+  struct Span {
+    const void* at;
+    long long bytes, cell, stride;  // cell: bytes of an element; stride: bytes from row to row, 0 for all rows' one
+  };
+  const long long w = p->width, rows = p->tokens, own = p->residual_f32 ? 4 : 2;
+  const Span outs[2] = {{p->y ? p->residual_out : nullptr, rows * w * own, own, w * own},
+                        {p->pre ? p->h : nullptr, rows * w * 2, 2, w * 2}};
+  const Span ins[7] = {{p->y, rows * w * 2, 2, w * 2},
+                       {p->residual, rows * w * own, own, w * own},
+                       {p->gate, ((p->gate_stride ? rows - 1 : 0) * p->gate_stride + w) * 2, 2,
+                        rows == 1 ? w * 2 : p->gate_stride * 2},
+                       {p->post, w * 2, 2, 0},
+                       {p->post_bias, w * 2, 2, 0},
+                       {p->pre, w * 2, 2, 0},
+                       {p->pre_bias, w * 2, 2, 0}};
+  auto meet = [](const Span& a, const Span& b) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+    return x && y && x < y + (uintptr_t)b.bytes && y < x + (uintptr_t)a.bytes;
+  };
+  if (meet(outs[0], outs[1])) return true;
+  for (const Span& o : outs)
+    for (const Span& i : ins)
+      if (meet(o, i) && !(o.at == i.at && o.cell == i.cell && o.stride == i.stride)) return true;
+  return false;
+}
+
 }  // namespace qg
 
 using namespace qg;
@@ -285,6 +315,8 @@ qgemm_status_t qgemm_residual_norm(const qgemm_residual_norm_t* p, void* stream)
                         reinterpret_cast<uintptr_t>(p->pre_bias) | reinterpret_cast<uintptr_t>(p->residual_out) |
                         reinterpret_cast<uintptr_t>(p->h);
   if (all & 15u) return fail(QGEMM_ERR_INVALID_ARG, "residual_norm: arrays must be 16-byte aligned");
+  if (norm_overlap(p))
+    return fail(QGEMM_ERR_INVALID_ARG, "residual_norm: outputs overlap each other, or an input at other places or of another type");
   NormArgs a;
   a.y = p->y; a.residual = p->residual; a.post = p->post; a.post_bias = p->post_bias; a.gate = p->gate;
   a.gate_stride = p->gate_stride; a.pre = p->pre; a.pre_bias = p->pre_bias; a.alpha = p->alpha; a.eps = p->eps;

@@ -278,6 +278,22 @@ def test_norms_read_what_the_call_before_wrote(qg, cuda, tokens, width, kind):
             assert torch.equal(x.view(torch.int16), z.view(torch.int16))
 
 
+@pytest.mark.parametrize("tokens", [1, 37])
+def test_norm_over_its_own_inputs(qg, cuda, tokens):
+    """An output may be any input of its layout: the stream, the block or the gate."""
+    g = torch.Generator(device="cuda").manual_seed(tokens)
+    y, r, gate = (torch.randn((tokens, 520), generator=g, device="cuda").to(torch.bfloat16) for _ in range(3))
+    w = (torch.randn(520, generator=g, device="cuda") * 0.1 + 1).to(torch.bfloat16)
+    want, h = qg.residual_norm(y, r, post=w, pre=w, gate=gate)
+    for a, b in ((1, 0), (0, 1), (2, 0), (1, 2), (0, 2)):
+        x = [y.clone(), r.clone(), gate.clone()]
+        got, got_h = qg.residual_norm(x[0], x[1], post=w, pre=w, gate=x[2], residual_out=x[a], h=x[b])
+        assert torch.equal(got, want) and torch.equal(got_h, h)
+        x = [y.clone(), r.clone(), gate.clone()]
+        with pytest.raises(ValueError, match="overlap"):
+            qg.residual_norm(x[0], x[1], post=w, pre=w, gate=x[2], residual_out=x[a], h=x[a])
+
+
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("news", [[1] * 9, [6] * 9, [150] * 9, [1, 150, 1, 1, 300, 1, 70, 1, 2], [1] * 300 + [90] * 4],
                          ids=["steps", "few", "prompts", "mixed", "many"])

@@ -5,7 +5,7 @@ import ctypes as C
 
 import pytest
 import torch
-from test_serving_abi import cache
+from test_serving_abi import Norm, cache
 
 M = 1 << 20  # plausible, aligned addresses that are never read, M apart
 
@@ -86,3 +86,22 @@ def test_a_caches_tensors_cannot_be_exchanged(qg):
     assert c.k is k and c.k_scales is s and c.type == qg.KV_E4M3
     c.k[0] = 5  # their contents can be changed
     assert c.values()[0].shape == (2, 1, 16, 64)
+
+
+def test_norm_refuses_outputs_on_each_other_and_across_inputs(qg):
+    """Only an element's own place may be written over: by residual_out for residual, by h
+    for y, or for another input of the same layout and type."""
+    def call(tokens=4, width=64, f32=0, y=M, residual=2 * M, post=3 * M, post_bias=None, gate=None, stride=0, pre=4 * M,
+             pre_bias=None, out=5 * M, h=6 * M, kind=0):
+        a = Norm(kind, tokens, width, f32, y, residual, post, post_bias, gate, stride, pre, pre_bias, 1.0, 1e-6, out, h)
+        return qg.lib().qgemm_residual_norm(C.byref(a), None)
+
+    row, whole = 64 * 2, 4 * 64 * 2
+    for kw in (dict(h=5 * M), dict(h=5 * M + row), dict(h=5 * M - row), dict(f32=1, h=5 * M + 2 * whole - 16),  # on one another
+               dict(h=M + row), dict(h=M - row), dict(out=2 * M + 16), dict(f32=1, out=2 * M - 16),         # shifted
+               dict(f32=1, h=2 * M), dict(f32=1, out=M), dict(y=None, post=None, f32=1, h=2 * M),          # another type
+               dict(out=3 * M), dict(h=4 * M + 112), dict(h=3 * M - whole + 16),                           # weights
+               dict(tokens=1, out=4 * M), dict(tokens=1, h=3 * M), dict(kind=1, post_bias=7 * M, out=7 * M), dict(kind=1, pre_bias=7 * M, h=7 * M),
+               dict(gate=7 * M, h=7 * M), dict(gate=7 * M, stride=72, out=7 * M), dict(gate=7 * M, stride=64, h=7 * M + row)):
+        assert call(**kw) == qg.ERR_INVALID_ARG, kw
+        assert b"overlap" in qg.lib().qgemm_last_error_message(), kw
