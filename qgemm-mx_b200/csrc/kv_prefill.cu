@@ -527,10 +527,11 @@ k_kv_prefill(const KvAttnArgs a) {
             }
             const float mx = fmaxf(fmaxf(mxa[0], mxa[1]), fmaxf(mxa[2], mxa[3]));
             // m moves, by a whole number, when a weight would pass 2^15, and at a
-            // row's first visible token (fresh: nothing is summed yet)
+            // row's first visible token (fresh: nothing is summed yet).  Rounded down,
+            // so that the largest weight is 2^10 at least, as kv_attention.cuh says.
             const bool move = mx > kKvGrow || (fresh && mx > -INFINITY);
             if (__any_sync(0xFFFFFFFFu, move)) {
-              const float by = move ? fminf(ceilf(mx) - kKvTop, 1e30f) : 0.0f;
+              const float by = move ? fminf(floorf(mx) - kKvTop, 1e30f) : 0.0f;
               const bool scale = move && !fresh;  // by > 0
               const float al = pow2f(scale ? -(int)fminf(by, 126.0f) : 0);
               if (move) fresh = false;

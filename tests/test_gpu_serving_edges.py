@@ -3,7 +3,7 @@ and counts near 2^31, block ids outside the pool, calls on other streams."""
 import pytest
 import serving_ref as R
 import torch
-from test_gpu_kv_attention import make
+from test_gpu_kv_attention import check, make
 from test_gpu_kv_cache import check_plan, i32, make_step
 
 pytestmark = pytest.mark.gpu
@@ -146,6 +146,20 @@ def test_a_workspace_belongs_to_the_calls_stream(qg, cuda, new):
         s.synchronize()
         assert torch.equal(out, want)
         del taken
+
+
+@pytest.mark.parametrize("lens,new,block,heads,group,d,seed,window,causal", [
+    ([3, 3, 3, 4, 3, 3, 3, 4], [3] * 8, 32, 4, 16, 64, 795860, 0, False),
+    ([3, 276, 26, 178], [162, 276, 26, 178], 128, 8, 4, 64, 183772, 0, False),
+    ([408, 29, 399, 3], [408, 73, 399, 263], 16, 4, 12, 128, 303701, 274, True),
+    ([2305, 373, 1611, 4, 836, 1224, 1684, 1454, 2083], [2, 4, 5, 4, 5, 2, 8, 7, 0], 128, 3, 16, 64, 736382, 297, True),
+    ([2, 9, 40], [1, 1, 1], 16, 8, 8, 128, 5, 0, True),
+])
+def test_small_weights_beside_a_codes_zero(qg, cuda, lens, new, block, heads, group, d, seed, window, causal):
+    """INT8 values that only small weights reach, the largest weight's code being 0: the
+    step of an f16 weight is 2^-35 of the largest in both kernels."""
+    check(qg, *make(qg, 1, lens, new, block, heads, group, d, seed, scales=(100, 130)), max(new), window=window,
+          causal=causal)
 
 
 @pytest.mark.parametrize("kv", [0, 1])
