@@ -137,7 +137,7 @@ struct KvLine {
   // 18.5 us, against 101 and 19.9 with 2, 97 and 19.2 with 8, 104 and 29.4 with 1.
   // Of the prefill kernel's 128 tokens a start weighs three: 13 decoding requests and 3
   // prompt chunks of up to 512 tokens 120 us, 132 with 1, 122 with 5.  (All of them
-  // calls behind one another in a CUDA graph.)
+  // calls behind one another in a CUDA graph, in one run.)
   static constexpr int kStart = TL == 4 ? 4 : 3;
   int h0, slope, groups;
   __host__ __device__ __forceinline__ KvLine(const KvAttnArgs& a, const KvRequest& q) {
